@@ -86,6 +86,22 @@ SIGNATURES = [
   ("af_attn_decode_noalloc", c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                      c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_int, c_void_p,
                                      c_void_p]),
+  ("af_sample", c_int, [c_void_p, c_int, ctypes.c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                        c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p]),
+  ("af_attn_tree_scratch_bytes", c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+  ("af_attn_tree", c_int, [c_void_p, c_int, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_int, c_void_p,
+                           c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float,
+                           c_float, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t,
+                           c_void_p, c_void_p]),
+  ("af_kv_fork", c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                         c_void_p]),
+  ("af_kv_reserve_scratch_bytes", c_size_t, [c_int, c_int]),
+  ("af_kv_reserve", c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                            c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
+  ("af_kv_free", c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                         c_void_p]),
+  ("af_kv_compact", c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                            c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
 ]
 
 W_I8, W_F16, W_I4G32 = 0, 1, 2

@@ -13,6 +13,8 @@ enum AfDevErr : int {
   AF_DEV_BAD_TOKEN = 1,     // embedding index outside [0, vocab)
   AF_DEV_BAD_POS = 2,       // decode position outside [0, max_len)
   AF_DEV_WAIT_TIMEOUT = 3,  // a bounded spin-wait gave up
+  AF_DEV_NO_PAGES = 4,      // fewer free pages than a reservation needs
+  AF_DEV_BAD_SLOT = 5,      // a cache slot, or a path through a tree, that cannot be
 };
 
 AF_DEV void af_set_err(int* err, int code) {

@@ -285,6 +285,80 @@ cudaError_t attn_prefill_with_q(const AttnPrefillArgs& a, const __half* qbuf, cu
 bool attn_prefill_tc_ok(const AttnPrefillArgs& a);
 cudaError_t attn_prefill_tc_launch(const AttnPrefillArgs& a, const __half* qbuf, cudaStream_t st);
 
+// One token per row of logits (sample.cu). Settings: per row where the pointer is given, else the scalar.
+struct SampleArgs {
+  const void* logits = nullptr;        // [R][ld], dtype 0 fp32, 1 fp16, 2 bf16
+  int dtype = 0;
+  long long ld = 0;
+  int R = 0, V = 0;
+  const float* u = nullptr;            // [R] uniform numbers in [0, 1)
+  const float* temperature = nullptr;  // [R]; <= 0: the first largest logit
+  const int* top_k = nullptr;          // [R]; <= 0 or >= V: off
+  const float* top_p = nullptr;        // [R]; <= 0 or >= 1: off
+  const float* min_p = nullptr;        // [R]; <= 0: off
+  float temperature_s = 1.f, top_p_s = 1.f, min_p_s = 0.f;
+  int top_k_s = 0;
+  int* tok = nullptr;                  // [R]; -1 for a row without a finite or +inf logit
+  float* logp = nullptr;               // [R] log-probability among the kept tokens, or null
+};
+cudaError_t sample_launch(const SampleArgs& a, cudaStream_t st, bool pdl);
+
+// Attention of a tree of drafted tokens over a paged cache (attn_tree.cu)
+constexpr int TREE_MAX_NODES = 256;
+struct AttnTreeArgs {
+  const float* qkv = nullptr;          // [B * T][ld_qkv] fp32: q (H * dh) | k (KV * dh) | v (KV * dh)
+  int ld_qkv = 0;
+  __half* kc = nullptr;                // [P][KV][page][dh], pages page_stride elements apart
+  __half* vc = nullptr;
+  long long page_stride = 0;
+  int P = 0, page = 0, W = 0;
+  const int* table = nullptr;          // [B][W] page of each run of `page` rows
+  const int* lens = nullptr;           // [B] rows before the tree
+  const int* nodes = nullptr;          // [B] live nodes (null: T)
+  const int* depth = nullptr;          // [B][T] node depth (null: t)
+  const int* mask = nullptr;           // [B][T][mask_words] visible nodes, 32 a word (null: u <= t)
+  int mask_words = 0;
+  const __half* cos_t = nullptr;       // [rope_rows][dh] (null: no RoPE)
+  const __half* sin_t = nullptr;
+  int rope_rows = 0;
+  const __half* qn_g = nullptr;        // optional per-head RMSNorm
+  const __half* kn_g = nullptr;
+  float qn_floor = 0.f, kn_floor = 0.f;
+  __half* out = nullptr;               // [B * T][ld_out]
+  int ld_out = 0;
+  int B = 0, T = 1, H = 0, KV = 0, dh = 0;
+  float scale = 0.f;
+  void* scratch = nullptr;             // attn_tree_scratch_bytes
+  size_t scratch_bytes = 0;
+  int* err = nullptr;
+  __half* q = nullptr;                 // set by the launcher: [B][KV][T * G][dh]
+};
+size_t attn_tree_scratch_bytes(int B, int T, int H, int KV, int dh);
+cudaError_t attn_tree_launch(const AttnTreeArgs& a, cudaStream_t st, bool pdl);
+
+// Page bookkeeping of a cache pool [layers][2][P][KV][page][row16 * 16 bytes] (kv_pages.cu)
+struct KvPagesArgs {
+  void* pool = nullptr;
+  int layers = 0, P = 0, KV = 0, page = 0, row16 = 0;
+  int* table = nullptr;                // [S][W], -1: no page
+  int S = 0, W = 0;
+  int* lens = nullptr;                 // [S]
+  int* refs = nullptr;                 // [P] slots that hold the page
+  const int* slots = nullptr;          // [n] distinct (fork: the targets)
+  const int* rows = nullptr;           // [n] free: rows kept (null: 0); fork: the sources; reserve: rows wanted; compact: path lengths
+  int n = 0;
+  const int* path = nullptr;           // compact: [n][D] node of each accepted row, rising
+  int D = 0;
+  int* lens_out = nullptr;             // compact: [S]
+  int* scratch = nullptr;              // reserve: kv_reserve_scratch_bytes
+  int* err = nullptr;
+};
+cudaError_t kv_free_launch(const KvPagesArgs& a, cudaStream_t st);
+cudaError_t kv_fork_launch(const KvPagesArgs& a, cudaStream_t st);
+size_t kv_reserve_scratch_bytes(int n, int P);
+cudaError_t kv_reserve_launch(const KvPagesArgs& a, cudaStream_t st);
+cudaError_t kv_compact_launch(const KvPagesArgs& a, cudaStream_t st);
+
 // ---- generic graph ops (graph_ops.cu): what `compile(graph)` lowers nodes onto when no fused kernel
 // covers them. fp32 values, fp16-rounded matmul operands, rank <= GRAPH_MAX_RANK.
 constexpr int GRAPH_MAX_RANK = 5;

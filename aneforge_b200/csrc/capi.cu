@@ -210,4 +210,80 @@ int af_attn_decode(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t* vc, con
   return rc_of(af::attn_decode_launch(a, static_cast<cudaStream_t>(stream), false), "af_attn_decode");
 }
 
+int af_sample(const void* logits, int dtype, long long ld, int rows, int vocab, const float* u, const float* temperature,
+              const int* top_k, const float* top_p, const float* min_p, float temperature_s, int top_k_s, float top_p_s,
+              float min_p_s, int* tok, float* logp, void* stream) {
+  af::SampleArgs a;
+  a.logits = logits; a.dtype = dtype; a.ld = ld; a.R = rows; a.V = vocab; a.u = u;
+  a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+  a.temperature_s = temperature_s; a.top_k_s = top_k_s; a.top_p_s = top_p_s; a.min_p_s = min_p_s;
+  a.tok = tok; a.logp = logp;
+  return rc_of(af::sample_launch(a, static_cast<cudaStream_t>(stream), false), "af_sample");
+}
+
+size_t af_attn_tree_scratch_bytes(int b, int t, int h, int kv, int dh) { return af::attn_tree_scratch_bytes(b, t, h, kv, dh); }
+
+int af_attn_tree(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t* vc, long long page_stride, int n_pages, int page,
+                 const int* table, int table_width, const int* lens, const int* nodes, const int* depth, const int* mask,
+                 int mask_words, const uint16_t* cos_t, const uint16_t* sin_t, int rope_rows, const uint16_t* qn,
+                 const uint16_t* kn, float qn_floor, float kn_floor, uint16_t* out, int ld_out, int b, int t, int h, int kv,
+                 int dh, float scale, void* scratch, size_t scratch_bytes, int* err, void* stream) {
+  af::AttnTreeArgs a;
+  a.qkv = qkv; a.ld_qkv = ld_qkv;
+  a.kc = reinterpret_cast<__half*>(kc); a.vc = reinterpret_cast<__half*>(vc);
+  a.page_stride = page_stride; a.P = n_pages; a.page = page; a.W = table_width;
+  a.table = table; a.lens = lens; a.nodes = nodes; a.depth = depth; a.mask = mask; a.mask_words = mask_words;
+  a.cos_t = reinterpret_cast<const __half*>(cos_t); a.sin_t = reinterpret_cast<const __half*>(sin_t);
+  a.rope_rows = rope_rows;
+  a.qn_g = reinterpret_cast<const __half*>(qn); a.kn_g = reinterpret_cast<const __half*>(kn);
+  a.qn_floor = qn_floor; a.kn_floor = kn_floor;
+  a.out = reinterpret_cast<__half*>(out); a.ld_out = ld_out;
+  a.B = b; a.T = t; a.H = h; a.KV = kv; a.dh = dh; a.scale = scale;
+  a.scratch = scratch; a.scratch_bytes = scratch_bytes; a.err = err;
+  return rc_of(af::attn_tree_launch(a, static_cast<cudaStream_t>(stream), false), "af_attn_tree");
+}
+
+static af::KvPagesArgs pages_of(int* table, int slots_total, int width, int* lens, int* refs, int n_pages, int page,
+                                const int* slots, const int* rows, int n, int* err) {
+  af::KvPagesArgs a;
+  a.table = table; a.S = slots_total; a.W = width; a.lens = lens; a.refs = refs; a.P = n_pages; a.page = page;
+  a.slots = slots; a.rows = rows; a.n = n; a.err = err;
+  return a;
+}
+
+int af_kv_fork(int* table, int slots_total, int width, int* lens, int* refs, int n_pages, int page, const int* src,
+               const int* dst, int n, int* err, void* stream) {
+  return rc_of(af::kv_fork_launch(pages_of(table, slots_total, width, lens, refs, n_pages, page, dst, src, n, err),
+                                  static_cast<cudaStream_t>(stream)), "af_kv_fork");
+}
+
+int af_kv_free(int* table, int slots_total, int width, int* lens, int* refs, int n_pages, int page, const int* slots,
+               const int* keep, int n, int* err, void* stream) {
+  return rc_of(af::kv_free_launch(pages_of(table, slots_total, width, lens, refs, n_pages, page, slots, keep, n, err),
+                                  static_cast<cudaStream_t>(stream)), "af_kv_free");
+}
+
+size_t af_kv_reserve_scratch_bytes(int n, int n_pages) { return n < 0 || n_pages < 0 ? 0 : af::kv_reserve_scratch_bytes(n, n_pages); }
+
+int af_kv_reserve(void* pool, int layers, int kv, int row_bytes, int* table, int slots_total, int width, int* lens,
+                  int* refs, int n_pages, int page, const int* slots, const int* rows, int n, void* scratch,
+                  size_t scratch_bytes, int* err, void* stream) {
+  af::KvPagesArgs a = pages_of(table, slots_total, width, lens, refs, n_pages, page, slots, rows, n, err);
+  a.pool = pool; a.layers = layers; a.KV = kv; a.row16 = row_bytes / 16;
+  a.scratch = static_cast<int*>(scratch);
+  if (row_bytes % 16 || scratch_bytes < af_kv_reserve_scratch_bytes(n, n_pages))
+    return rc_of(cudaErrorInvalidValue, "af_kv_reserve: row bytes or scratch");
+  return rc_of(af::kv_reserve_launch(a, static_cast<cudaStream_t>(stream)), "af_kv_reserve");
+}
+
+int af_kv_compact(void* pool, int layers, int kv, int row_bytes, int n_pages, int page, int* table, int slots_total,
+                  int width, int* lens, const int* slots, const int* path, int path_ld, const int* n_path, int n,
+                  int* lens_out, int* err, void* stream) {
+  af::KvPagesArgs a = pages_of(table, slots_total, width, lens, nullptr, n_pages, page, slots, n_path, n, err);
+  a.pool = pool; a.layers = layers; a.KV = kv; a.row16 = row_bytes / 16;
+  a.path = path; a.D = path_ld; a.lens_out = lens_out;
+  if (row_bytes % 16) return rc_of(cudaErrorInvalidValue, "af_kv_compact: row bytes");
+  return rc_of(af::kv_compact_launch(a, static_cast<cudaStream_t>(stream)), "af_kv_compact");
+}
+
 }  // extern "C"

@@ -965,8 +965,9 @@ static int check_err(Program& p) {
     return -1;
   }
   if (h != 0) {
-    static const char* names[] = {"ok", "token id out of range", "decode position out of range", "bounded wait timed out"};
-    set_error(std::string("kernel reported error ") + std::to_string(h) + " (" + (h > 0 && h < 4 ? names[h] : "?") + ")");
+    static const char* names[] = {"ok", "token id out of range", "decode position out of range", "bounded wait timed out",
+                                  "cache pages exhausted", "bad cache slot or path"};
+    set_error(std::string("kernel reported error ") + std::to_string(h) + " (" + (h > 0 && h < 6 ? names[h] : "?") + ")");
     cudaMemsetAsync(p.d_err, 0, 4, p.stream);
     cudaStreamSynchronize(p.stream);
     return -2;

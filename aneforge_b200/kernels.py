@@ -237,3 +237,194 @@ def gemm_tc(x, tiles, scales, N, K, wf=R.W_I8, bias=None, epi=R.EPI_F32, y=None)
   R.check(R.lib().af_gemm_tc(wf, epi, _p(x), x.stride(0), _p(tiles), _p(scales), _p(bias), _p(y), y.stride(0), M, N, K,
                              _stream(x)), "af_gemm_tc")
   return y
+
+
+_SAMPLE_DT = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
+def _i32(t, shape, name):
+  import torch
+  _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and tuple(t.shape) == tuple(shape),
+        f"{name} must be a contiguous int32 CUDA tensor of shape {tuple(shape)}")
+  return t.data_ptr()
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+  """One token per row of logits [R, V] (fp32, fp16 or bf16, rows any stride apart), drawn with the uniform numbers
+  u [R] in [0, 1): temperature, then the top_k largest logits (ties with the last stay), of these the most
+  probable until their mass reaches top_p (ties: lowest index first), of these the ones at least min_p as
+  probable as the best; one draw in the order of the vocabulary. Each setting is a number or a CUDA tensor [R]
+  (fp32; top_k int32); 0 (or top_p 1) turns it off, temperature 0 takes the first largest logit. Returns
+  (tokens int32 [R], log-probabilities among the kept tokens fp32 [R]); -1 and -inf for a row that is all -inf
+  or NaN. `out` = the two outputs, preallocated."""
+  import torch
+  _need(logits.is_cuda and logits.dim() == 2 and logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+        "logits must be a 2-D CUDA tensor whose rows are contiguous")
+  dt = _SAMPLE_DT.get(str(logits.dtype))
+  _need(dt is not None, "logits must be fp32, fp16 or bf16")
+  n, V = logits.shape
+  _need(V <= 1 << 24, "at most 2^24 logits in a row")
+  ld = logits.stride(0) if n > 1 else V
+  _need(ld >= V, "rows of logits must not overlap")
+  _need(u.is_cuda and u.dtype == torch.float32 and u.is_contiguous() and u.shape == (n,), "u must be fp32 [R] on the GPU")
+  ptr, val = [], []
+  for x, name, want in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
+                        (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
+    if isinstance(x, torch.Tensor):
+      _need(x.is_cuda and x.dtype == want and x.is_contiguous() and x.shape == (n,), f"{name} must be {want} [R] on the GPU")
+      ptr.append(x.data_ptr()); val.append(0)
+    else:
+      _need(x == x and abs(x) != float("inf"), f"{name} must be finite")
+      ptr.append(0); val.append(x)
+  if out is None:
+    out = torch.empty((n,), dtype=torch.int32, device=u.device), torch.empty((n,), dtype=torch.float32, device=u.device)
+  else:
+    _need(out[0].dtype == torch.int32 and out[1].dtype == torch.float32 and all(o.shape == (n,) and o.is_contiguous() for o in out),
+          "out must be (int32 [R], fp32 [R])")
+  R.check(R.lib().af_sample(logits.data_ptr(), dt, ld, n, V, u.data_ptr(), *ptr, float(val[0]), int(val[1]), float(val[2]),
+                            float(val[3]), out[0].data_ptr(), out[1].data_ptr(), _stream(logits)), "af_sample")
+  return out
+
+
+def tree_layout(parents):
+  """Depths [T] and visibility masks [T, ceil(T / 32)] (int32, bit u of word w: node 32 w + u) of a tree given by
+  each node's parent (-1: hangs on the prefix; parents come before their children), as numpy arrays."""
+  T = len(parents)
+  depth = np.zeros(T, np.int32)
+  mask = np.zeros((T, -(-T // 32)), np.uint32)
+  for t, p in enumerate(parents):
+    _need(-1 <= p < t, f"node {t}: parent {p} must be -1 or an earlier node")
+    if p >= 0:
+      depth[t] = depth[p] + 1
+      mask[t] = mask[p]
+    mask[t, t >> 5] |= np.uint32(1 << (t & 31))
+  return depth, mask.view(np.int32)
+
+
+def attn_tree_scratch(B, T, H, KV, dh, device=None):
+  """Workspace of `attn_tree` for these sizes; it may serve any number of calls of one stream."""
+  import torch
+  return torch.zeros((max(1, R.load_library().af_attn_tree_scratch_bytes(B, T, H, KV, dh)),), dtype=torch.uint8,
+                     device=device or "cuda")
+
+
+def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=None, depth=None, nodes=None, qn=None, kn=None,
+              qn_floor=0.0, kn_floor=0.0, scratch=None, err=None, out=None):
+  """Attention of T drafted tokens (nodes of a tree) for each of B sequences over a paged cache. qkv [B * T,
+  (H + 2 KV) dh] fp32; kc / vc [P, KV, page, dh] fp16 (pages any stride apart); table [B, W] int32: the page of
+  each run of `page` rows; lens [B] int32: the rows before the tree. Node t becomes cache row lens + t (k and v
+  are written there), its rotary position is lens + depth[b, t] (default t); it sees the rows before lens and the
+  nodes set in mask [B, T, ceil(T / 32)] (int32 bits, see `tree_layout`; default: a chain). T = 1 is the ordinary
+  decode step. nodes [B]: live nodes of each sequence. lens is left as it is (`kv_compact` advances it). Returns
+  fp16 [B * T, H * dh], zeros for nodes that see nothing or are not live. err: int32 [1], zero: gets the device
+  error code of a node without a page or rotary position."""
+  import torch
+  _need(qkv.is_cuda and qkv.dtype == torch.float32 and qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be fp32 [B * T, cols] on the GPU")
+  _need(table.dim() == 2, "table must be int32 [B, W]")
+  B, W = table.shape
+  _need(KV >= 1 and H % KV == 0 and qkv.shape[1] >= (H + 2 * KV) * dh, "qkv needs (H + 2 KV) dh columns, H a multiple of KV")
+  _need(B >= 1 and qkv.shape[0] % B == 0 and qkv.shape[0] >= B, "qkv needs the same number of rows for each sequence of the table")
+  T = qkv.shape[0] // B
+  _need(T <= 256, "at most 256 nodes")
+  _need(dh in (16, 32, 64, 128), "head dims 16, 32, 64 and 128")
+  _need(kc.shape == vc.shape and kc.dim() == 4 and kc.dtype == vc.dtype == torch.float16 and kc.is_cuda and vc.is_cuda,
+        "kc / vc must be fp16 [P, KV, page, dh] on the GPU")
+  P, kvh, page, d = kc.shape
+  _need(kvh == KV and d == dh, "kc / vc must be fp16 [P, KV, page, dh] on the GPU")
+  ps = kc.stride(0) if P > 1 else KV * page * dh
+  _need(kc.stride()[1:] == (page * dh, dh, 1) and vc.stride() == kc.stride() and ps >= KV * page * dh and ps % 8 == 0,
+        "kc / vc pages must be contiguous, and alike")
+  pt, pl = _i32(table, (B, W), "table"), _i32(lens, (B,), "lens")
+  pn = 0 if nodes is None else _i32(nodes, (B,), "nodes")
+  pd = 0 if depth is None else _i32(depth, (B, T), "depth")
+  words = (T + 31) // 32
+  pm = 0 if mask is None else _i32(mask, (B, T, words), "mask")
+  rows = 0
+  if cos_t is not None:
+    rows = cos_t.shape[0]
+    _need(cos_t.shape == sin_t.shape == (rows, dh) and cos_t.dtype == sin_t.dtype == torch.float16 and cos_t.is_contiguous()
+          and sin_t.is_contiguous() and cos_t.is_cuda and sin_t.is_cuda, "cos_t / sin_t must be fp16 [rows, dh] on the GPU")
+  for g, name in ((qn, "qn"), (kn, "kn")):
+    _need(g is None or (g.is_cuda and g.dtype == torch.float16 and g.shape == (dh,) and g.is_contiguous()), f"{name} must be fp16 [dh] on the GPU")
+  if out is None:
+    out = torch.empty((B * T, H * dh), dtype=torch.float16, device=qkv.device)
+  else:
+    _need(out.is_cuda and out.dtype == torch.float16 and out.shape == (B * T, H * dh) and out.stride(1) == 1, "out must be fp16 [B * T, H * dh]")
+  if scratch is None:
+    scratch = attn_tree_scratch(B, T, H, KV, dh, qkv.device)
+  R.check(R.lib().af_attn_tree(qkv.data_ptr(), qkv.stride(0), kc.data_ptr(), vc.data_ptr(), ps, P, page, pt, W, pl, pn, pd, pm,
+                               words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), float(qn_floor), float(kn_floor),
+                               out.data_ptr(), out.stride(0), B, T, H, KV, dh, float(scale), scratch.data_ptr(),
+                               scratch.numel(), _p(err), _stream(qkv)), "af_attn_tree")
+  return out
+
+
+def _book(table, lens, refs, slots):
+  import torch
+  _need(table.dim() == 2 and lens.dim() == 1 and slots.dim() == 1, "table [S, W], lens [S] and slots [n] are wanted")
+  S, W = table.shape
+  n = slots.shape[0]
+  _need(n <= 1024, "at most 1024 slots a call")
+  pr = 0
+  if refs is not None:
+    _need(refs.dim() == 1, "refs must be int32 [P]")
+    pr = _i32(refs, refs.shape, "refs")
+  return _i32(table, (S, W), "table"), S, W, _i32(lens, (S,), "lens"), pr, _i32(slots, (n,), "slots"), n
+
+
+def _pool(pool):
+  import torch
+  _need(pool.is_cuda and pool.dim() == 6 and pool.shape[1] == 2 and pool.is_contiguous() and pool.element_size() == 2,
+        "pool must be a contiguous 16-bit CUDA tensor [layers, 2, P, KV, page, dh]")
+  L, _, P, KV, page, dh = pool.shape
+  _need(2 * dh % 16 == 0, "dh must be a multiple of 8")
+  return L, P, KV, page, 2 * dh
+
+
+def kv_fork(table, lens, refs, src, dst, page, err=None):
+  """Slots dst[i] become copies of slots src[i]: they give back the pages they hold and share the ones that src
+  fills (counted in refs [P]); no row moves until `kv_reserve` makes a shared page writable. All int32 on the GPU;
+  table [S, W], lens [S]. The dst are distinct and none is a src."""
+  pt, S, W, pl, pr, pd, n = _book(table, lens, refs, dst)
+  _need(page >= 1, "page must be positive")
+  R.check(R.lib().af_kv_fork(pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src"), pd, n, _p(err), _stream(table)),
+          "af_kv_fork")
+
+
+def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
+  """Rows [lens, lens + rows[i]) of each slot get pages of the slot's own: free ones, lowest number first, and
+  copies (in every layer of pool [layers, 2, P, KV, page, dh]) of a shared page that rows are appended to."""
+  import torch
+  pt, S, W, pl, pr, ps, n = _book(table, lens, refs, slots)
+  L, P, KV, page, rb = _pool(pool)
+  _need(refs.shape[0] == P, "refs must have an entry for each page of the pool")
+  if scratch is None:
+    scratch = torch.empty((R.lib().af_kv_reserve_scratch_bytes(n, P),), dtype=torch.uint8, device=pool.device)
+  R.check(R.lib().af_kv_reserve(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows"), n,
+                                scratch.data_ptr(), scratch.numel(), _p(err), _stream(pool)), "af_kv_reserve")
+
+
+def kv_free(table, lens, refs, slots, page, keep=None, err=None):
+  """Gives back what the slots hold past keep[i] rows (default: everything)."""
+  pt, S, W, pl, pr, ps, n = _book(table, lens, refs, slots)
+  _need(page >= 1, "page must be positive")
+  R.check(R.lib().af_kv_free(pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep"), n,
+                             _p(err), _stream(table)), "af_kv_free")
+
+
+def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
+  """The rows lens + path[i, j], j < n_path[i], of each slot move to lens + j in every layer's K and V: the accepted
+  path [n, D] through a drafted tree (node numbers, rising) becomes part of the prefix. Returns the new lengths:
+  lens with n_path added to the listed slots (a new tensor, or lens_out)."""
+  import torch
+  pt, S, W, pl, _, ps, n = _book(table, lens, None, slots)
+  L, P, KV, page, rb = _pool(pool)
+  _need(path.dim() == 2, "path must be int32 [n, D]")
+  D = path.shape[1]
+  if lens_out is None:
+    lens_out = torch.empty_like(lens)
+  _need(lens_out.data_ptr() != lens.data_ptr(), "lens_out must be another buffer than lens")
+  R.check(R.lib().af_kv_compact(pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path"), D,
+                                _i32(n_path, (n,), "n_path"), n, _i32(lens_out, (S,), "lens_out"), _p(err), _stream(pool)),
+          "af_kv_compact")
+  return lens_out

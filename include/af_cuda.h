@@ -238,6 +238,60 @@ int af_attn_decode_noalloc(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t*
                            int kv, int dh, int m, int n_split, float scale, float kv_c, int expand, int* err,
                            void* stream);
 
+/* One token per row of logits [rows][ld] (dtype 0 fp32, 1 fp16, 2 bf16; ld >= vocab, vocab <= 2^24),
+ * drawn with the given uniform numbers u [rows] in [0, 1): the device form of LlamaPrefill._sample
+ * (aneforge/llm.py:407-419) with min-p added. The settings are per row where their pointer is given,
+ * else the scalar: temperature (<= 0: the first largest logit), top_k (<= 0 or >= vocab: off; ties with
+ * the k-th stay), top_p (outside (0, 1): off; the token that crosses it stays), min_p (<= 0: off).
+ * Weights are whole numbers, so equal inputs give equal tokens however the work is split. tok [rows]:
+ * -1 for a row whose logits are all -inf or NaN; logp [rows] (may be NULL): the token's log-probability
+ * among the kept ones. */
+int af_sample(const void* logits, int dtype, long long ld, int rows, int vocab, const float* u, const float* temperature,
+              const int* top_k, const float* top_p, const float* min_p, float temperature_s, int top_k_s, float top_p_s,
+              float min_p_s, int* tok, float* logp, void* stream);
+
+/* Attention of t drafted tokens (nodes of a tree) per sequence over a paged cache: extends af_attn_decode
+ * (the attention part of _attn_decode, aneforge/llm.py:214-237) to trees and pages. kc / vc
+ * [n_pages][kv][page][dh] fp16, page_stride elements between pages; table [b][table_width] names the
+ * page of each `page` rows; lens [b] rows come before the tree. Node t of sequence b (qkv row b * T + t,
+ * fp32) is appended as cache row lens[b] + t with its rotary position at lens[b] + depth[b][t], and sees
+ * the prefix and the nodes whose bit is set in mask [b][t][mask_words]. NULL: nodes = t for all, depth =
+ * node number, mask = the nodes up to itself, cos_t / sin_t = no RoPE, qn / kn = no per-head norm. A
+ * node that sees nothing and nodes from nodes[b] on give zeros. dh 16, 32, 64 or 128; t <= 256. lens is
+ * not changed. A row without a page, or a position past rope_rows, records AF_DEV_BAD_POS in err (may be
+ * NULL) and is left out. Scratch: af_attn_tree_scratch_bytes, zero before the first call, left so that
+ * the next call can use it. */
+size_t af_attn_tree_scratch_bytes(int b, int t, int h, int kv, int dh);
+int af_attn_tree(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t* vc, long long page_stride, int n_pages, int page,
+                 const int* table, int table_width, const int* lens, const int* nodes, const int* depth, const int* mask,
+                 int mask_words, const uint16_t* cos_t, const uint16_t* sin_t, int rope_rows, const uint16_t* qn,
+                 const uint16_t* kn, float qn_floor, float kn_floor, uint16_t* out, int ld_out, int b, int t, int h, int kv,
+                 int dh, float scale, void* scratch, size_t scratch_bytes, int* err, void* stream);
+
+/* Pages of a cache pool [layers][2][n_pages][kv][page][row_bytes] (no counterpart in the reference, whose
+ * caches are one block per sequence). Slot s holds pages table[s][0..width) (-1: none), lens[s] rows of
+ * them filled; refs[p] slots hold page p. At most 1024 slots a call, all distinct; a slot out of range or
+ * listed twice is left out and recorded in err (may be NULL).
+ *   af_kv_fork     dst[i] gives back its pages and shares the ones that src[i] fills; no dst is a src
+ *   af_kv_reserve  rows [lens, lens + rows[i]) of each slot become its own to write: missing pages are
+ *                  taken from the free ones, lowest first, and a shared page with rows in it is copied
+ *                  (in every layer) by all its holders but the last. Too few free pages: nothing is
+ *                  changed, AF_DEV_NO_PAGES. Scratch: af_kv_reserve_scratch_bytes
+ *   af_kv_free     gives back what lies past keep[i] rows (keep NULL: everything)
+ *   af_kv_compact  rows lens + path[i][j], j < n_path[i], move to lens + j in every layer (path rises),
+ *                  lens_out [slots_total] (another buffer than lens) = lens with n_path added */
+int af_kv_fork(int* table, int slots_total, int width, int* lens, int* refs, int n_pages, int page, const int* src,
+               const int* dst, int n, int* err, void* stream);
+size_t af_kv_reserve_scratch_bytes(int n, int n_pages);
+int af_kv_reserve(void* pool, int layers, int kv, int row_bytes, int* table, int slots_total, int width, int* lens,
+                  int* refs, int n_pages, int page, const int* slots, const int* rows, int n, void* scratch,
+                  size_t scratch_bytes, int* err, void* stream);
+int af_kv_free(int* table, int slots_total, int width, int* lens, int* refs, int n_pages, int page, const int* slots,
+               const int* keep, int n, int* err, void* stream);
+int af_kv_compact(void* pool, int layers, int kv, int row_bytes, int n_pages, int page, int* table, int slots_total,
+                  int width, int* lens, const int* slots, const int* path, int path_ld, const int* n_path, int n,
+                  int* lens_out, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

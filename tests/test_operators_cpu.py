@@ -1,0 +1,78 @@
+"""Refusals of the sampling, tree-attention and cache-page entry points, and the tree helper (no GPU)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from aneforge_b200 import kernels as K
+
+
+def test_tree_layout():
+  depth, mask = K.tree_layout([-1, 0, 0, 1, -1])
+  assert depth.tolist() == [0, 1, 1, 2, 0]
+  assert mask[:, 0].tolist() == [0b1, 0b11, 0b101, 0b1011, 0b10000]
+  depth, mask = K.tree_layout(list(range(-1, 69)))
+  assert depth[-1] == 69 and mask.shape == (70, 3) and mask.dtype == np.int32
+  assert mask.view(np.uint32)[63].tolist() == [0xFFFFFFFF, 0xFFFFFFFF, 0] and mask.view(np.uint32)[69, 2] == 0b111111
+  for bad in ([0], [-1, 1], [-2], [-1, 0, 5]):
+    with pytest.raises(ValueError):
+      K.tree_layout(bad)
+
+
+def test_host_tensors_are_refused():
+  f, i = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
+  with pytest.raises(ValueError):
+    K.sample(f, torch.zeros(2))
+  with pytest.raises(ValueError):
+    K.attn_tree(torch.zeros(2, 3 * 64), torch.zeros(4, 1, 8, 64).half(), torch.zeros(4, 1, 8, 64).half(), i.view(2, 1), i, None,
+                None, 1, 1, 64, 1.0)
+  with pytest.raises(ValueError):
+    K.kv_fork(i.view(2, 1), i, i, i, i, 8)
+  with pytest.raises(ValueError):
+    K.kv_free(i.view(2, 1), i, i, i, 8)
+  with pytest.raises(ValueError):
+    K.kv_reserve(torch.zeros(1, 2, 2, 1, 8, 8).half(), i.view(2, 1), i, i, i, i)
+  with pytest.raises(ValueError):
+    K.kv_compact(torch.zeros(1, 2, 2, 1, 8, 8).half(), i.view(2, 1), i, i, i.view(2, 1), i)
+
+
+def test_native_entries_refuse_before_they_launch():
+  """Bad arguments give -1 and a message; none of these calls reaches the device."""
+  from aneforge_b200 import build
+  L = ctypes.CDLL(str(build.build()))
+  from aneforge_b200 import _runtime as R
+  for name, res, args in R.SIGNATURES:
+    getattr(L, name).restype, getattr(L, name).argtypes = res, args
+  p = 1 << 20                                              # never read
+  sample = lambda **k: L.af_sample(*[dict(dict(l=p, dt=0, ld=8, r=1, v=8, u=p, tok=p), **k)[x] for x in ("l", "dt", "ld", "r", "v", "u")],
+                                   None, None, None, None, 1.0, 0, 1.0, 0.0, dict(dict(tok=p), **k)["tok"], None, None)
+  for bad in (dict(l=None), dict(u=None), dict(tok=None), dict(v=0), dict(ld=7), dict(r=-1), dict(dt=3), dict(v=(1 << 24) + 1, ld=1 << 25)):
+    assert sample(**bad) == -1, bad
+    assert b"af_sample" in L.af_last_error()
+  base = dict(qkv=p, ld=192, kc=p, vc=p, ps=512, P=4, page=8, table=p, W=1, lens=p, words=1, rows=0, out=p, ldo=64, b=1, t=1, h=1,
+              kv=1, dh=64, scr=p, nb=1 << 30, cos=None, sin=None, mask=None)
+
+  def tree(**k):
+    a = dict(base, **k)
+    return L.af_attn_tree(a["qkv"], a["ld"], a["kc"], a["vc"], a["ps"], a["P"], a["page"], a["table"], a["W"], a["lens"], None, None,
+                          a["mask"], a["words"], a["cos"], a["sin"], a["rows"], None, None, 0.0, 0.0, a["out"], a["ldo"], a["b"],
+                          a["t"], a["h"], a["kv"], a["dh"], 1.0, a["scr"], a["nb"], None, None)
+
+  for bad in (dict(qkv=None), dict(kc=None), dict(kc=p + 2), dict(vc=p + 8), dict(table=None), dict(lens=None), dict(out=None), dict(scr=None),
+              dict(nb=3), dict(ld=191), dict(ldo=63), dict(ps=511), dict(ps=516), dict(P=0), dict(page=0), dict(W=0), dict(b=-1), dict(t=0),
+              dict(t=257), dict(h=0), dict(kv=0), dict(h=3, kv=2), dict(dh=48), dict(dh=256, ps=1 << 20, ld=1 << 12, ldo=1 << 12),
+              dict(cos=p), dict(cos=p, sin=p, rows=0), dict(mask=p, t=33, words=1)):
+    assert tree(**bad) == -1, bad
+  for n in (-1, 1025):
+    assert L.af_kv_fork(p, 4, 4, p, p, 8, 8, p, p, n, None, None) == -1
+    assert L.af_kv_free(p, 4, 4, p, p, 8, 8, p, None, n, None, None) == -1
+    assert L.af_kv_reserve(p, 1, 1, 128, p, 4, 4, p, p, 8, 8, p, p, n, p, 1 << 30, None, None) == -1
+  assert L.af_kv_fork(p, 4, 4, p, None, 8, 8, p, p, 1, None, None) == -1
+  assert L.af_kv_reserve(p, 1, 1, 120, p, 4, 4, p, p, 8, 8, p, p, 1, p, 1 << 30, None, None) == -1
+  assert L.af_kv_reserve(p, 1, 1, 128, p, 4, 4, p, p, 8, 8, p, p, 1, p, 8, None, None) == -1
+  assert L.af_kv_reserve(p + 2, 1, 1, 128, p, 4, 4, p, p, 8, 8, p, p, 1, p, 1 << 30, None, None) == -1
+  assert L.af_kv_compact(p, 1, 1, 128, 8, 8, p, 4, 4, p, p, p, 1, p, 1, p, None, None) == -1           # lens_out is lens
+  assert L.af_kv_compact(p, 1, 1, 128, 8, 8, p, 4, 4, p, p, p, 0, p, 1, p + 64, None, None) == -1
+  assert L.af_attn_tree_scratch_bytes(1, 0, 1, 1, 64) == 0 and L.af_attn_tree_scratch_bytes(1, 1, 3, 2, 64) == 0
+  assert L.af_kv_reserve_scratch_bytes(-1, 4) == 0
