@@ -331,9 +331,17 @@ struct AttnTreeArgs {
   void* scratch = nullptr;             // attn_tree_scratch_bytes
   size_t scratch_bytes = 0;
   int* err = nullptr;
-  __half* q = nullptr;                 // set by the launcher: [B][KV][T * G][dh]
+  // set by the launcher (pieces of scratch, and the tensor-core form's geometry)
+  __half* q = nullptr;                 // [B][KV][T * G][dh]
+  unsigned char* flags = nullptr;      // [B][KV][T] 1: the node's k or v is not finite
+  float* part = nullptr;               // [blocks][2][part_rows * (dh + 2)] partial O, (m, l)
+  int part_rows = 0, box_rows = 0, row_groups = 1, paged = 0, out16 = 0;
 };
 size_t attn_tree_scratch_bytes(int B, int T, int H, int KV, int dh);
+// the tensor-core form (attn_tree_tc.cu), after tree_append
+bool attn_tree_tc_ok(const AttnTreeArgs& a);
+cudaError_t attn_tree_tc_launch(AttnTreeArgs a, cudaStream_t st);
+int attn_tree_tc_blocks();
 cudaError_t attn_tree_launch(const AttnTreeArgs& a, cudaStream_t st, bool pdl);
 
 // Page bookkeeping of a cache pool [layers][2][P][KV][page][row16 * 16 bytes] (kv_pages.cu)

@@ -18,6 +18,7 @@
 #include "af_common.cuh"
 #include "af_kernels.h"
 #include "attn_common.cuh"
+#include "tree_common.cuh"
 
 namespace af {
 
@@ -29,13 +30,6 @@ AF_DEV int tree_page(const AttnTreeArgs& a, int b, int j) {
   return p >= 0 && p < a.P ? p : -1;
 }
 
-// prefix rows and live nodes of sequence b, cut to what the table can hold
-AF_DEV void tree_extent(const AttnTreeArgs& a, int b, int& len, int& nodes) {
-  len = min(max(__ldcg(a.lens + b), 0), a.W * a.page);
-  nodes = a.nodes ? min(max(__ldcg(a.nodes + b), 0), a.T) : a.T;
-  nodes = min(nodes, a.W * a.page - len);
-}
-
 // grid (B * T, ceil((H + KV) / 8)), a warp per head
 template <int DH>
 __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
@@ -45,7 +39,9 @@ __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
   const int y = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (y >= a.H + a.KV) return;
   const bool active = lane < HL::LANES;
+  // triggered after the wait: a dependent that starts now may read everything written before this kernel
   pdl_wait();
+  pdl_trigger();
   int len, nodes;
   tree_extent(a, b, len, nodes);
   if (t >= nodes) {
@@ -73,17 +69,25 @@ __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
   }
   const int kvh = y - a.H, j = len + t, p = tree_page(a, b, j);
   if (p < 0) {
-    if (lane == 0) af_set_err(a.err, AF_DEV_BAD_POS);
+    if (lane == 0) {
+      af_set_err(a.err, AF_DEV_BAD_POS);
+      a.flags[((size_t)b * a.KV + kvh) * a.T + t] = 0;
+    }
     return;
   }
   norm_rope_head_pre<DH>(v, lane, a.kn_g, a.kn_floor, rope, rc, rs);
   const size_t o = (size_t)p * a.page_stride + ((size_t)kvh * a.page + j % a.page) * DH + lane * EPL;
+  bool finite = true;
   if (active)
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
-      a.kc[o + e] = f2h(v[e]);
-      a.vc[o + e] = f2h(__ldcg(x + (size_t)(y + a.KV) * DH + lane * EPL + e));
+      const __half kh = f2h(v[e]), vh = f2h(__ldcg(x + (size_t)(y + a.KV) * DH + lane * EPL + e));
+      a.kc[o + e] = kh;
+      a.vc[o + e] = vh;
+      finite &= isfinite(h2f(kh)) && isfinite(h2f(vh));
     }
+  finite = __all_sync(0xffffffffu, finite);
+  if (lane == 0) a.flags[((size_t)b * a.KV + kvh) * a.T + t] = !finite;
 }
 
 // grid (ceil(T * G / 8), KV, B), a warp per query row: 32 keys at a time, a key per lane for the scores,
@@ -161,9 +165,26 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(AttnTreeArgs a) {
     for (int e = 0; e < EPL; ++e) out[lane * EPL + e] = f2h(acc[e] * il);
 }
 
+// scratch: q, flags, and for the tensor-core form two partial results a block (a pair that a block does
+// not have whole: one at the start of its run, one at the end)
+struct TreeScratch {
+  size_t flags, part, bytes;
+  int part_rows;
+};
+static TreeScratch tree_scratch(int B, int T, int H, int KV, int dh) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  const int R = T * (H / KV);
+  TreeScratch s;
+  s.flags = up((size_t)B * T * H * dh * 2);
+  s.part = s.flags + up((size_t)B * KV * T);
+  s.part_rows = R > 128 ? 256 : (R + 7) / 8 * 8;
+  s.bytes = s.part + (dh == 64 || dh == 128 ? (size_t)attn_tree_tc_blocks() * 2 * s.part_rows * (dh + 2) * 4 : 0);
+  return s;
+}
+
 size_t attn_tree_scratch_bytes(int B, int T, int H, int KV, int dh) {
   if (B < 0 || T < 1 || KV < 1 || H % KV || dh < 1) return 0;
-  return (((size_t)B * T * H * dh * 2) + 255) / 256 * 256;
+  return tree_scratch(B, T, H, KV, dh).bytes;
 }
 
 template <int DH>
@@ -179,6 +200,8 @@ static cudaError_t tree_launch(const AttnTreeArgs& a, cudaStream_t st, bool pdl)
   cfg.gridDim = dim3(a.B * a.T, (a.H + a.KV + 7) / 8);
   cudaError_t e = cudaLaunchKernelEx(&cfg, tree_append_kernel<DH>, a);
   if (e != cudaSuccess) return e;
+  if constexpr (DH >= 64)
+    if (attn_tree_tc_ok(a)) return attn_tree_tc_launch(a, st);
   cfg.gridDim = dim3((a.T * (a.H / a.KV) + 7) / 8, a.KV, a.B);
   cfg.numAttrs = 0;
   return cudaLaunchKernelEx(&cfg, attn_tree_kernel<DH>, a);
@@ -196,7 +219,13 @@ cudaError_t attn_tree_launch(const AttnTreeArgs& a0, cudaStream_t st, bool pdl) 
   if (!a.qkv || !a.kc || !a.vc || !a.table || !a.lens || !a.out || !a.scratch ||
       a.scratch_bytes < attn_tree_scratch_bytes(a.B, a.T, a.H, a.KV, a.dh) || a.B > 65535 || a.KV > 65535)
     return cudaErrorInvalidValue;
-  a.q = static_cast<__half*>(a.scratch);
+  const TreeScratch s = tree_scratch(a.B, a.T, a.H, a.KV, a.dh);
+  char* base = static_cast<char*>(a.scratch);
+  if (reinterpret_cast<uintptr_t>(base) & 15) return cudaErrorInvalidValue;
+  a.q = reinterpret_cast<__half*>(base);
+  a.flags = reinterpret_cast<unsigned char*>(base + s.flags);
+  a.part = reinterpret_cast<float*>(base + s.part);
+  a.part_rows = s.part_rows;
   switch (a.dh) {
     case 16: return tree_launch<16>(a, st, pdl);
     case 32: return tree_launch<32>(a, st, pdl);

@@ -1,0 +1,735 @@
+// Tree attention over a paged cache on the 5th-generation tensor cores (head dims 64 and 128).
+//
+// The T * G query rows that share a key head are the rows of one product; keys go through in tiles of
+// 128. A block (one per SM) holds two streams, each with its own scores S, running maximum and sum, and
+// output O in tensor memory, so that the tensor cores work on one stream while the other takes its
+// exponentials:
+//   more than 128 rows   the streams are two tiles of 128 rows over the same keys (K and V read once)
+//   at most 128 rows     the streams take the even and the odd key tiles of the same rows, joined at the
+//                        end: O and O' = O e^(m - M) + O' e^(m' - M)
+//
+//   S = Q K^T    Q and K in shared memory (128-byte swizzle), S in tensor memory
+//   P            a thread per row: maximum, exponentials (fp16, the operand of the next product), sum;
+//                P takes S's place in tensor memory
+//   O += P V     P from tensor memory, V from shared memory as an MN-major operand
+// O is rescaled only when the maximum has risen by more than 2^8: P stays under 2^14 (weights carry a
+// factor 2^6, so that the small ones keep their bits), and the sum uses the same factor.
+//
+// Work split: the key tiles of all (sequence, key head) pairs in a row are cut into equal runs, one for
+// each block, whatever the sequences' lengths; a pair that was cut leaves partial (m, l, O) behind, which
+// tree_combine joins in the order of the keys, so the result does not depend on timing. The cut comes
+// from lens on the device.
+//
+// K and V arrive by TMA in boxes of as many rows as divide the page (8..128, or 128 where a sequence is
+// one page) into a ring of tiles. Rows before the prefix's end are loaded while tree_append still runs.
+// Rows that hold nothing (past the last node, or without a page) are taken out of the scores and zeroed
+// in V; nodes whose k or v is not finite are taken out of the products too and added by the row's thread
+// at the end, for the rows that see them only.
+//
+// Roles (320 threads): warps 0-3 and 4-7 the streams' rows, warp 8 tensor memory and the products
+// (one thread), warp 9 the copies. Every wait is bounded; a block that gives up records
+// AF_DEV_WAIT_TIMEOUT, waits for its copies and products in flight, frees its tensor memory and returns.
+#include <cuda.h>
+
+#include "af_common.cuh"
+#include "af_kernels.h"
+#include "tcgen05.cuh"
+#include "tree_common.cuh"
+
+namespace af {
+
+namespace tt {
+constexpr int BK = 128;                        // keys per tile
+constexpr int THREADS = 320;
+constexpr int MMA_WARP = 8, TMA_WARP = 9;
+constexpr int SLICE = 128 * 64 * 2;            // 128 rows x 64 fp16, 128-byte swizzled
+constexpr long long LIMIT = 1ll << 26;
+constexpr float SHIFT = 6.f, RISE = 8.f;       // log2 of the weights' factor; rise of the maximum that is let pass
+constexpr int MAXW = TREE_MAX_NODES / 32;
+template <int DH, bool TWO> struct Cfg {
+  static constexpr int TILE = SLICE * (DH / 64);
+  static constexpr int QT = TWO ? 2 : 1;       // row tiles
+  static constexpr int NS = DH == 128 ? (TWO ? 5 : 6) : 8;   // ring slots (K or V tiles)
+  static constexpr int RING = QT * TILE;
+  static constexpr int SH = RING + NS * TILE;
+};
+constexpr uint32_t S_COL = 0, O_COL = 256;     // S / P of stream w at 128 w, O at 256 + 128 w
+constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+template <int DH> struct IdescPV {
+  static constexpr uint32_t v = (1u << 4) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+};
+}  // namespace tt
+
+struct TreeShared {
+  uint64_t q_full, q_empty;
+  uint64_t full[8], empty[8];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t acc_free;                           // both streams' O read out
+  uint64_t done;
+  float2 ml[2][128];                           // split streams: (m, l) of the other half
+  uint32_t vmask[8];                           // boxes of the tile that have a page
+  uint32_t bad[tt::MAXW];                      // nodes whose k or v is not finite
+  uint32_t tmem;
+  int abort;
+};
+
+AF_DEV bool tt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  SpinBudget budget;
+  for (long long i = 0; i < tt::LIMIT; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255) == 255 && (*abort || budget.spent())) return false;
+  }
+  return false;
+}
+AF_DEV bool tt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, tt_wait(bar, parity, abort));
+}
+
+// barrier of the 256 row threads; true if `ok` holds in all of them
+AF_DEV bool rows_all(bool ok) {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(r) : "r"((uint32_t)ok) : "memory");
+  return r != 0;
+}
+
+AF_DEV float tt_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+#define TT_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define TT_R32(v, o) TT_R8(v, o), TT_R8(v, o + 8), TT_R8(v, o + 16), TT_R8(v, o + 24)
+// 128 columns of this warp's 32 lanes
+AF_DEV void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
+  asm volatile(
+      "{\n"
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n"
+      "tcgen05.wait::ld.sync.aligned;\n}\n"
+      : TT_R32(v, 0), TT_R32(v, 32), TT_R32(v, 64), TT_R32(v, 96)
+      : "r"(taddr)
+      : "memory");
+}
+
+AF_DEV void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+      ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+AF_DEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+}
+
+// where a tile's K and V stand in the order in which they are loaded and used: two row tiles K0 V0 K1 V1
+// ..., split streams K0 K1 V0 K2 V1 K3 ...
+template <bool TWO> AF_DEV int seq_k(int j) { return TWO ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
+template <bool TWO> AF_DEV int seq_v(int j, int nt) { return TWO ? 2 * j + 1 : (j == nt - 1 ? 2 * nt - 1 : 2 * j + 2); }
+
+// visibility of 32 nodes from node number u0 (may be negative: prefix rows) for a node's mask row
+AF_DEV uint32_t see32(const int* mask, int words, int t, int u0) {
+  if (u0 <= -32) return 0xffffffffu;
+  auto word = [&](int w) -> uint32_t {
+    if (w < 0) return 0xffffffffu;
+    if (mask) return w < words ? (uint32_t)__ldg(mask + w) : 0u;
+    const int k = t - 32 * w;                  // chain: nodes 0..t
+    return k < 0 ? 0u : k >= 31 ? 0xffffffffu : (2u << k) - 1;
+  };
+  const int w = u0 >> 5, s = u0 & 31;          // floor division: u0 = 32 w + s
+  return s ? __funnelshift_r(word(w), word(w + 1), s) : word(w);
+}
+AF_DEV uint32_t ones_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+
+template <int DH, bool TWO>
+__global__ void __launch_bounds__(tt::THREADS, 1)
+    attn_tree_tc_kernel(AttnTreeArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap) {
+  using namespace tt;
+  using C = Cfg<DH, TWO>;
+  constexpr int NS = C::NS, TILE = C::TILE;
+  // the swizzle's period is 1024 bytes; there is no room to align by hand, so a wrong base is an error
+  extern __shared__ __align__(1024) unsigned char tt_raw[];
+  unsigned char* smem = tt_raw;
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) af_set_err(a.err, AF_DEV_WAIT_TIMEOUT);
+    return;
+  }
+  TreeShared* sh = reinterpret_cast<TreeShared*>(smem + C::SH);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.H / a.KV, R = a.T * G;
+  pdl_trigger();
+  TreeSched sc;
+  sc.init(a, blockIdx.x, gridDim.x, lane);
+  if (sc.u >= sc.u1) return;                   // fewer tiles than blocks
+
+  if (threadIdx.x == 0) {
+    mbar_init(&sh->q_full, 1);
+    mbar_init(&sh->q_empty, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&sh->s_full[w], 1);
+      mbar_init(&sh->p_full[w], 128);
+      mbar_init(&sh->o_full[w], 1);
+    }
+    mbar_init(&sh->acc_free, 256);
+    mbar_init(&sh->done, 1);
+    sh->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&sh->tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sh->tmem;
+  volatile int* abort = &sh->abort;
+
+  if (warp == TMA_WARP) {
+    // ------------------------------------------------------------- copies (a lane per box)
+    const int nbox = BK / a.box_rows;                        // boxes of a tile, for each 64 columns
+    const int half = lane / nbox, box = lane - half * nbox;
+    const bool mine = half < DH / 64;
+    bool waited = false, ok = true;
+    int seq0 = 0, nseg = 0, issued = 0, nq = 0;              // issued: ring slots, nq: Q tiles
+    auto dependency = [&] {                                  // q and the nodes' rows come from tree_append
+      if (waited) return;
+      pdl_wait();
+      asm volatile("fence.proxy.async.global;" ::: "memory");
+      waited = true;
+    };
+    for (; ok && sc.u < sc.u1; sc.next(a), ++nseg) {
+      const int nt = sc.tiles();
+      bool have_q = false;
+      auto load_q = [&]() -> bool {
+        dependency();
+        if (nseg && !tt_wait_warp(&sh->q_empty, (uint32_t)((nseg - 1) & 1), abort)) return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh->q_full, C::QT * TILE);
+          for (int w = 0; w < C::QT; ++w)
+            for (int k = 0; k < DH / 64; ++k)
+              tma_load_3d(smem + w * TILE + k * SLICE, &qmap, 64 * k, sc.rg * 256 + 128 * w, sc.b * a.KV + sc.h, &sh->q_full);
+        }
+        have_q = true;
+        ++nq;
+        return true;
+      };
+      // the loads in the order of their use
+      for (int i = 0; ok && i < 2 * nt; ++i) {
+        int j;
+        bool is_v;
+        if (TWO) { j = i >> 1; is_v = i & 1; }
+        else if (i == 0) { j = 0; is_v = false; }
+        else if (i == 2 * nt - 1) { j = nt - 1; is_v = true; }
+        else { is_v = !(i & 1); j = is_v ? (i - 2) >> 1 : (i + 1) >> 1; }
+        const int seq = seq0 + i, st = seq % NS;
+        const int row = (sc.t0 + j) * BK + box * a.box_rows;
+        if (!have_q && (waited || seq >= NS || (sc.t0 + j + 1) * BK > sc.len)) {
+          if (!load_q()) { ok = false; break; }
+        }
+        if (seq >= NS && !tt_wait_warp(&sh->empty[st], (uint32_t)((seq / NS - 1) & 1), abort)) { ok = false; break; }
+        int p = -1;
+        if (mine && row < sc.len + sc.nodes) {
+          p = __ldg(a.table + (size_t)sc.b * a.W + row / a.page);
+          if (p < 0 || p >= a.P) { p = -1; af_set_err(a.err, AF_DEV_BAD_POS); }
+        }
+        const unsigned live = __ballot_sync(0xffffffffu, p >= 0);
+        if (lane == 0) {
+          sh->vmask[st] = live & (nbox == 32 ? 0xffffffffu : (1u << nbox) - 1);
+          mbar_arrive_expect_tx(&sh->full[st], (uint32_t)(__popc(live) * a.box_rows * 128));
+        }
+        __syncwarp();
+        if (p >= 0)
+          tma_load_4d(smem + C::RING + st * TILE + half * SLICE + box * a.box_rows * 128, is_v ? &vmap : &kmap, 64 * half,
+                      row % a.page, sc.h, p, &sh->full[st]);
+        issued = seq + 1;
+      }
+      if (ok && !have_q) ok = load_q();
+      if (ok) seq0 += 2 * nt;
+    }
+    if (!ok) *abort = 1;
+    dependency();
+    // shared memory must outlive every copy issued: a block that gave up waits (bounded) for the last ones
+    if (!ok) {
+      for (int s = max(0, issued - NS); s < issued; ++s) {
+        SpinBudget b;
+        while (!mbar_try_wait(&sh->full[s % NS], (uint32_t)((s / NS) & 1)) && !b.spent()) {
+        }
+      }
+      SpinBudget b;
+      while (nq && !mbar_try_wait(&sh->q_full, (uint32_t)((nq - 1) & 1)) && !b.spent()) {
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    // ------------------------------------------------------------- products (one thread)
+    if (lane == 0) {
+      bool ok = true;
+      int seq0 = 0, nseg = 0;
+      uint32_t np[2] = {0, 0};                               // tiles of each stream so far
+      for (; ok && sc.u < sc.u1; sc.next(a), ++nseg) {
+        const int nt = sc.tiles();
+        const uint32_t qa = smem_u32(smem);
+        auto scores = [&](int w, int j, bool last_use) -> bool {
+          const int seq = seq0 + seq_k<TWO>(j), st = seq % NS;
+          if (!tt_wait(&sh->full[st], (uint32_t)((seq / NS) & 1), abort)) return false;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t kb = smem_u32(smem + C::RING + st * TILE), qw = qa + (TWO ? w * TILE : 0);
+#pragma unroll
+          for (int ks = 0; ks < DH / 16; ++ks) {
+            const uint32_t off = (uint32_t)((ks >> 2) * SLICE + (ks & 3) * 32);
+            mma_f16(tmem + S_COL + 128 * w, smem_desc(qw + off), smem_desc(kb + off), IDESC_S, ks != 0);
+          }
+          mma_commit(&sh->s_full[w]);
+          if (last_use) mma_commit(&sh->empty[st]);
+          return true;
+        };
+        auto values = [&](int w, int j, bool first, bool last_use) -> bool {
+          const int seq = seq0 + seq_v<TWO>(j, nt), st = seq % NS;
+          if (!tt_wait(&sh->full[st], (uint32_t)((seq / NS) & 1), abort)) return false;
+          if (!tt_wait(&sh->p_full[w], np[w] & 1, abort)) return false;
+          ++np[w];
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t vb = smem_u32(smem + C::RING + st * TILE);
+#pragma unroll
+          for (int ks = 0; ks < BK / 16; ++ks)
+            mma_f16_ts(tmem + O_COL + 128 * w, tmem + S_COL + 128 * w + ks * 8, smem_desc_mn(vb + (uint32_t)(ks * 2048), SLICE, 1024),
+                       IdescPV<DH>::v, !(first && ks == 0));
+          if (last_use) mma_commit(&sh->empty[st]);
+          return true;
+        };
+        ok = tt_wait(&sh->q_full, (uint32_t)(nseg & 1), abort);
+        if (TWO) {
+          ok = ok && scores(0, 0, false) && scores(1, 0, true);
+          if (ok && nt == 1) mma_commit(&sh->q_empty);
+          if (ok && nseg) ok = tt_wait(&sh->acc_free, (uint32_t)((nseg - 1) & 1), abort);
+          for (int j = 0; ok && j < nt; ++j)
+            for (int w = 0; ok && w < 2; ++w) {
+              ok = values(w, j, j == 0, w == 1);
+              if (ok && j == nt - 1) mma_commit(&sh->o_full[w]);
+              if (ok && j + 1 < nt) ok = scores(w, j + 1, w == 1);
+              if (ok && j + 2 == nt && w == 1) mma_commit(&sh->q_empty);
+            }
+        } else {
+          ok = ok && scores(0, 0, true) && (nt < 2 || scores(1, 1, true));
+          if (ok && nt <= 2) mma_commit(&sh->q_empty);
+          if (ok && nseg) ok = tt_wait(&sh->acc_free, (uint32_t)((nseg - 1) & 1), abort);
+          for (int j = 0; ok && j < nt; ++j) {
+            const int w = j & 1;
+            ok = values(w, j, j < 2, true);
+            if (ok && j + 2 >= nt) mma_commit(&sh->o_full[w]);
+            if (ok && j + 2 < nt) ok = scores(w, j + 2, true);
+            if (ok && j + 3 == nt) mma_commit(&sh->q_empty);
+          }
+          if (ok && nt == 1) mma_commit(&sh->o_full[1]);     // the second stream had nothing
+        }
+        seq0 += 2 * nt;
+      }
+      if (!ok) *abort = 1;
+      mma_commit(&sh->done);
+    }
+  } else {
+    // ------------------------------------------------------------- rows (two groups of four warps)
+    const int w = warp >> 2, wr = (warp & 3) * 32 + lane;    // stream, row of the tile = TMEM lane
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float sl2 = a.scale * 1.4426950408889634f;
+    bool ok = true;
+    int seq0 = 0, nseg = 0;
+    uint32_t ns = 0;                                         // tiles of this stream so far
+    pdl_wait();                                              // the flags of nodes that are not finite
+    for (; sc.u < sc.u1; sc.next(a), ++nseg) {
+      // all rows go on, or none (barriers lie ahead); `bad` is free from here
+      ok = rows_all(ok);
+      if (!ok) break;
+      const int nt = sc.tiles();
+      const int r = (TWO ? sc.rg * 256 + 128 * w : 0) + wr;  // row of the pair
+      const bool live_warp = r - lane < R;
+      const bool in = r < R;
+      const int t = in ? r / G : 0;
+      const int n = sc.len + sc.nodes;
+      const int* mrow = a.mask ? a.mask + ((size_t)sc.b * a.T + t) * a.mask_words : nullptr;
+      // nodes that are not finite: only a segment that meets the nodes looks
+      const bool tail = (sc.t0 + nt) * BK > sc.len;
+      if (tail && warp < MAXW) {
+        const int u = 32 * warp + lane;
+        const bool b = u < sc.nodes && __ldcg(a.flags + ((size_t)sc.b * a.KV + sc.h) * a.T + u);
+        const unsigned m = __ballot_sync(0xffffffffu, b);
+        if (lane == 0) sh->bad[warp] = m;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      float m = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int j = TWO ? 0 : w; j < nt; j += TWO ? 1 : 2) {
+        if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
+        ++ns;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int j0 = (sc.t0 + j) * BK;
+        const int seqv = seq0 + seq_v<TWO>(j, nt), stv = seqv % NS;
+        // a tile that reaches past the prefix, or into rows without a page
+        bool odd = j0 + BK > sc.len;
+        uint32_t boxes = 0xffffffffu;
+        if (a.paged || odd) {
+          if (!tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
+          boxes = *(volatile uint32_t*)&sh->vmask[stv];
+          odd |= boxes != (BK / a.box_rows == 32 ? 0xffffffffu : (1u << (BK / a.box_rows)) - 1);
+        }
+        if (odd) {
+          // rows of V that nobody may see become zeros (whatever lies there times a weight of 0 must be 0)
+          unsigned char* vt = smem + C::RING + stv * TILE;
+          const int k = wr, key = j0 + k;
+          const int u = key - sc.len;
+          const bool gone = key >= n || !(boxes >> (k / a.box_rows) & 1) || (u >= 0 && (sh->bad[u >> 5] >> (u & 31) & 1));
+          if (gone)
+            for (int c = 0; c < DH / 8; ++c)
+              *reinterpret_cast<uint4*>(vt + (c >> 3) * SLICE + sw128(k, c & 7)) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (live_warp) {
+          uint32_t v[128];
+          tmem_ld128(lanes + S_COL + 128 * w, v);
+          if (odd) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int k0 = j0 + 32 * c, u0 = k0 - sc.len;
+              uint32_t vis = see32(mrow, a.mask_words, t, u0) & ones_below(n - k0);
+              if (u0 > -32) {                                // not the nodes that are added at the end
+                const int bw = u0 >> 5, bs = u0 & 31;
+                const uint32_t lo = bw >= 0 && bw < MAXW ? sh->bad[bw] : 0u, hi = bw + 1 >= 0 && bw + 1 < MAXW ? sh->bad[bw + 1] : 0u;
+                vis &= ~(bs ? __funnelshift_r(lo, hi, bs) : lo);
+              }
+              for (int e = 0; e < 32; e += a.box_rows)       // box_rows >= 8
+                if (!(boxes >> ((32 * c + e) / a.box_rows) & 1))
+                  vis &= ~((a.box_rows >= 32 ? 0xffffffffu : (1u << a.box_rows) - 1) << e);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(vis >> e & 1)) v[32 * c + e] = 0xff800000u;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 128; e += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(v[e + k]));
+          const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+          const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY;
+          if (__any_sync(0xffffffffu, rise)) {
+            const float mn = fmaxf(m, tm);
+            const float corr = m == -INFINITY ? 0.f : tt_ex2(m - mn);
+            m = mn;
+            l *= corr;
+            if (!first) {
+              // s_full came after the products before it, so O is at rest
+#pragma unroll 1
+              for (int c0 = 0; c0 < DH; c0 += 32) {
+                uint32_t o[32];
+                tmem_ld32(lanes + O_COL + 128 * w + c0, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                tmem_st32(lanes + O_COL + 128 * w + c0, o);
+              }
+            }
+          }
+          const float mb = m == -INFINITY ? 0.f : m - SHIFT;
+          float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float p0 = tt_ex2(fmaf(__uint_as_float(v[64 * c + 2 * e]), sl2, -mb));
+              const float p1 = tt_ex2(fmaf(__uint_as_float(v[64 * c + 2 * e + 1]), sl2, -mb));
+              ps[(e & 1) * 2] += p0;
+              ps[(e & 1) * 2 + 1] += p1;
+              const __half2 hp = __floats2half2_rn(p0, p1);
+              pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
+            }
+            tmem_st32(lanes + S_COL + 128 * w + 32 * c, pk);
+          }
+          l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        }
+        first = false;
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        mbar_arrive(&sh->p_full[w]);
+      }
+      seq0 += 2 * nt;
+      // ---- the segment's end
+      ok = ok && tt_wait_warp(&sh->o_full[w], (uint32_t)(nseg & 1), abort);
+      if (!TWO) ok = ok && tt_wait_warp(&sh->o_full[w ^ 1], (uint32_t)(nseg & 1), abort);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      float f0 = 1.f, f1 = 0.f;                              // weights of O and of the other stream's O
+      bool have0 = !first, have1 = false;
+      if (!TWO) {
+        sh->ml[w][wr] = make_float2(m, l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float2 o = sh->ml[w ^ 1][wr];
+        const float M = fmaxf(m, o.x);
+        f0 = m == -INFINITY ? 0.f : tt_ex2(m - M);
+        f1 = o.x == -INFINITY ? 0.f : tt_ex2(o.x - M);
+        l = l * f0 + o.y * f1;
+        m = M;
+        have1 = nt > (w ? 0 : 1);
+      }
+      // nodes that are not finite, for the segment that ends with the sequence
+      const bool ends = sc.ends();
+      bool any_bad = false;
+      if (tail && ends)
+        for (int k = 0; k < MAXW; ++k) any_bad |= sh->bad[k] != 0;
+      auto visible = [&](int u) { return mrow ? (__ldg(mrow + (u >> 5)) >> (u & 31)) & 1 : u <= t; };
+      auto node_row = [&](const __half* c, int u) {
+        const int row = sc.len + u, p = __ldg(a.table + (size_t)sc.b * a.W + row / a.page);
+        return p < 0 || p >= a.P ? nullptr : c + (size_t)p * a.page_stride + ((size_t)sc.h * a.page + row % a.page) * DH;
+      };
+      auto node_score = [&](const __half* kr) {
+        const __half* q = a.q + (((size_t)sc.b * a.KV + sc.h) * R + r) * DH;
+        float s = 0.f;
+        for (int d = 0; d < DH; ++d) s = fmaf(h2f(__ldcg(q + d)), h2f(__ldcg(kr + d)), s);
+        return s * sl2;
+      };
+      float m2 = m;
+      if (any_bad && in) {
+        for (int u = 0; u < sc.nodes; ++u)
+          if ((sh->bad[u >> 5] >> (u & 31) & 1) && visible(u)) {
+            const __half* kr = node_row(a.kc, u);
+            if (kr) m2 = fmaxf(m2, node_score(kr));
+          }
+        const float c = m == -INFINITY ? 0.f : tt_ex2(m - m2);
+        f0 *= c; f1 *= c; l *= c;
+        m = m2;
+        for (int u = 0; u < sc.nodes; ++u)
+          if ((sh->bad[u >> 5] >> (u & 31) & 1) && visible(u)) {
+            const __half* kr = node_row(a.kc, u);
+            if (kr) l += tt_ex2(node_score(kr) - (m - SHIFT));
+          }
+      }
+      const bool whole = sc.whole();
+      const float il = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);       // NaN stays
+      // split streams: each group writes half of the columns
+      constexpr int CW = TWO ? DH : DH / 2;
+      const int cb = TWO ? 0 : w * CW;
+      float* part = nullptr;
+      if (!whole) {
+        part = a.part + (size_t)(blockIdx.x * 2 + sc.slot()) * a.part_rows * (DH + 2);
+        if ((TWO || w == 0) && ok && in) {
+          const int pr = (TWO ? 128 * w : 0) + wr;
+          reinterpret_cast<float2*>(part + (size_t)a.part_rows * DH)[pr] = make_float2(m, l);
+        }
+      }
+      if (ok && live_warp)
+#pragma unroll 1
+        for (int c0 = cb; c0 < cb + CW; c0 += 32) {
+          float x[32];
+          uint32_t o[32];
+          if (have0) {
+            tmem_ld32(lanes + O_COL + 128 * w + c0, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * f0;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = 0.f;
+          }
+          if (have1) {
+            tmem_ld32(lanes + O_COL + 128 * (w ^ 1) + c0, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = fmaf(__uint_as_float(o[e]), f1, x[e]);
+          }
+          if (any_bad && in)
+            for (int u = 0; u < sc.nodes; ++u)
+              if ((sh->bad[u >> 5] >> (u & 31) & 1) && visible(u)) {
+                const __half* kr = node_row(a.kc, u);
+                const __half* vr = node_row(a.vc, u);
+                if (!kr) continue;
+                const float p = tt_ex2(node_score(kr) - (m - SHIFT));
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = fmaf(p, h2f(__ldcg(vr + c0 + e)), x[e]);
+              }
+          if (!in) continue;
+          if (whole) {
+            const int g = r - t * G;
+            __half* dst = a.out + ((size_t)sc.b * a.T + t) * a.ld_out + (size_t)(sc.h * G + g) * DH + c0;
+            const bool live = t < sc.nodes;
+            if (a.out16) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint32_t o4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const __half2 hv = live ? __floats2half2_rn(x[8 * q + 2 * i] * il, x[8 * q + 2 * i + 1] * il) : __half2();
+                  o4[i] = *reinterpret_cast<const uint32_t*>(&hv);
+                }
+                *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) dst[e] = live ? f2h(x[e] * il) : __half();
+            }
+          } else {
+            const int pr = (TWO ? 128 * w : 0) + wr;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              __stcg(reinterpret_cast<float4*>(part) + (size_t)(c0 / 4 + q) * a.part_rows + pr,
+                     make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
+          }
+        }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      mbar_arrive(&sh->acc_free);
+    }
+    if (!ok) {
+      *abort = 1;
+      af_set_err(a.err, AF_DEV_WAIT_TIMEOUT);
+    }
+  }
+  // the tensor memory is freed only once the products are idle
+  if (warp == MMA_WARP) {
+    SpinBudget b;
+    if (lane == 0)
+      while (!mbar_try_wait(&sh->done, 0) && !b.spent()) {
+      }
+    __syncwarp();
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// joins the parts of the pairs that were cut: grid (row blocks, KV, B), a thread per 4 output elements
+template <int DH>
+__global__ void __launch_bounds__(256) tree_combine_kernel(AttnTreeArgs a, int blocks) {
+  constexpr int C4 = DH / 4, ROWS = 256 / C4;
+  const int lane = threadIdx.x & 31;
+  const int G = a.H / a.KV, R = a.T * G;
+  const int r = blockIdx.x * ROWS + threadIdx.x % ROWS, c4 = threadIdx.x / ROWS;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int rg = a.row_groups > 1 ? r / 256 : 0;
+  TreeSched sc;
+  long long first, total;
+  sc.find(a, b, lane, first, total);
+  const int rg0 = a.row_groups > 1 ? blockIdx.x * ROWS / 256 : 0;    // ROWS divides 256: one group a block
+  const long long u0 = first + (long long)(h * a.row_groups + rg0) * sc.nt, u1 = u0 + sc.nt;
+  const int c0 = tree_block_of(u0, total, blocks), c1 = tree_block_of(u1 - 1, total, blocks);
+  pdl_wait();
+  if (c0 == c1 || r >= R) return;
+  const int pr = r - rg * 256, t = r / G, g = r - t * G;
+  float M = -INFINITY;
+  for (int c = c0; c <= c1; ++c) {
+    const int slot = tree_unit(c, total, blocks) > u0 ? 0 : 1;
+    const float* part = a.part + (size_t)(c * 2 + slot) * a.part_rows * (DH + 2);
+    M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part + (size_t)a.part_rows * DH) + pr).x);
+  }
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0; c <= c1; ++c) {
+    const int slot = tree_unit(c, total, blocks) > u0 ? 0 : 1;
+    const float* part = a.part + (size_t)(c * 2 + slot) * a.part_rows * (DH + 2);
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + (size_t)a.part_rows * DH) + pr);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float f = tt_ex2(ml.x - M);
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(part) + (size_t)c4 * a.part_rows + pr);
+    l = fmaf(ml.y, f, l);
+    o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+  }
+  float il = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (t >= sc.nodes) { il = 0.f; o = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __half2 x[2] = {__floats2half2_rn(o.x * il, o.y * il), __floats2half2_rn(o.z * il, o.w * il)};
+  __half* dst = a.out + ((size_t)b * a.T + t) * a.ld_out + (size_t)(h * G + g) * DH + 4 * c4;
+  if (a.out16) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(x);
+  else {
+    const __half* e = reinterpret_cast<const __half*>(x);
+    for (int k = 0; k < 4; ++k) dst[k] = e[k];
+  }
+}
+
+// K / V [P][KV][page][dh]: boxes of 64 columns and box_rows rows of one head's page
+static bool cache_map(CUtensorMap* map, const AttnTreeArgs& a, const __half* base) {
+  const EncodeTiledFn enc = encode_tiled();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.dh, (cuuint64_t)a.page, (cuuint64_t)a.KV, (cuuint64_t)a.P};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.dh * 2, (cuuint64_t)a.page * a.dh * 2, (cuuint64_t)a.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)a.box_rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static bool q_map(CUtensorMap* map, const AttnTreeArgs& a, int rows) {
+  const EncodeTiledFn enc = encode_tiled();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.dh, (cuuint64_t)rows, (cuuint64_t)a.B * a.KV};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.dh * 2, (cuuint64_t)rows * a.dh * 2};
+  const cuuint32_t box[3] = {64, 128, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.q, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int attn_tree_tc_blocks() { return device_attr(cudaDevAttrMultiProcessorCount, 148); }
+
+// rows of a page that one box can cover: a box never crosses a page (unless the sequence is one page,
+// where it ends at the map's bound), and starts at a multiple of 8 rows, the swizzle's period
+static int box_rows(const AttnTreeArgs& a) { return a.W == 1 ? 128 : (a.page & -a.page) > 128 ? 128 : a.page & -a.page; }
+
+bool attn_tree_tc_ok(const AttnTreeArgs& a) {
+  return (a.dh == 64 || a.dh == 128) && a.scale > 0.f && a.scale < 1e30f && box_rows(a) >= 8;
+}
+
+template <int DH, bool TWO>
+static cudaError_t tc_launch(const AttnTreeArgs& a, cudaStream_t st) {
+  const int R = a.T * (a.H / a.KV);
+  CUtensorMap qm, km, vm;
+  if (!q_map(&qm, a, R) || !cache_map(&km, a, a.kc) || !cache_map(&vm, a, a.vc)) return cudaErrorInvalidValue;
+  constexpr int SMEM = tt::Cfg<DH, TWO>::SH + (int)sizeof(TreeShared);
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static PerDeviceOnce attrs;
+  const cudaError_t ae = attrs.run([] {
+    return cudaFuncSetAttribute(attn_tree_tc_kernel<DH, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  });
+  if (ae != cudaSuccess) return ae;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  const int blocks = attn_tree_tc_blocks();
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(tt::THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_tree_tc_kernel<DH, TWO>, a, qm, km, vm);
+  if (e != cudaSuccess) return e;
+  constexpr int ROWS = 1024 / DH;
+  cfg.gridDim = dim3((R + ROWS - 1) / ROWS, a.KV, a.B);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<DH>, a, blocks);
+}
+
+cudaError_t attn_tree_tc_launch(AttnTreeArgs a, cudaStream_t st) {
+  const int R = a.T * (a.H / a.KV);
+  a.box_rows = box_rows(a);
+  a.paged = a.W > 1;
+  a.row_groups = (R + 255) / 256;
+  a.out16 = a.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  if (R <= 128) return a.dh == 128 ? tc_launch<128, false>(a, st) : tc_launch<64, false>(a, st);
+  return a.dh == 128 ? tc_launch<128, true>(a, st) : tc_launch<64, true>(a, st);
+}
+
+}  // namespace af
