@@ -130,11 +130,17 @@ def load_library():
   return L
 
 
+_usable = False
+
+
 def lib():
-  """The bound library, after checking a CUDA device is usable (no CPU fallback)."""
-  import torch
-  if not torch.cuda.is_available():
-    raise RuntimeError("aneforge_b200 needs a CUDA device (B200); no CPU fallback exists")
+  """The bound library, after checking (once) that a CUDA device is usable (no CPU fallback)."""
+  global _usable
+  if not _usable:
+    import torch
+    if not torch.cuda.is_available():
+      raise RuntimeError("aneforge_b200 needs a CUDA device (B200); no CPU fallback exists")
+    _usable = True
   return load_library()
 
 

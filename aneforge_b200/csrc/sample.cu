@@ -59,9 +59,9 @@ AF_DEV T block_sum(T v, T* buf) {
   return s;
 }
 
-// grid: one block per row
+// ---- rows too long for a cluster's registers: one block per row, the row read again for each step
 template <class T>
-__global__ void __launch_bounds__(smp::THREADS) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(smp::THREADS) sample_long_kernel(SampleArgs a) {
   __shared__ u64 sum_s[32];
   __shared__ u64 hist[256];
   __shared__ u64 best_s;
@@ -197,17 +197,694 @@ __global__ void __launch_bounds__(smp::THREADS) sample_kernel(SampleArgs a) {
   }
 }
 
+// ---- rows held in registers: a cluster of blocks per row
+//
+// Each thread keeps NV vectors of 16 bytes of the row as fp32 for the whole call, so the row is read
+// once. Steps (a cluster barrier after each): the maximum; a histogram of how far the logits lie below
+// it, in eighths of a nat (top-k), or the bound that min-p sets; the tokens that can still be kept are
+// listed. At most LIST of them: the first block sorts them, and everything else happens there. More:
+// the k-th key and the nucleus' last key come from a radix search (8 bits a step, whole-number sums),
+// then the token from the blocks' kept sums, over the lists or, where a list overflows, the registers.
+// A nucleus without top-k can hold a quarter of the vocabulary: the weights are summed by the upper bits
+// of e (exactly: a bin's tokens share an octave, so a count and the sum of the lower bits give their
+// weight), only the bin that the limit falls into is sorted, and the kept sums come from the registers.
+namespace smr {
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int BINS = 128;                      // 16 nats
+constexpr int LIST = 1024;                     // tokens that the first block sorts
+constexpr int LOCAL = 3072;                    // listed tokens of one block
+constexpr int MAXC = 16;
+// nucleus: weights by the upper bits of e (32 bins an octave, bin 0 is e = 1), down to 2^-24
+constexpr int EBITS = 18, EBINS = 24 * 32 + 1;
+}  // namespace smr
+
+struct SampleShared {
+  uint32_t kmax[smr::MAXC];                    // written by every block of the cluster: its maximum,
+  uint32_t first[smr::MAXC];                   // first index of the maximum,
+  uint32_t count[smr::MAXC];                   // listed tokens,
+  u64 total[smr::MAXC];                        // weight
+  u64 kept[smr::MAXC];                         // and kept weight
+  uint32_t hist[smr::BINS];
+  uint32_t ecnt[smr::EBINS], elow[smr::EBINS]; // tokens, and the sum of their weights' lower bits
+  u64 radix[2][256];
+  u64 sums[smr::WARPS * 12];                   // kept weight (or ties) of a (vector, warp)
+  u64 scan[smr::WARPS];
+  u64 list[smr::LIST];                         // key << 32 | ~index, of the whole row (first block)
+  u64 local[smr::LOCAL];                       // the same, of this block
+  uint32_t nlist, nlocal, kloc, floc;
+  u64 pick;
+  u64 total_w;
+  u64 cut;                                     // the nucleus' last token, key << 32 | ~index
+  int where;
+};
+
+AF_DEV float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
+template <class P> AF_DEV P* peer(P* p, int rank) {
+  uint64_t r;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"((uint64_t)p), "r"(rank));
+  return reinterpret_cast<P*>(r);
+}
+AF_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+AF_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// weight in two whole-number parts, w = hi * 2^20 + lo: adding 8 (2^-17) rounds down to a multiple of 2^-20 (2^-40)
+AF_DEV void weight_parts(float e, uint32_t& hi, uint32_t& lo) {
+  const float t = __fadd_rd(e, 8.f);
+  const float t2 = __fadd_rd(e - (t - 8.f), 7.62939453125e-06f);
+  hi = __float_as_uint(t) - 0x41000000u;
+  lo = __float_as_uint(t2) - 0x37000000u;
+}
+
+// descending bitonic sort of N (a power of two) 64-bit values in shared memory by the whole block (one
+// warp where that is enough)
+AF_DEV void sort_desc(u64* x, int N) {
+  const int tid = threadIdx.x;
+  const bool small = N <= 64;
+  if (small && tid >= 32) N = 0;
+  for (int k = 2; k <= N; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = tid; i < N / 2; i += smr::THREADS) {
+        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const u64 a = x[lo], b = x[hi];
+        const bool up = lo & k;                // this run ascends
+        if ((a < b) != up) { x[lo] = b; x[hi] = a; }
+        if (small) continue;
+      }
+      if (small) __syncwarp();
+      else __syncthreads();
+    }
+  __syncthreads();
+}
+
+// exclusive sum over the block's threads; `total` gets all of it
+AF_DEV u64 scan_excl(u64 v, u64* buf, u64& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) buf[warp] = x;
+  __syncthreads();
+  u64 before = 0;
+  total = 0;
+#pragma unroll
+  for (int k = 0; k < smr::WARPS; ++k) {
+    const u64 s = buf[k];
+    if (k < warp) before += s;
+    total += s;
+  }
+  return before + x - v;
+}
+
+// target of the draw among `total`: floor(u * total), inside [0, total)
+AF_DEV u64 draw_target(float u, u64 total) {
+  const u64 t = (u64)fmax(floor((double)u * (double)total), 0.0);
+  return t < total ? t : total - 1;
+}
+AF_DEV float logp_of(const RowScale& sc, float l, u64 total) { return sc.below(l) - logf((float)total / 1099511627776.f); }
+
+template <class T, int NV>
+__global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ? 2 : 1) sample_kernel(SampleArgs a, int C) {
+  using namespace smr;
+  constexpr int VE = 16 / (int)sizeof(T), E = NV * VE;
+  extern __shared__ __align__(16) unsigned char sample_raw[];
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = blockIdx.x / C, rank = blockIdx.x % C, V = a.V;
+  if (tid < BINS) sh.hist[tid] = 0;
+  for (int k = tid; k < EBINS; k += THREADS) sh.ecnt[k] = sh.elow[k] = 0;
+  if (tid == 0) { sh.nlist = 0; sh.nlocal = 0; sh.kloc = 0; sh.floc = 0xffffffffu; }
+  __syncthreads();
+  cluster_arrive();                            // the others may write here from their first wait on
+  // ---- the row: vectors from the 16-byte boundary at or before its start, this block's share of them
+  const T* row = static_cast<const T*>(a.logits) + (size_t)r * a.ld;
+  const int skip = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  const int nvec = (skip + V + VE - 1) / VE, per = (nvec + C - 1) / C;
+  float v[E];
+  uint32_t kmax = 0;
+  auto load_row = [&] {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int vi = i * THREADS + tid, i0 = (rank * per + vi) * VE - skip;
+      if (vi < per && i0 >= 0 && i0 + VE <= V) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + i0));
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) v[i * VE + k] = load_logit<T>(e, k);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+          v[i * VE + k] = vi < per && i0 + k >= 0 && i0 + k < V ? load_logit<T>(row, i0 + k) : -INFINITY;
+      }
+    }
+  };
+  load_row();
+  auto index_of = [&](int j) { return (rank * per + (j / VE) * THREADS + tid) * VE - skip + j % VE; };
+  {
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < E; ++j) m = fmaxf(m, v[j]);
+    kmax = __reduce_max_sync(0xffffffffu, key_of(m));
+  }
+  if (lane == 0) atomicMax(&sh.kloc, kmax);
+  __syncthreads();
+  cluster_wait();
+  if (tid < C) *peer(&sh.kmax[rank], tid) = sh.kloc;
+  cluster_arrive();
+  cluster_wait();
+  kmax = sh.kmax[0];
+  for (int k = 1; k < C; ++k) kmax = max(kmax, sh.kmax[k]);
+  const float temp = a.temperature ? a.temperature[r] : a.temperature_s;
+  const int top_k = a.top_k ? a.top_k[r] : a.top_k_s;
+  const float top_p = a.top_p ? a.top_p[r] : a.top_p_s;
+  const float min_p = fminf(a.min_p ? a.min_p[r] : a.min_p_s, 1.f);
+  const float u = a.u[r];
+  RowScale sc;
+  sc.lmax = logit_of(kmax);
+  sc.temp = temp > 0.f ? temp : 1.f;
+  sc.zmax = __fdiv_rn(sc.lmax, sc.temp);
+  if (sc.lmax == -INFINITY) {
+    if (rank == 0 && tid == 0) {
+      a.tok[r] = -1;
+      if (a.logp) a.logp[r] = -INFINITY;
+    }
+    return;
+  }
+  if (!(temp > 0.f)) {
+    uint32_t f = 0xffffffffu;
+#pragma unroll
+    for (int j = E - 1; j >= 0; --j)
+      if (v[j] == sc.lmax) f = (uint32_t)index_of(j);
+    f = __reduce_min_sync(0xffffffffu, f);
+    if (lane == 0) atomicMin(&sh.floc, f);
+    __syncthreads();
+    if (tid == 0) *peer(&sh.first[rank], 0) = sh.floc;
+    cluster_arrive();
+    cluster_wait();
+    if (rank == 0 && tid == 0) {
+      uint32_t b = sh.first[0];
+      for (int k = 1; k < C; ++k) b = min(b, sh.first[k]);
+      a.tok[r] = (int)b;
+      if (a.logp) a.logp[r] = 0.f;
+    }
+    return;
+  }
+  const bool use_k = top_k > 0 && top_k < V, use_p = top_p > 0.f && top_p < 1.f, use_m = min_p > 0.f;
+  // ---- how far below the maximum the logits lie; total weight
+  const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
+  const float scale = 8.f / sc.temp;
+  float cut = -INFINITY;                       // no token under `cut` can be kept
+  u64 total_w = 0, limit = 0;
+  // the nucleus of a whole row: e takes the logits' place (a block's 2^14 values keep a bin's sum in 32 bits)
+  const bool binned = use_p && !use_k && !far && E <= 32;
+  if (use_p && !use_k) {
+    uint32_t hi = 0, lo = 0;
+    auto add = [&](float e) {
+      uint32_t h, l;
+      weight_parts(e, h, l);
+      hi += h;
+      lo += l;
+    };
+    if (binned) {
+      if (sc.temp == 1.f) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) add(v[j] = expf(v[j] - sc.zmax));
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) add(v[j] = expf(__fdiv_rn(v[j], sc.temp) - sc.zmax));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) add(sc.e(v[j]));
+    }
+    hi = __reduce_add_sync(0xffffffffu, hi);
+    lo = __reduce_add_sync(0xffffffffu, lo);
+    if (lane == 0) sh.scan[warp] = ((u64)hi << 20) + lo;
+    __syncthreads();
+    if (tid == 0) {
+      u64 s = 0;
+      for (int k = 0; k < WARPS; ++k) s += sh.scan[k];
+      sh.total_w = s;
+    }
+    __syncthreads();
+    if (tid < C) *peer(&sh.total[rank], tid) = sh.total_w;
+    cluster_arrive();
+    cluster_wait();
+    for (int k = 0; k < C; ++k) total_w += sh.total[k];
+    limit = (u64)ceil((double)top_p * (double)total_w);
+    if (binned) {
+      // tokens so light that all V of them together would not reach past the nucleus need no bin
+      const float light = fmaxf((float)((double)(total_w - limit) / (double)V * (0.999 / 1099511627776.0)), 6.0e-8f);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (v[j] >= light) {
+          const uint32_t b = __float_as_uint(v[j]);
+          const int bin = (int)((0x3f800000u >> EBITS) - (b >> EBITS)), drop = 110 - (int)(b >> 23);
+          atomicAdd(&sh.ecnt[bin], 1u);
+          atomicAdd(&sh.elow[bin], (b & ((1u << EBITS) - 1)) >> max(drop, 0));
+        }
+      cluster_arrive();
+      cluster_wait();
+    }
+  }
+  if (use_k && !far) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float d = (sc.lmax - v[j]) * scale;
+      if (d < (float)BINS) atomicAdd(&sh.hist[(int)d], 1u);
+    }
+    cluster_arrive();
+    cluster_wait();
+    // each block sums the cluster's histograms, then finds the first bin by which k tokens are there
+    u64 n = 0;
+    if (tid < BINS)
+      for (int k = 0; k < C; ++k) n += *peer(&sh.hist[tid], k);
+    u64 all;
+    const u64 before = scan_excl(n, sh.scan, all);
+    if (tid == 0) sh.where = BINS;
+    __syncthreads();
+    if (before < (u64)top_k && (u64)top_k <= before + n) sh.where = tid;
+    __syncthreads();
+    if (sh.where < BINS) cut = -(float)(sh.where + 1);       // a distance, see below
+  } else if (use_m && !use_p && !use_k && !far) {
+    cut = -(-8.f * logf(min_p) * 1.0001f + 1.f);
+  }
+  // a token may be kept if its distance is under -cut: the same product as in the histogram
+  auto may = [&](float l) { return cut == -INFINITY || (sc.lmax - l) * scale < -cut; };
+  // ---- list the tokens that may be kept
+  bool listed = false, small = false;
+  uint32_t n_local = 0;
+  if (cut != -INFINITY) {
+    u64* list0 = peer(sh.list, 0);
+    uint32_t* n0 = peer(&sh.nlist, 0);
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const bool yes = may(v[j]);
+      const unsigned who = __ballot_sync(0xffffffffu, yes);
+      if (!who) continue;
+      uint32_t at = 0, at0 = 0;
+      if (lane == 0) {
+        at = atomicAdd(&sh.nlocal, (uint32_t)__popc(who));
+        if (at < (uint32_t)LIST) at0 = atomicAdd(n0, (uint32_t)__popc(who));
+      }
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+      at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(who & ((1u << lane) - 1));
+      if (yes) {
+        const u64 x = (u64)key_of(v[j]) << 32 | (uint32_t)~index_of(j);
+        if (at < (uint32_t)LOCAL) sh.local[at] = x;
+        if (at < (uint32_t)LIST && at0 < (uint32_t)LIST) list0[at0] = x;
+      }
+    }
+    __syncthreads();
+    n_local = sh.nlocal;
+    if (tid < C) *peer(&sh.count[rank], tid) = n_local;
+    cluster_arrive();
+    cluster_wait();
+    uint32_t all = 0;
+    bool fits = true;
+    for (int k = 0; k < C; ++k) {
+      all += sh.count[k];
+      fits &= sh.count[k] <= (uint32_t)LOCAL;
+    }
+    small = all <= (uint32_t)LIST;
+    listed = fits;                             // the same answer in every block
+    if (small) {
+      if (rank) return;                        // nobody reads the other blocks' memory any more
+      const int n = (int)all;
+      int N = 2;
+      while (N < n) N <<= 1;
+      for (int i = n + tid; i < N; i += THREADS) sh.list[i] = 0;
+      __syncthreads();
+      sort_desc(sh.list, N);
+      const uint32_t kth = use_k ? (uint32_t)(sh.list[top_k - 1] >> 32) : 0u;
+      const int p0 = 2 * tid;
+      u64 w[2];
+      float e[2];
+      u64 mine = 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t key = p0 + k < n ? (uint32_t)(sh.list[p0 + k] >> 32) : 0u;
+        const bool ok = p0 + k < n && key >= kth;
+        e[k] = ok ? sc.e(logit_of(key)) : 0.f;
+        w[k] = ok ? (u64)(e[k] * 1099511627776.f) : 0;
+        if (!ok) e[k] = -1.f;
+        mine += w[k];
+      }
+      u64 sum;
+      u64 before = scan_excl(mine, sh.scan, sum);
+      if (use_p && use_k) limit = (u64)ceil((double)top_p * (double)sum);
+      u64 kept = 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const bool ok = e[k] >= 0.f && (!use_p || before < limit) && e[k] >= min_p;
+        before += w[k];
+        if (!ok) w[k] = 0;
+        kept += w[k];
+      }
+      scan_excl(kept, sh.scan, sum);
+      // the kept ones in index order: index << 32 | key, ascending as the complement descends
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (p0 + k < N) {
+          const u64 x = sh.list[p0 + k];
+          sh.list[p0 + k] = w[k] ? (x << 32 | x >> 32) : 0;      // ~index << 32 | key, descending
+        }
+      __syncthreads();
+      sort_desc(sh.list, N);
+      mine = 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const u64 x = p0 + k < N ? sh.list[p0 + k] : 0;
+        w[k] = x ? sc.w(logit_of((uint32_t)x)) : 0;
+        mine += w[k];
+      }
+      const u64 target = draw_target(u, sum);
+      u64 all_w;
+      before = scan_excl(mine, sh.scan, all_w);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (before <= target && target < before + w[k]) {
+          const u64 x = sh.list[p0 + k];
+          a.tok[r] = (int)~(uint32_t)(x >> 32);
+          if (a.logp) a.logp[r] = logp_of(sc, logit_of((uint32_t)x), sum);
+        }
+        before += w[k];
+      }
+      return;
+    }
+  }
+  // ---- the general way: f(value, index) for each token that may be kept (the value is the logit, or e once
+  // the registers hold that)
+  auto each = [&](auto f) {
+    if (listed) {
+      for (uint32_t i = tid; i < n_local; i += THREADS) {
+        const u64 x = sh.local[i];
+        f(logit_of((uint32_t)(x >> 32)), (int)~(uint32_t)x);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int idx = index_of(j);
+        if (idx >= 0 && idx < V && (j / VE) * THREADS + tid < per) f(v[j], idx);
+      }
+    }
+  };
+  // the largest key such that the weights (or counts) of the keys over it stay under `want`; `left` gets
+  // what is wanted of that key itself
+  int round = 0;
+  auto search = [&](bool counts, uint32_t floor_key, u64 want, u64& left) -> uint32_t {
+    uint32_t lo = floor_key, hi = kmax;
+    left = want;
+    while (true) {
+      const uint32_t range = hi - lo;
+      const int bits = 32 - __clz(range | 1u), shift = bits > 8 ? bits - 8 : 0;
+      u64* hist = sh.radix[round & 1];
+      ++round;
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      each([&](float l, int) {
+        const uint32_t k = key_of(l);
+        if (k >= lo && k <= hi) atomicAdd(&hist[(hi - k) >> shift], counts ? 1ull : sc.w(l));
+      });
+      cluster_arrive();
+      cluster_wait();
+      u64 s = 0;
+      if (tid < 256)
+        for (int k = 0; k < C; ++k) s += *peer(&hist[tid], k);
+      u64 all;
+      const u64 before = scan_excl(s, sh.scan, all);
+      if (tid == 0) sh.where = 255;
+      __syncthreads();
+      if (tid < 256 && before < left && left <= before + s) {
+        sh.where = tid;
+        sh.pick = before;
+      }
+      __syncthreads();
+      const int bin = sh.where;
+      left -= sh.pick;
+      hi -= (uint32_t)bin << shift;
+      if (shift == 0) return hi;
+      const uint32_t width = (1u << shift) - 1;
+      lo = hi - lo > width ? hi - width : lo;
+    }
+  };
+  // the weights of f's results (0: not kept) summed in index order, and the first token whose running sum
+  // passes `target`; -1 in the blocks that do not have it
+  auto find = [&](auto f, u64* totals, auto target_of, u64& total) -> int {
+    // sums of each (vector, warp): index order is (block, vector, warp, lane, element)
+    if (listed) {
+      for (int k = tid; k < NV * WARPS; k += THREADS) sh.sums[k] = 0;
+      __syncthreads();
+      each([&](float x, int idx) {
+        const u64 w = (u64)(f(x, idx) * 1099511627776.f);
+        const int vi = (idx + skip) / VE - rank * per;
+        if (w) atomicAdd(&sh.sums[(vi / THREADS) * WARPS + (vi % THREADS) / 32], w);
+      });
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        uint32_t hi = 0, lo = 0;               // 32 * VE values of at most 2^20 each
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          const int idx = index_of(i * VE + k);
+          uint32_t h, l;
+          weight_parts(f(v[i * VE + k], idx), h, l);      // past the row's end: -inf, or e = 0
+          hi += h;
+          lo += l;
+        }
+        hi = __reduce_add_sync(0xffffffffu, hi);
+        lo = __reduce_add_sync(0xffffffffu, lo);
+        if (lane == 0) sh.sums[i * WARPS + warp] = ((u64)hi << 20) + lo;
+      }
+    }
+    __syncthreads();
+    u64 mine = tid < NV * WARPS ? sh.sums[tid] : 0;
+    u64 all;
+    const u64 before = scan_excl(mine, sh.scan, all);
+    if (tid < C) *peer(&totals[rank], tid) = all;
+    cluster_arrive();
+    cluster_wait();
+    total = 0;
+    u64 base = 0;
+    for (int k = 0; k < C; ++k) {
+      if (k < rank) base += totals[k];
+      total += totals[k];
+    }
+    const u64 target = target_of(total);
+    if (target < base || target >= base + all) return -1;       // another block's (the same answer in all threads)
+    if (tid < NV * WARPS && base + before <= target && target < base + before + mine) {
+      sh.where = tid;
+      sh.pick = target - base - before;
+    }
+    __syncthreads();
+    // inside one (vector, warp): VE * 32 consecutive tokens
+    const int cell = sh.where;
+    const u64 in = sh.pick;
+    const int first = (rank * per + (cell / WARPS) * THREADS + (cell % WARPS) * 32) * VE - skip;
+    for (int k = tid; k < 32 * VE; k += THREADS) sh.list[k] = 0;
+    __syncthreads();
+    each([&](float x, int idx) {
+      if (idx >= first && idx < first + 32 * VE) sh.list[idx - first] = (u64)(f(x, idx) * 1099511627776.f);
+    });
+    __syncthreads();
+    mine = tid < 32 * VE ? sh.list[tid] : 0;
+    const u64 b2 = scan_excl(mine, sh.scan, all);
+    if (tid < 32 * VE && b2 <= in && in < b2 + mine) sh.where = first + tid;
+    __syncthreads();
+    return sh.where;
+  };
+  auto finish = [&](int at, u64 sum) {
+    if (at >= 0 && tid == 0) {
+      a.tok[r] = at;
+      if (a.logp) a.logp[r] = logp_of(sc, load_logit<T>(row, at), sum);
+    }
+    cluster_arrive();                          // peers may still read this block's histograms
+    cluster_wait();
+  };
+  u64 sum;
+  if (binned) {
+    // ---- nucleus: e is in the registers, the weights by bins are known; the bin that the limit falls into
+    // is put in order by the first block
+    u64 mine[2] = {0, 0};
+    uint32_t cnt[2] = {0, 0};
+    const int k0 = 2 * tid;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (k0 + q < EBINS) {
+        u64 low = 0;
+        for (int k = 0; k < C; ++k) {
+          cnt[q] += *peer(&sh.ecnt[k0 + q], k);
+          low += *peer(&sh.elow[k0 + q], k);
+        }
+        // e = mantissa * 2^(octave - 23), a weight counts 2^-40: 2^(17 + octave) of them a mantissa unit
+        const uint32_t bits = 0x3f800000u - ((uint32_t)(k0 + q) << EBITS);
+        const int up = 17 + (int)(bits >> 23) - 127;
+        const u64 base = (bits & 0x7fffffu) | 0x800000u;
+        mine[q] = up >= 0 ? (cnt[q] * base + low) << up : cnt[q] * (base >> -up) + low;
+      }
+    u64 all;
+    const u64 before = scan_excl(mine[0] + mine[1], sh.scan, all);
+    if (tid == 0) sh.where = -1;
+    __syncthreads();
+    if (before < limit && limit <= before + mine[0]) {
+      sh.where = k0;
+      sh.pick = limit - before;
+      sh.nlocal = cnt[0];
+    } else if (before + mine[0] < limit && limit <= before + mine[0] + mine[1]) {
+      sh.where = k0 + 1;
+      sh.pick = limit - before - mine[0];
+      sh.nlocal = cnt[1];
+    }
+    __syncthreads();
+    const int bin = sh.where, n = (int)sh.nlocal;
+    const u64 need = sh.pick;
+    if (bin >= 0 && n <= LIST) {               // the same in every block
+      const uint32_t q = (0x3f800000u >> EBITS) - (uint32_t)bin;
+      u64* list0 = peer(sh.list, 0);
+      uint32_t* n0 = peer(&sh.nlist, 0);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (__float_as_uint(v[j]) >> EBITS == q) {
+          const int idx = index_of(j);
+          list0[atomicAdd(n0, 1u)] = (u64)key_of(load_logit<T>(row, idx)) << 32 | (uint32_t)~idx;
+        }
+      cluster_arrive();
+      cluster_wait();
+      if (rank == 0) {
+        int N = 2;
+        while (N < n) N <<= 1;
+        for (int i = n + tid; i < N; i += THREADS) sh.list[i] = 0;
+        __syncthreads();
+        sort_desc(sh.list, N);
+        u64 w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) w[k] = k0 + k < n ? sc.w(logit_of((uint32_t)(sh.list[k0 + k] >> 32))) : 0;
+        u64 b = scan_excl(w[0] + w[1], sh.scan, all);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {          // the last one with less than `need` before it
+          if (k0 + k < n && b < need && need <= b + w[k])
+            for (int c = 0; c < C; ++c) *peer(&sh.cut, c) = sh.list[k0 + k];
+          b += w[k];
+        }
+        __syncthreads();
+      }
+      cluster_arrive();
+      cluster_wait();
+      const u64 last = sh.cut;
+      const int at = find(
+          [&](float e, int idx) -> float {
+            const uint32_t x = __float_as_uint(e) >> EBITS;
+            bool keep = x > q;
+            if (x == q) keep = ((u64)key_of(load_logit<T>(row, idx)) << 32 | (uint32_t)~idx) >= last;
+            return keep && e >= min_p ? e : 0.f;
+          },
+          sh.kept, [&](u64 t) { return draw_target(u, t); }, sum);
+      finish(at, sum);
+      return;
+    }
+    load_row();                                // a bin too full to be sorted: by keys
+  }
+  uint32_t kth = 0, pth = 0;
+  int pidx = V;
+  u64 left;
+  if (use_k) kth = search(true, 0u, (u64)top_k, left);
+  if (use_p) {
+    if (use_k) {
+      // total weight of the top k
+      u64 mine = 0;
+      each([&](float l, int) { if (key_of(l) >= kth) mine += sc.w(l); });
+      u64 all;
+      scan_excl(mine, sh.scan, all);
+      if (tid < C) *peer(&sh.total[rank], tid) = all;
+      cluster_arrive();
+      cluster_wait();
+      total_w = 0;
+      for (int k = 0; k < C; ++k) total_w += sh.total[k];
+      limit = (u64)ceil((double)top_p * (double)total_w);
+    }
+    pth = search(false, kth, limit, left);
+    // of the tokens with exactly this key the first ceil(left / weight) are kept
+    const u64 w1 = sc.w(logit_of(pth));
+    const u64 ties = w1 ? (left + w1 - 1) / w1 : 1;
+    u64 count;
+    // (a tie counts as the smallest weight, 2^-40)
+    const int at = find([&](float l, int) -> float { return key_of(l) == pth ? 9.094947017729282e-13f : 0.f; }, sh.kept,
+                        [&](u64 n) { return ties - 1 < n ? ties - 1 : n - 1; }, count);
+    if (at >= 0 && tid < C) *peer(&sh.first[0], tid) = (uint32_t)at;
+    cluster_arrive();
+    cluster_wait();
+    pidx = (int)sh.first[0];
+  }
+  const int at = find(
+      [&](float l, int idx) -> float {
+        const uint32_t k = key_of(l);
+        if (k < kth || k < pth || (k == pth && idx > pidx)) return 0.f;
+        const float e = sc.e(l);
+        return e >= min_p ? e : 0.f;
+      },
+      sh.total, [&](u64 n) { return draw_target(u, n); }, sum);
+  finish(at, sum);
+}
+
+template <class T, int NV>
+static cudaError_t launch_rows(const SampleArgs& a, int C, cudaStream_t st) {
+  static PerDeviceOnce attrs;
+  const cudaError_t ae = attrs.run([] {
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel<T, NV>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return e;
+  });
+  if (ae != cudaSuccess) return ae;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(a.R * C));
+  cfg.blockDim = dim3(smr::THREADS);
+  cfg.dynamicSmemBytes = sizeof(SampleShared);
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, NV>, a, C);
+}
+
+template <class T>
+static cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  const int nvec = (a.V + 2 * VE - 2) / VE;    // one more than the row's own where it starts off a boundary
+  // blocks per row: few rows are spread over all SMs (down to a vector a thread), many take as few blocks
+  // as hold a row at 32 values a thread, two blocks an SM
+  const int sms = device_attr(cudaDevAttrMultiProcessorCount, 148);
+  int C = 1;
+  while (C < smr::MAXC && ((nvec + C - 1) / C > smr::THREADS * (32 / VE) ||
+                           ((long long)a.R * C * 2 <= sms && (nvec + C - 1) / C > smr::THREADS)))
+    C <<= 1;
+  const int NV = ((nvec + C - 1) / C + smr::THREADS - 1) / smr::THREADS;
+  if (NV > 48 / VE) {
+    sample_long_kernel<T><<<a.R, smp::THREADS, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  if (NV <= 8 / VE) return launch_rows<T, 8 / VE>(a, C, st);
+  if (NV <= 16 / VE) return launch_rows<T, 16 / VE>(a, C, st);
+  if (NV <= 32 / VE) return launch_rows<T, 32 / VE>(a, C, st);
+  return launch_rows<T, 48 / VE>(a, C, st);
+}
+
 cudaError_t sample_launch(const SampleArgs& a, cudaStream_t st, bool pdl) {
   (void)pdl;
   if (a.R < 0 || a.V < 1 || a.ld < a.V || a.V > (1 << 24) || a.dtype < 0 || a.dtype > 2) return cudaErrorInvalidValue;
   if (a.R == 0) return cudaSuccess;
   if (!a.logits || !a.u || !a.tok) return cudaErrorInvalidValue;
   switch (a.dtype) {
-    case 0: sample_kernel<float><<<a.R, smp::THREADS, 0, st>>>(a); break;
-    case 1: sample_kernel<__half><<<a.R, smp::THREADS, 0, st>>>(a); break;
-    default: sample_kernel<__nv_bfloat16><<<a.R, smp::THREADS, 0, st>>>(a); break;
+    case 0: return launch_sample<float>(a, st);
+    case 1: return launch_sample<__half>(a, st);
+    default: return launch_sample<__nv_bfloat16>(a, st);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace af

@@ -12,7 +12,7 @@ from . import _runtime as R
 
 def _stream(t) -> int:
   import torch
-  return torch.cuda.current_stream(t.device).cuda_stream
+  return torch._C._cuda_getCurrentRawStream(t.get_device())       # a twentieth of current_stream(...).cuda_stream
 
 
 def _p(t) -> int:
@@ -239,14 +239,31 @@ def gemm_tc(x, tiles, scales, N, K, wf=R.W_I8, bias=None, epi=R.EPI_F32, y=None)
   return y
 
 
-_SAMPLE_DT = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-
-
 def _i32(t, shape, name):
   import torch
-  _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and tuple(t.shape) == tuple(shape),
-        f"{name} must be a contiguous int32 CUDA tensor of shape {tuple(shape)}")
+  if not (t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.shape == shape):
+    raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of shape {tuple(shape)}")
   return t.data_ptr()
+
+
+_SAMPLE_DT = {}
+
+
+def _sample_types():
+  if not _SAMPLE_DT:
+    import torch
+    _SAMPLE_DT.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+  return _SAMPLE_DT
+
+
+def _per_row(x, name, dtype, rows):
+  """A setting as (pointer of its row values, 0) or (0, the number for all rows)."""
+  if hasattr(x, "data_ptr"):
+    if not (x.is_cuda and x.dtype == dtype and x.shape == rows and x.is_contiguous()):
+      raise ValueError(f"{name} must be a number or a contiguous {dtype} CUDA tensor [R]")
+    return x.data_ptr(), 0
+  _need(x == x and abs(x) != float("inf"), f"{name} must be finite")
+  return 0, (max(-1, min(int(x), 0x7fffffff)) if name == "top_k" else x)
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
@@ -258,32 +275,31 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
   (tokens int32 [R], log-probabilities among the kept tokens fp32 [R]); -1 and -inf for a row that is all -inf
   or NaN. `out` = the two outputs, preallocated."""
   import torch
-  _need(logits.is_cuda and logits.dim() == 2 and logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-        "logits must be a 2-D CUDA tensor whose rows are contiguous")
-  dt = _SAMPLE_DT.get(str(logits.dtype))
-  _need(dt is not None, "logits must be fp32, fp16 or bf16")
+  if not (logits.is_cuda and logits.dim() == 2 and logits.dtype in _sample_types()):
+    raise ValueError("logits must be a 2-D CUDA tensor of fp32, fp16 or bf16")
   n, V = logits.shape
-  _need(V <= 1 << 24, "at most 2^24 logits in a row")
-  ld = logits.stride(0) if n > 1 else V
+  ld, col = logits.stride()
+  _need(1 <= V <= 1 << 24 and (col == 1 or V == 1), "logits must have contiguous rows of 1 to 2^24 values")
+  if n <= 1:
+    ld = V
   _need(ld >= V, "rows of logits must not overlap")
-  _need(u.is_cuda and u.dtype == torch.float32 and u.is_contiguous() and u.shape == (n,), "u must be fp32 [R] on the GPU")
-  ptr, val = [], []
-  for x, name, want in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
-                        (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
-    if isinstance(x, torch.Tensor):
-      _need(x.is_cuda and x.dtype == want and x.is_contiguous() and x.shape == (n,), f"{name} must be {want} [R] on the GPU")
-      ptr.append(x.data_ptr()); val.append(0)
-    else:
-      _need(x == x and abs(x) != float("inf"), f"{name} must be finite")
-      ptr.append(0); val.append(x)
+  rows = (n,)
+  _need(u.is_cuda and u.dtype == torch.float32 and u.shape == rows and u.is_contiguous(), "u must be fp32 [R] on the GPU")
+  pt, st = _per_row(temperature, "temperature", torch.float32, rows)
+  pk, sk = _per_row(top_k, "top_k", torch.int32, rows)
+  pp, sp = _per_row(top_p, "top_p", torch.float32, rows)
+  pm, sm = _per_row(min_p, "min_p", torch.float32, rows)
   if out is None:
-    out = torch.empty((n,), dtype=torch.int32, device=u.device), torch.empty((n,), dtype=torch.float32, device=u.device)
+    tok, logp = torch.empty_like(u, dtype=torch.int32), torch.empty_like(u)
   else:
-    _need(out[0].dtype == torch.int32 and out[1].dtype == torch.float32 and all(o.shape == (n,) and o.is_contiguous() for o in out),
-          "out must be (int32 [R], fp32 [R])")
-  R.check(R.lib().af_sample(logits.data_ptr(), dt, ld, n, V, u.data_ptr(), *ptr, float(val[0]), int(val[1]), float(val[2]),
-                            float(val[3]), out[0].data_ptr(), out[1].data_ptr(), _stream(logits)), "af_sample")
-  return out
+    tok, logp = out
+    _need(tok.dtype == torch.int32 and logp.dtype == torch.float32 and all(o.is_cuda and o.shape == rows and o.is_contiguous() for o in out),
+          "out must be (int32 [R], fp32 [R]) on the GPU")
+  rc = R.lib().af_sample(logits.data_ptr(), _SAMPLE_DT[logits.dtype], ld, n, V, u.data_ptr(), pt, pk, pp, pm, st, sk, sp, sm,
+                         tok.data_ptr(), logp.data_ptr(), _stream(logits))
+  if rc:
+    R.check(rc, "af_sample")
+  return tok, logp
 
 
 def tree_layout(parents):
