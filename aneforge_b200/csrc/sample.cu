@@ -210,12 +210,14 @@ __global__ void __launch_bounds__(smp::THREADS) sample_long_kernel(SampleArgs a)
 // weight), only the bin that the limit falls into is sorted, and the kept sums come from the registers.
 namespace smr {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
-constexpr int BINS = 128;                      // 16 nats
-constexpr int LIST = 1024;                     // tokens that the first block sorts
-constexpr int LOCAL = 3072;                    // listed tokens of one block
+constexpr int BINS = 256;                      // 32 nats: what lies further below weighs nothing
+constexpr int LIST = 1024;                     // tokens that one block puts in order: LIST / C from each
+constexpr int PAIRS = 256;                     // up to so many by comparing all pairs
+constexpr int LOCAL = 3200;                    // listed tokens of one block
 constexpr int MAXC = 16;
-// nucleus: weights by the upper bits of e (32 bins an octave, bin 0 is e = 1), down to 2^-24
-constexpr int EBITS = 18, EBINS = 24 * 32 + 1;
+// nucleus: weights by the upper bits of e (128 bins an octave, bin 0 is e = 1), down to 2^-24
+constexpr int EBITS = 16, EBINS = 24 * 128 + 1;
+static_assert(EBINS <= LOCAL, "the bins' weights are summed in the local list's place");
 }  // namespace smr
 
 struct SampleShared {
@@ -229,13 +231,13 @@ struct SampleShared {
   u64 radix[2][256];
   u64 sums[smr::WARPS * 12];                   // kept weight (or ties) of a (vector, warp)
   u64 scan[smr::WARPS];
-  u64 list[smr::LIST];                         // key << 32 | ~index, of the whole row (first block)
+  u64 list[smr::LIST];                         // key << 32 | ~index, LIST / C from each block of the cluster
   u64 local[smr::LOCAL];                       // the same, of this block
-  uint32_t nlist, nlocal, kloc, floc;
+  uint32_t nlocal, kloc, floc, in_bin;
   u64 pick;
   u64 total_w;
-  u64 cut;                                     // the nucleus' last token, key << 32 | ~index
-  int where;
+  u64 need;                                    // weight that the nucleus takes from its last bin
+  int where, bin;
 };
 
 AF_DEV float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
@@ -307,6 +309,161 @@ AF_DEV u64 draw_target(float u, u64 total) {
 }
 AF_DEV float logp_of(const RowScale& sc, float l, u64 total) { return sc.below(l) - logf((float)total / 1099511627776.f); }
 
+// the blocks' shares of the list one after the other, into `local`
+AF_DEV void gather(SampleShared& sh, int C, int share) {
+  for (int i = threadIdx.x; i < C * share; i += smr::THREADS) {
+    const int k = i / share, j = i - k * share;
+    int off = 0;
+    for (int q = 0; q < k; ++q) off += (int)sh.count[q];
+    if (j < (int)sh.count[k]) sh.local[off + j] = sh.list[i];
+  }
+  __syncthreads();
+}
+
+// The last token in order (falling key, rising index) with less than `need` of the weight before it, of
+// the n <= LIST in `local`; by comparing all pairs, or by sorting where those are many.
+AF_DEV u64 last_of(SampleShared& sh, const RowScale& sc, int n, u64 need) {
+  using namespace smr;
+  const int tid = threadIdx.x;
+  if (n <= PAIRS) {
+    int pad = 16;
+    while (pad < n) pad <<= 1;
+    const int L = THREADS / pad, i = tid / L, part = tid % L;
+    for (int k = tid; k < n; k += THREADS) sh.list[k] = sc.w(logit_of((uint32_t)(sh.local[k] >> 32)));
+    __syncthreads();
+    const u64 x = i < n ? sh.local[i] : ~0ull;
+    u64 before = 0;
+    for (int j = part; j < n; j += L)
+      if (sh.local[j] > x) before += sh.list[j];
+    for (int o = L >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (part == 0 && i < n && before < need && need <= before + sh.list[i]) sh.pick = x;
+    __syncthreads();
+    return sh.pick;
+  }
+  int N = 2;
+  while (N < n) N <<= 1;
+  for (int k = tid; k < N; k += THREADS) sh.list[k] = k < n ? sh.local[k] : 0;
+  __syncthreads();
+  sort_desc(sh.list, N);
+  u64 w[2], all;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) w[k] = 2 * tid + k < n ? sc.w(logit_of((uint32_t)(sh.list[2 * tid + k] >> 32))) : 0;
+  u64 b = scan_excl(w[0] + w[1], sh.scan, all);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (2 * tid + k < n && b < need && need <= b + w[k]) sh.pick = sh.list[2 * tid + k];
+    b += w[k];
+  }
+  __syncthreads();
+  return sh.pick;
+}
+
+// The whole choice among the n <= LIST tokens in `local`, which hold every token that may be kept (k 0: no
+// top-k; without it `limit` is the nucleus' weight).
+AF_DEV void few_tokens(const SampleArgs& a, SampleShared& sh, const RowScale& sc, int r, int n, int k, bool use_p, float top_p,
+                       float min_p, float u, u64 limit) {
+  using namespace smr;
+  const int tid = threadIdx.x;
+  u64 sum;
+  if (n <= PAIRS) {
+    int pad = 16;
+    while (pad < n) pad <<= 1;
+    const int L = THREADS / pad, i = tid / L, part = tid % L;
+    for (int q = tid; q < n; q += THREADS) sh.list[q] = sc.w(logit_of((uint32_t)(sh.local[q] >> 32)));
+    __syncthreads();
+    const u64 x = i < n ? sh.local[i] : ~0ull;
+    const uint32_t key = (uint32_t)(x >> 32);
+    u64 before = 0;
+    int over = 0;                              // larger logits
+    for (int j = part; j < n; j += L) {
+      const u64 y = sh.local[j];
+      if (y > x) before += sh.list[j];
+      over += (uint32_t)(y >> 32) > key;
+    }
+    for (int o = L >> 1; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      over += __shfl_xor_sync(0xffffffffu, over, o);
+    }
+    const bool mine = part == 0 && i < n;
+    const bool in_k = mine && (k == 0 || over < k);
+    const u64 w = in_k ? sh.list[i] : 0;
+    if (k && use_p) {
+      scan_excl(w, sh.scan, sum);
+      limit = (u64)ceil((double)top_p * (double)sum);
+    }
+    const u64 kept = in_k && (!use_p || before < limit) && sc.e(logit_of(key)) >= min_p ? w : 0;
+    scan_excl(kept, sh.scan, sum);             // also the barrier before the weights are replaced
+    if (mine) sh.list[i] = kept;
+    __syncthreads();
+    const u64 target = draw_target(u, sum);
+    before = 0;
+    for (int j = part; j < n; j += L)
+      if ((uint32_t)sh.local[j] > (uint32_t)x) before += sh.list[j];       // a lower index: the complement is larger
+    for (int o = L >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (mine && before <= target && target < before + kept) {
+      a.tok[r] = (int)~(uint32_t)x;
+      if (a.logp) a.logp[r] = logp_of(sc, logit_of(key), sum);
+    }
+    return;
+  }
+  int N = 2;
+  while (N < n) N <<= 1;
+  for (int q = tid; q < N; q += THREADS) sh.list[q] = q < n ? sh.local[q] : 0;
+  __syncthreads();
+  sort_desc(sh.list, N);
+  const uint32_t kth = k && k <= n ? (uint32_t)(sh.list[k - 1] >> 32) : 0u;
+  const int p0 = 2 * tid;
+  u64 w[2], mine = 0;
+  float e[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t key = p0 + q < n ? (uint32_t)(sh.list[p0 + q] >> 32) : 0u;
+    const bool ok = p0 + q < n && key >= kth;
+    e[q] = ok ? sc.e(logit_of(key)) : -1.f;
+    w[q] = ok ? (u64)(e[q] * 1099511627776.f) : 0;
+    mine += w[q];
+  }
+  u64 before = scan_excl(mine, sh.scan, sum);
+  if (use_p && k) limit = (u64)ceil((double)top_p * (double)sum);
+  u64 kept = 0;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const bool ok = e[q] >= 0.f && (!use_p || before < limit) && e[q] >= min_p;
+    before += w[q];
+    if (!ok) w[q] = 0;
+    kept += w[q];
+  }
+  scan_excl(kept, sh.scan, sum);
+  // the kept ones in index order: ~index << 32 | key, descending
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+    if (p0 + q < N) {
+      const u64 x = sh.list[p0 + q];
+      sh.list[p0 + q] = w[q] ? (x << 32 | x >> 32) : 0;
+    }
+  __syncthreads();
+  sort_desc(sh.list, N);
+  mine = 0;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const u64 x = p0 + q < N ? sh.list[p0 + q] : 0;
+    w[q] = x ? sc.w(logit_of((uint32_t)x)) : 0;
+    mine += w[q];
+  }
+  const u64 target = draw_target(u, sum);
+  u64 all;
+  before = scan_excl(mine, sh.scan, all);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if (before <= target && target < before + w[q]) {
+      const u64 x = sh.list[p0 + q];
+      a.tok[r] = (int)~(uint32_t)(x >> 32);
+      if (a.logp) a.logp[r] = logp_of(sc, logit_of((uint32_t)x), sum);
+    }
+    before += w[q];
+  }
+}
+
 template <class T, int NV>
 __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ? 2 : 1) sample_kernel(SampleArgs a, int C) {
   using namespace smr;
@@ -315,9 +472,13 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / C, rank = blockIdx.x % C, V = a.V;
+  const float temp = a.temperature ? __ldg(a.temperature + r) : a.temperature_s;
+  const int top_k = a.top_k ? __ldg(a.top_k + r) : a.top_k_s;
+  const float top_p = a.top_p ? __ldg(a.top_p + r) : a.top_p_s;
+  const float min_p = fminf(a.min_p ? __ldg(a.min_p + r) : a.min_p_s, 1.f);
+  const float u = __ldg(a.u + r);
   if (tid < BINS) sh.hist[tid] = 0;
-  for (int k = tid; k < EBINS; k += THREADS) sh.ecnt[k] = sh.elow[k] = 0;
-  if (tid == 0) { sh.nlist = 0; sh.nlocal = 0; sh.kloc = 0; sh.floc = 0xffffffffu; }
+  if (tid == 0) { sh.nlocal = 0; sh.kloc = 0; sh.floc = 0xffffffffu; sh.in_bin = 0; sh.bin = -1; }
   __syncthreads();
   cluster_arrive();                            // the others may write here from their first wait on
   // ---- the row: vectors from the 16-byte boundary at or before its start, this block's share of them
@@ -344,6 +505,9 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   };
   load_row();
   auto index_of = [&](int j) { return (rank * per + (j / VE) * THREADS + tid) * VE - skip + j % VE; };
+  const bool use_k = top_k > 0 && top_k < V, use_p = top_p > 0.f && top_p < 1.f, use_m = min_p > 0.f;
+  if (use_p && !use_k)                         // while the row is on its way
+    for (int k = tid; k < EBINS; k += THREADS) sh.ecnt[k] = sh.elow[k] = 0;
   {
     float m = -INFINITY;
 #pragma unroll
@@ -358,11 +522,6 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   cluster_wait();
   kmax = sh.kmax[0];
   for (int k = 1; k < C; ++k) kmax = max(kmax, sh.kmax[k]);
-  const float temp = a.temperature ? a.temperature[r] : a.temperature_s;
-  const int top_k = a.top_k ? a.top_k[r] : a.top_k_s;
-  const float top_p = a.top_p ? a.top_p[r] : a.top_p_s;
-  const float min_p = fminf(a.min_p ? a.min_p[r] : a.min_p_s, 1.f);
-  const float u = a.u[r];
   RowScale sc;
   sc.lmax = logit_of(kmax);
   sc.temp = temp > 0.f ? temp : 1.f;
@@ -393,14 +552,13 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     }
     return;
   }
-  const bool use_k = top_k > 0 && top_k < V, use_p = top_p > 0.f && top_p < 1.f, use_m = min_p > 0.f;
   // ---- how far below the maximum the logits lie; total weight
   const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
   const float scale = 8.f / sc.temp;
   float cut = -INFINITY;                       // no token under `cut` can be kept
   u64 total_w = 0, limit = 0;
-  // the nucleus of a whole row: e takes the logits' place (a block's 2^14 values keep a bin's sum in 32 bits)
-  const bool binned = use_p && !use_k && !far && E <= 32;
+  // the nucleus of a whole row: e takes the logits' place (a block's 2^15 values keep a bin's sum in 32 bits)
+  const bool binned = use_p && !use_k && !far;
   if (use_p && !use_k) {
     uint32_t hi = 0, lo = 0;
     auto add = [&](float e) {
@@ -469,7 +627,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     __syncthreads();
     if (before < (u64)top_k && (u64)top_k <= before + n) sh.where = tid;
     __syncthreads();
-    if (sh.where < BINS) cut = -(float)(sh.where + 1);       // a distance, see below
+    cut = -(float)(min(sh.where, BINS - 1) + 1);             // a distance, see below; fewer than k weigh anything: all of those
   } else if (use_m && !use_p && !use_k && !far) {
     cut = -(-8.f * logf(min_p) * 1.0001f + 1.f);
   }
@@ -477,103 +635,40 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   auto may = [&](float l) { return cut == -INFINITY || (sc.lmax - l) * scale < -cut; };
   // ---- list the tokens that may be kept
   bool listed = false, small = false;
-  uint32_t n_local = 0;
+  uint32_t n_local = 0, n_all = 0;
+  const int share = LIST / C;                  // of sh.list, for each block
   if (cut != -INFINITY) {
-    u64* list0 = peer(sh.list, 0);
-    uint32_t* n0 = peer(&sh.nlist, 0);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const bool yes = may(v[j]);
       const unsigned who = __ballot_sync(0xffffffffu, yes);
       if (!who) continue;
-      uint32_t at = 0, at0 = 0;
-      if (lane == 0) {
-        at = atomicAdd(&sh.nlocal, (uint32_t)__popc(who));
-        if (at < (uint32_t)LIST) at0 = atomicAdd(n0, (uint32_t)__popc(who));
-      }
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&sh.nlocal, (uint32_t)__popc(who));
       at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
-      at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(who & ((1u << lane) - 1));
-      if (yes) {
-        const u64 x = (u64)key_of(v[j]) << 32 | (uint32_t)~index_of(j);
-        if (at < (uint32_t)LOCAL) sh.local[at] = x;
-        if (at < (uint32_t)LIST && at0 < (uint32_t)LIST) list0[at0] = x;
-      }
+      if (yes && at < (uint32_t)LOCAL) sh.local[at] = (u64)key_of(v[j]) << 32 | (uint32_t)~index_of(j);
     }
     __syncthreads();
     n_local = sh.nlocal;
+    if (n_local <= (uint32_t)share) {
+      u64* list0 = peer(sh.list + rank * share, 0);
+      for (uint32_t i = tid; i < n_local; i += THREADS) list0[i] = sh.local[i];
+    }
     if (tid < C) *peer(&sh.count[rank], tid) = n_local;
     cluster_arrive();
     cluster_wait();
-    uint32_t all = 0;
     bool fits = true;
+    small = true;                              // the same answers in every block
     for (int k = 0; k < C; ++k) {
-      all += sh.count[k];
+      n_all += sh.count[k];
       fits &= sh.count[k] <= (uint32_t)LOCAL;
+      small &= sh.count[k] <= (uint32_t)share;
     }
-    small = all <= (uint32_t)LIST;
-    listed = fits;                             // the same answer in every block
+    listed = fits;
     if (small) {
       if (rank) return;                        // nobody reads the other blocks' memory any more
-      const int n = (int)all;
-      int N = 2;
-      while (N < n) N <<= 1;
-      for (int i = n + tid; i < N; i += THREADS) sh.list[i] = 0;
-      __syncthreads();
-      sort_desc(sh.list, N);
-      const uint32_t kth = use_k ? (uint32_t)(sh.list[top_k - 1] >> 32) : 0u;
-      const int p0 = 2 * tid;
-      u64 w[2];
-      float e[2];
-      u64 mine = 0;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t key = p0 + k < n ? (uint32_t)(sh.list[p0 + k] >> 32) : 0u;
-        const bool ok = p0 + k < n && key >= kth;
-        e[k] = ok ? sc.e(logit_of(key)) : 0.f;
-        w[k] = ok ? (u64)(e[k] * 1099511627776.f) : 0;
-        if (!ok) e[k] = -1.f;
-        mine += w[k];
-      }
-      u64 sum;
-      u64 before = scan_excl(mine, sh.scan, sum);
-      if (use_p && use_k) limit = (u64)ceil((double)top_p * (double)sum);
-      u64 kept = 0;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bool ok = e[k] >= 0.f && (!use_p || before < limit) && e[k] >= min_p;
-        before += w[k];
-        if (!ok) w[k] = 0;
-        kept += w[k];
-      }
-      scan_excl(kept, sh.scan, sum);
-      // the kept ones in index order: index << 32 | key, ascending as the complement descends
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (p0 + k < N) {
-          const u64 x = sh.list[p0 + k];
-          sh.list[p0 + k] = w[k] ? (x << 32 | x >> 32) : 0;      // ~index << 32 | key, descending
-        }
-      __syncthreads();
-      sort_desc(sh.list, N);
-      mine = 0;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const u64 x = p0 + k < N ? sh.list[p0 + k] : 0;
-        w[k] = x ? sc.w(logit_of((uint32_t)x)) : 0;
-        mine += w[k];
-      }
-      const u64 target = draw_target(u, sum);
-      u64 all_w;
-      before = scan_excl(mine, sh.scan, all_w);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (before <= target && target < before + w[k]) {
-          const u64 x = sh.list[p0 + k];
-          a.tok[r] = (int)~(uint32_t)(x >> 32);
-          if (a.logp) a.logp[r] = logp_of(sc, logit_of((uint32_t)x), sum);
-        }
-        before += w[k];
-      }
+      gather(sh, C, share);
+      few_tokens(a, sh, sc, r, (int)n_all, use_k ? top_k : 0, use_p, top_p, min_p, u, use_k ? 0 : limit);
       return;
     }
   }
@@ -707,74 +802,72 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   };
   u64 sum;
   if (binned) {
-    // ---- nucleus: e is in the registers, the weights by bins are known; the bin that the limit falls into
-    // is put in order by the first block
-    u64 mine[2] = {0, 0};
-    uint32_t cnt[2] = {0, 0};
-    const int k0 = 2 * tid;
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (k0 + q < EBINS) {
-        u64 low = 0;
-        for (int k = 0; k < C; ++k) {
-          cnt[q] += *peer(&sh.ecnt[k0 + q], k);
-          low += *peer(&sh.elow[k0 + q], k);
-        }
-        // e = mantissa * 2^(octave - 23), a weight counts 2^-40: 2^(17 + octave) of them a mantissa unit
-        const uint32_t bits = 0x3f800000u - ((uint32_t)(k0 + q) << EBITS);
-        const int up = 17 + (int)(bits >> 23) - 127;
-        const u64 base = (bits & 0x7fffffu) | 0x800000u;
-        mine[q] = up >= 0 ? (cnt[q] * base + low) << up : cnt[q] * (base >> -up) + low;
+    // ---- nucleus: e is in the registers, the blocks' bins are filled. Each block adds up its share of the
+    // bins over the cluster; the one whose share the limit falls into tells the others which bin it is
+    const int bins = (EBINS + C - 1) / C, b0 = rank * bins, b1 = min(EBINS, b0 + bins);
+    for (int b = b0 + tid; b < b1; b += THREADS) {
+      u64 cnt = 0, low = 0;
+#pragma unroll 4
+      for (int k = 0; k < C; ++k) {
+        cnt += *peer(&sh.ecnt[b], k);
+        low += *peer(&sh.elow[b], k);
       }
-    u64 all;
-    const u64 before = scan_excl(mine[0] + mine[1], sh.scan, all);
-    if (tid == 0) sh.where = -1;
-    __syncthreads();
-    if (before < limit && limit <= before + mine[0]) {
-      sh.where = k0;
-      sh.pick = limit - before;
-      sh.nlocal = cnt[0];
-    } else if (before + mine[0] < limit && limit <= before + mine[0] + mine[1]) {
-      sh.where = k0 + 1;
-      sh.pick = limit - before - mine[0];
-      sh.nlocal = cnt[1];
+      // e = mantissa * 2^(octave - 23), a weight counts 2^-40: 2^(17 + octave) of them a mantissa unit
+      const uint32_t bits = 0x3f800000u - ((uint32_t)b << EBITS);
+      const int up = 17 + (int)(bits >> 23) - 127;
+      const u64 base = (bits & 0x7fffffu) | 0x800000u;
+      sh.local[b - b0] = up >= 0 ? (cnt * base + low) << up : cnt * (base >> -up) + low;
     }
     __syncthreads();
-    const int bin = sh.where, n = (int)sh.nlocal;
-    const u64 need = sh.pick;
-    if (bin >= 0 && n <= LIST) {               // the same in every block
-      const uint32_t q = (0x3f800000u >> EBITS) - (uint32_t)bin;
-      u64* list0 = peer(sh.list, 0);
-      uint32_t* n0 = peer(&sh.nlist, 0);
+    const int run = (bins + THREADS - 1) / THREADS, k0 = b0 + tid * run;
+    u64 mine = 0, all;
+    for (int k = k0; k < min(k0 + run, b1); ++k) mine += sh.local[k - b0];
+    u64 before = scan_excl(mine, sh.scan, all);
+    if (tid < C) *peer(&sh.kept[rank], tid) = all;
+    cluster_arrive();
+    cluster_wait();
+    for (int k = 0; k < rank; ++k) before += sh.kept[k];
+    if (before < limit && limit <= before + mine)
+      for (int k = k0; k < min(k0 + run, b1); ++k) {
+        const u64 w = sh.local[k - b0];
+        if (before < limit && limit <= before + w)
+          for (int c = 0; c < C; ++c) {
+            *peer(&sh.bin, c) = k;
+            *peer(&sh.need, c) = limit - before;
+          }
+        before += w;
+      }
+    cluster_arrive();
+    cluster_wait();
+    // its tokens, to every block
+    const int bin = sh.bin;
+    const u64 need = sh.need;
+    const uint32_t q = (0x3f800000u >> EBITS) - (uint32_t)bin;
+    if (bin >= 0) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (__float_as_uint(v[j]) >> EBITS == q) {
+          const uint32_t at = atomicAdd(&sh.in_bin, 1u);
           const int idx = index_of(j);
-          list0[atomicAdd(n0, 1u)] = (u64)key_of(load_logit<T>(row, idx)) << 32 | (uint32_t)~idx;
+          if (at < (uint32_t)share) sh.local[at] = (u64)key_of(load_logit<T>(row, idx)) << 32 | (uint32_t)~idx;
         }
-      cluster_arrive();
-      cluster_wait();
-      if (rank == 0) {
-        int N = 2;
-        while (N < n) N <<= 1;
-        for (int i = n + tid; i < N; i += THREADS) sh.list[i] = 0;
-        __syncthreads();
-        sort_desc(sh.list, N);
-        u64 w[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) w[k] = k0 + k < n ? sc.w(logit_of((uint32_t)(sh.list[k0 + k] >> 32))) : 0;
-        u64 b = scan_excl(w[0] + w[1], sh.scan, all);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {          // the last one with less than `need` before it
-          if (k0 + k < n && b < need && need <= b + w[k])
-            for (int c = 0; c < C; ++c) *peer(&sh.cut, c) = sh.list[k0 + k];
-          b += w[k];
-        }
-        __syncthreads();
-      }
-      cluster_arrive();
-      cluster_wait();
-      const u64 last = sh.cut;
+      __syncthreads();
+      const int n = (int)sh.in_bin;
+      if (n <= share)
+        for (int i = tid; i < n * C; i += THREADS) *peer(&sh.list[rank * share + i / C], i % C) = sh.local[i / C];
+      if (tid < C) *peer(&sh.count[rank], tid) = (uint32_t)n;
+    }
+    cluster_arrive();
+    cluster_wait();
+    bool fit = bin >= 0;
+    int n_bin = 0;
+    for (int k = 0; fit && k < C; ++k) {
+      fit = sh.count[k] <= (uint32_t)share;
+      n_bin += (int)sh.count[k];
+    }
+    if (fit) {                                 // the same in every block
+      gather(sh, C, share);
+      const u64 last = last_of(sh, sc, n_bin, need);
       const int at = find(
           [&](float e, int idx) -> float {
             const uint32_t x = __float_as_uint(e) >> EBITS;
@@ -791,7 +884,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   uint32_t kth = 0, pth = 0;
   int pidx = V;
   u64 left;
-  if (use_k) kth = search(true, 0u, (u64)top_k, left);
+  if (use_k && (!listed || (uint32_t)top_k <= n_all)) kth = search(true, 0u, (u64)top_k, left);
   if (use_p) {
     if (use_k) {
       // total weight of the top k
