@@ -233,6 +233,7 @@ struct SampleShared {
   u64 scan[smr::WARPS];
   u64 list[smr::LIST];                         // key << 32 | ~index, LIST / C from each block of the cluster
   u64 local[smr::LOCAL];                       // the same, of this block
+  u64 mine[smr::LIST];                         // this block's tokens in the nucleus' last bin
   uint32_t nlocal, kloc, floc, in_bin;
   u64 pick;
   u64 total_w;
@@ -557,6 +558,16 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   const float scale = 8.f / sc.temp;
   float cut = -INFINITY;                       // no token under `cut` can be kept
   u64 total_w = 0, limit = 0;
+  // e in the logits' place (past the row's end: 0)
+  auto to_e = [&] {
+    if (sc.temp == 1.f) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = expf(v[j] - sc.zmax);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = expf(__fdiv_rn(v[j], sc.temp) - sc.zmax);
+    }
+  };
   // the nucleus of a whole row: e takes the logits' place (a block's 2^15 values keep a bin's sum in 32 bits)
   const bool binned = use_p && !use_k && !far;
   if (use_p && !use_k) {
@@ -568,13 +579,9 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
       lo += l;
     };
     if (binned) {
-      if (sc.temp == 1.f) {
+      to_e();
 #pragma unroll
-        for (int j = 0; j < E; ++j) add(v[j] = expf(v[j] - sc.zmax));
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) add(v[j] = expf(__fdiv_rn(v[j], sc.temp) - sc.zmax));
-      }
+      for (int j = 0; j < E; ++j) add(v[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j) add(sc.e(v[j]));
@@ -801,6 +808,91 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     cluster_wait();
   };
   u64 sum;
+  // the draw where e is in the registers: kept are the tokens whose e has at least the bits `least`, and of
+  // the n_in in `mine` those from `last` on
+  auto draw_e = [&](uint32_t least, int n_in, u64 last) {
+    auto extra = [&](int i, int& vi, int& idx) -> u64 {
+      const u64 x = sh.mine[i];
+      const float e = sc.e(logit_of((uint32_t)(x >> 32)));
+      idx = (int)~(uint32_t)x;
+      vi = (idx + skip) / VE - rank * per;
+      return x >= last && e >= min_p ? (u64)(e * 1099511627776.f) : 0;
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t hi = 0, lo = 0;                 // 32 * VE values of at most 2^20 each
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        const float e = v[i * VE + k];
+        uint32_t h, l;
+        weight_parts(__float_as_uint(e) >= least ? e : 0.f, h, l);
+        hi += h;
+        lo += l;
+      }
+      hi = __reduce_add_sync(0xffffffffu, hi);
+      lo = __reduce_add_sync(0xffffffffu, lo);
+      if (lane == 0) sh.sums[i * WARPS + warp] = ((u64)hi << 20) + lo;
+    }
+    __syncthreads();
+    for (int i = tid; i < n_in; i += THREADS) {
+      int vi, idx;
+      const u64 w = extra(i, vi, idx);
+      if (w) atomicAdd(&sh.sums[(vi / THREADS) * WARPS + (vi % THREADS) / 32], w);
+    }
+    __syncthreads();
+    u64 mine = tid < NV * WARPS ? sh.sums[tid] : 0, all;
+    u64 before = scan_excl(mine, sh.scan, all);
+    if (tid < C) *peer(&sh.total[rank], tid) = all;
+    if (tid == 0) sh.where = -1;
+    cluster_arrive();
+    cluster_wait();
+    u64 base = 0;
+    sum = 0;
+    for (int k = 0; k < C; ++k) {
+      if (k < rank) base += sh.total[k];
+      sum += sh.total[k];
+    }
+    // nobody reads another block's memory from here on
+    const u64 target = draw_target(u, sum);
+    if (target < base || target >= base + all) return;
+    before += base;
+    if (tid < NV * WARPS && before <= target && target < before + mine) {
+      sh.where = tid;
+      sh.pick = target - before;
+    }
+    __syncthreads();
+    const int cell = sh.where;
+    const u64 in = sh.pick;
+    // the 32 * VE consecutive tokens of one (vector, warp)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * WARPS + warp == cell) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          const float e = v[i * VE + k];
+          sh.list[lane * VE + k] = __float_as_uint(e) >= least ? (u64)(e * 1099511627776.f) : 0;
+        }
+      }
+    __syncthreads();
+    for (int i = tid; i < n_in; i += THREADS) {
+      int vi, idx;
+      const u64 w = extra(i, vi, idx);
+      if (w && (vi / THREADS) * WARPS + (vi % THREADS) / 32 == cell) sh.list[(vi % 32) * VE + (idx + skip) % VE] = w;
+    }
+    __syncthreads();
+    mine = tid < 32 * VE ? sh.list[tid] : 0;
+    before = scan_excl(mine, sh.scan, all);
+    if (tid < 32 * VE && before <= in && in < before + mine) {
+      const int at = (rank * per + (cell / WARPS) * THREADS + (cell % WARPS) * 32) * VE - skip + tid;
+      a.tok[r] = at;
+      if (a.logp) a.logp[r] = logp_of(sc, load_logit<T>(row, at), sum);
+    }
+  };
+  if (!use_k && !use_p && !far) {
+    to_e();
+    draw_e(use_m ? __float_as_uint(min_p) : 0u, 0, 0);
+    return;
+  }
   if (binned) {
     // ---- nucleus: e is in the registers, the blocks' bins are filled. Each block adds up its share of the
     // bins over the cluster; the one whose share the limit falls into tells the others which bin it is
@@ -848,13 +940,16 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
       for (int j = 0; j < E; ++j)
         if (__float_as_uint(v[j]) >> EBITS == q) {
           const uint32_t at = atomicAdd(&sh.in_bin, 1u);
-          const int idx = index_of(j);
-          if (at < (uint32_t)share) sh.local[at] = (u64)key_of(load_logit<T>(row, idx)) << 32 | (uint32_t)~idx;
+          if (at < (uint32_t)share) sh.mine[at] = (uint32_t)~index_of(j);
         }
       __syncthreads();
       const int n = (int)sh.in_bin;
       if (n <= share)
-        for (int i = tid; i < n * C; i += THREADS) *peer(&sh.list[rank * share + i / C], i % C) = sh.local[i / C];
+        for (int i = tid; i < n; i += THREADS) {
+          const u64 x = (u64)key_of(load_logit<T>(row, (int)~(uint32_t)sh.mine[i])) << 32 | (uint32_t)sh.mine[i];
+          sh.mine[i] = x;
+          for (int c = 0; c < C; ++c) *peer(&sh.list[rank * share + i], c) = x;
+        }
       if (tid < C) *peer(&sh.count[rank], tid) = (uint32_t)n;
     }
     cluster_arrive();
@@ -868,15 +963,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     if (fit) {                                 // the same in every block
       gather(sh, C, share);
       const u64 last = last_of(sh, sc, n_bin, need);
-      const int at = find(
-          [&](float e, int idx) -> float {
-            const uint32_t x = __float_as_uint(e) >> EBITS;
-            bool keep = x > q;
-            if (x == q) keep = ((u64)key_of(load_logit<T>(row, idx)) << 32 | (uint32_t)~idx) >= last;
-            return keep && e >= min_p ? e : 0.f;
-          },
-          sh.kept, [&](u64 t) { return draw_target(u, t); }, sum);
-      finish(at, sum);
+      draw_e(max((q + 1) << EBITS, __float_as_uint(fmaxf(min_p, 0.f))), (int)sh.in_bin, last);
       return;
     }
     load_row();                                // a bin too full to be sorted: by keys
