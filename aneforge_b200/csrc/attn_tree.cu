@@ -42,6 +42,15 @@ __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
   // triggered after the wait: a dependent that starts now may read everything written before this kernel
   pdl_wait();
   pdl_trigger();
+  // the row, the extent and the depth are on their way together
+  float rc[EPL], rs[EPL], v[EPL], vv[EPL];
+  const float* x = a.qkv + (size_t)row * a.ld_qkv;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    v[e] = active ? __ldcg(x + (size_t)y * DH + lane * EPL + e) : 0.f;
+    vv[e] = active && y >= a.H ? __ldcg(x + (size_t)(y + a.KV) * DH + lane * EPL + e) : 0.f;
+  }
+  const int depth = a.depth ? __ldg(a.depth + row) : t;
   int len, nodes;
   tree_extent(a, b, len, nodes);
   if (t >= nodes) {
@@ -49,15 +58,15 @@ __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
     if (cut && lane == 0) af_set_err(a.err, AF_DEV_BAD_POS);
     return;
   }
-  const int pos = len + (a.depth ? __ldg(a.depth + row) : t);
+  const int pos = len + depth;
   const bool rope = a.cos_t != nullptr;
   const bool lost = rope && (pos < 0 || pos >= a.rope_rows);       // no such position: the node's q and k are zeros
-  if (lost && lane == 0) af_set_err(a.err, AF_DEV_BAD_POS);
-  float rc[EPL], rs[EPL], v[EPL];
-  load_rope_row<DH>(a.cos_t, a.sin_t, rope && !lost ? pos : 0, lane, rc, rs);
-  const float* x = a.qkv + (size_t)row * a.ld_qkv;
+  if (lost) {
+    if (lane == 0) af_set_err(a.err, AF_DEV_BAD_POS);
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) v[e] = active && !lost ? __ldcg(x + (size_t)y * DH + lane * EPL + e) : 0.f;
+    for (int e = 0; e < EPL; ++e) v[e] = 0.f;
+  }
+  load_rope_row<DH>(a.cos_t, a.sin_t, rope && !lost ? pos : 0, lane, rc, rs);
   if (y < a.H) {
     norm_rope_head_pre<DH>(v, lane, a.qn_g, a.qn_floor, rope, rc, rs);
     const int G = a.H / a.KV;
@@ -81,7 +90,7 @@ __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
   if (active)
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
-      const __half kh = f2h(v[e]), vh = f2h(__ldcg(x + (size_t)(y + a.KV) * DH + lane * EPL + e));
+      const __half kh = f2h(v[e]), vh = f2h(vv[e]);
       a.kc[o + e] = kh;
       a.vc[o + e] = vh;
       finite &= isfinite(h2f(kh)) && isfinite(h2f(vh));

@@ -70,6 +70,7 @@ struct TreeShared {
   uint32_t vmask[8];                           // boxes of the tile that have a page
   uint32_t bad[tt::MAXW];                      // nodes whose k or v is not finite
   uint32_t tmem;
+  int holes;                                   // some row of the segments so far has no page
   int abort;
 };
 
@@ -119,6 +120,28 @@ AF_DEV void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
       : "memory");
 }
 
+#define TT_IN16(v) "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), \
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+AF_DEV void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "{\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;\n}\n"
+      : TT_R8(v, 0), TT_R8(v, 8)
+      : "r"(taddr)
+      : "memory");
+}
+AF_DEV void tmem_st16_async(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::TT_IN16(v),
+      "r"(taddr)
+      : "memory");
+}
+AF_DEV void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  tmem_st16_async(taddr, v);
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 AF_DEV void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -150,6 +173,121 @@ AF_DEV uint32_t see32(const int* mask, int words, int t, int u0) {
   return s ? __funnelshift_r(word(w), word(w + 1), s) : word(w);
 }
 AF_DEV uint32_t ones_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+
+// what a row's thread has at the end of a segment: its O (one or two accumulators with their weights), m, l
+struct TreeEnd {
+  uint32_t o0, o1;
+  bool have0, have1;
+  float f0, f1, m, l;
+  int c0, r, t, pr;
+  float* part;                                 // where a cut pair's partial result goes; null: the pair is whole
+};
+
+template <int DH, bool TWO> struct EndCols { static constexpr int n = TWO ? DH : DH / 2; };
+
+// 16 columns from c0 of the row's sum (a warp)
+AF_DEV void tree_take(const TreeEnd& e, int c0, float (&x)[16]) {
+  uint32_t o[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) x[k] = 0.f;
+  if (e.have0) {
+    tmem_ld16(e.o0 + c0, o);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = __uint_as_float(o[k]) * e.f0;
+  }
+  if (e.have1) {
+    tmem_ld16(e.o1 + c0, o);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = fmaf(__uint_as_float(o[k]), e.f1, x[k]);
+  }
+}
+
+template <int DH>
+AF_DEV void tree_put(const AttnTreeArgs& a, int b, int h, int nodes, const TreeEnd& e, int c0, const float (&x)[16]) {
+  const int G = a.H / a.KV;
+  if (e.r >= a.T * G) return;
+  if (e.part) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      __stcg(reinterpret_cast<float4*>(e.part) + (size_t)(c0 / 4 + q) * a.part_rows + e.pr,
+             make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
+    return;
+  }
+  const float il = e.t >= nodes || e.l == 0.f ? 0.f : 1.f / e.l;       // NaN stays
+  __half* dst = a.out + ((size_t)b * a.T + e.t) * a.ld_out + (size_t)(h * G + e.r - e.t * G) * DH + c0;
+  __half2 y[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y[k] = e.t >= nodes ? __half2() : __floats2half2_rn(x[2 * k] * il, x[2 * k + 1] * il);
+  if (a.out16) {
+    reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(y)[0];
+    reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(y)[1];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { dst[2 * k] = __low2half(y[k]); dst[2 * k + 1] = __high2half(y[k]); }
+  }
+}
+
+template <int DH, bool TWO>
+AF_DEV void tree_store(const AttnTreeArgs& a, int b, int h, int nodes, const TreeEnd& e) {
+  if (e.part && (TWO || e.c0 == 0) && e.r < a.T * (a.H / a.KV))
+    __stcg(reinterpret_cast<float2*>(e.part + (size_t)a.part_rows * DH) + e.pr, make_float2(e.m, e.l));
+#pragma unroll 1
+  for (int c0 = e.c0; c0 < e.c0 + EndCols<DH, TWO>::n; c0 += 16) {
+    float x[16];
+    tree_take(e, c0, x);
+    tree_put<DH>(a, b, h, nodes, e, c0, x);
+  }
+}
+
+// The same where nodes of the sequence are not finite: they were left out of the products, and are added to
+// the rows that see them here, key by key.
+template <int DH, bool TWO>
+__device__ __noinline__ void tree_bad_nodes(const AttnTreeArgs& a, int b, int h, int len, int nodes, const uint32_t* bad,
+                                            const int* mrow, TreeEnd e) {
+  const int R = a.T * (a.H / a.KV);
+  const bool in = e.r < R;
+  const float sl2 = a.scale * 1.4426950408889634f;
+  auto sees = [&](int u) {
+    return (bad[u >> 5] >> (u & 31) & 1) && (mrow ? (__ldg(mrow + (u >> 5)) >> (u & 31)) & 1 : u <= e.t);
+  };
+  auto row = [&](const __half* c, int u) -> const __half* {
+    const int j = len + u, p = __ldg(a.table + (size_t)b * a.W + j / a.page);
+    return p < 0 || p >= a.P ? nullptr : c + (size_t)p * a.page_stride + ((size_t)h * a.page + j % a.page) * DH;
+  };
+  auto score = [&](const __half* k) {
+    const __half* q = a.q + (((size_t)b * a.KV + h) * R + e.r) * DH;
+    float s = 0.f;
+    for (int d = 0; d < DH; ++d) s = fmaf(h2f(__ldcg(q + d)), h2f(__ldcg(k + d)), s);
+    return s * sl2;
+  };
+  float m2 = e.m;
+  for (int u = 0; in && u < nodes; ++u)
+    if (sees(u))
+      if (const __half* k = row(a.kc, u)) m2 = fmaxf(m2, score(k));
+  const float c = e.m == -INFINITY ? 0.f : tt_ex2(e.m - m2);
+  e.f0 *= c; e.f1 *= c; e.l *= c;
+  e.m = m2;
+  for (int u = 0; in && u < nodes; ++u)
+    if (sees(u))
+      if (const __half* k = row(a.kc, u)) e.l += tt_ex2(score(k) - (e.m - tt::SHIFT));
+  if (e.part && (TWO || e.c0 == 0) && in)
+    __stcg(reinterpret_cast<float2*>(e.part + (size_t)a.part_rows * DH) + e.pr, make_float2(e.m, e.l));
+#pragma unroll 1
+  for (int c0 = e.c0; c0 < e.c0 + EndCols<DH, TWO>::n; c0 += 16) {
+    float x[16];
+    tree_take(e, c0, x);
+    for (int u = 0; in && u < nodes; ++u)
+      if (sees(u))
+        if (const __half* k = row(a.kc, u)) {
+          const __half* v = row(a.vc, u) + c0;
+          const float p = tt_ex2(score(k) - (e.m - tt::SHIFT));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = fmaf(p, h2f(__ldcg(v + i)), x[i]);
+        }
+    __syncwarp();
+    tree_put<DH>(a, b, h, nodes, e, c0, x);
+  }
+}
 
 template <int DH, bool TWO>
 __global__ void __launch_bounds__(tt::THREADS, 1)
@@ -188,6 +326,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
     mbar_init(&sh->acc_free, 256);
     mbar_init(&sh->done, 1);
     sh->abort = 0;
+    sh->holes = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) {
@@ -247,9 +386,14 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         int p = -1;
         if (mine && row < sc.len + sc.nodes) {
           p = __ldg(a.table + (size_t)sc.b * a.W + row / a.page);
-          if (p < 0 || p >= a.P) { p = -1; af_set_err(a.err, AF_DEV_BAD_POS); }
+          if (p < 0 || p >= a.P) {
+            p = -1;
+            *(volatile int*)&sh->holes = 1;
+            af_set_err(a.err, AF_DEV_BAD_POS);
+          }
         }
         const unsigned live = __ballot_sync(0xffffffffu, p >= 0);
+        __syncwarp();
         if (lane == 0) {
           sh->vmask[st] = live & (nbox == 32 ? 0xffffffffu : (1u << nbox) - 1);
           mbar_arrive_expect_tx(&sh->full[st], (uint32_t)(__popc(live) * a.box_rows * 128));
@@ -347,6 +491,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
     // ------------------------------------------------------------- rows (two groups of four warps)
     const int w = warp >> 2, wr = (warp & 3) * 32 + lane;    // stream, row of the tile = TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t scol = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
     const float sl2 = a.scale * 1.4426950408889634f;
     bool ok = true;
     int seq0 = 0, nseg = 0;
@@ -358,68 +503,74 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       if (!ok) break;
       const int nt = sc.tiles();
       const int r = (TWO ? sc.rg * 256 + 128 * w : 0) + wr;  // row of the pair
-      const bool live_warp = r - lane < R;
-      const bool in = r < R;
+      const bool live_warp = r - lane < R, in = r < R;
       const int t = in ? r / G : 0;
-      const int n = sc.len + sc.nodes;
       const int* mrow = a.mask ? a.mask + ((size_t)sc.b * a.T + t) * a.mask_words : nullptr;
       // nodes that are not finite: only a segment that meets the nodes looks
       const bool tail = (sc.t0 + nt) * BK > sc.len;
-      if (tail && warp < MAXW) {
-        const int u = 32 * warp + lane;
-        const bool b = u < sc.nodes && __ldcg(a.flags + ((size_t)sc.b * a.KV + sc.h) * a.T + u);
-        const unsigned m = __ballot_sync(0xffffffffu, b);
-        if (lane == 0) sh->bad[warp] = m;
+      bool any_bad = false;
+      if (tail) {
+        if (warp < MAXW) {
+          const int u = 32 * warp + lane;
+          const bool b = u < sc.nodes && __ldcg(a.flags + ((size_t)sc.b * a.KV + sc.h) * a.T + u);
+          const unsigned m = __ballot_sync(0xffffffffu, b);
+          if (lane == 0) sh->bad[warp] = m;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < MAXW; ++k) any_bad |= sh->bad[k] != 0;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
       float m = -INFINITY, l = 0.f;
       bool first = true;
       for (int j = TWO ? 0 : w; j < nt; j += TWO ? 1 : 2) {
+        const int j0 = (sc.t0 + j) * BK;
+        const bool odd = j0 + BK > sc.len;                   // reaches past the prefix
+        uint32_t vis[4];                                     // visible keys, while the scores are on their way
+        if (odd) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) vis[c] = see32(mrow, a.mask_words, t, j0 + 32 * c - sc.len) & ones_below(sc.len + sc.nodes - j0 - 32 * c);
+        }
         if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
         ++ns;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int j0 = (sc.t0 + j) * BK;
-        const int seqv = seq0 + seq_v<TWO>(j, nt), stv = seqv % NS;
-        // a tile that reaches past the prefix, or into rows without a page
-        bool odd = j0 + BK > sc.len;
-        uint32_t boxes = 0xffffffffu;
-        if (a.paged || odd) {
+        if (odd || *(volatile int*)&sh->holes) {
+          // keys that are not there: out of the scores; rows of V that nobody may see become zeros (whatever
+          // lies there times a weight of 0 must be 0)
+          const int seqv = seq0 + seq_v<TWO>(j, nt), stv = seqv % NS;
           if (!tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
-          boxes = *(volatile uint32_t*)&sh->vmask[stv];
-          odd |= boxes != (BK / a.box_rows == 32 ? 0xffffffffu : (1u << (BK / a.box_rows)) - 1);
-        }
-        if (odd) {
-          // rows of V that nobody may see become zeros (whatever lies there times a weight of 0 must be 0)
-          unsigned char* vt = smem + C::RING + stv * TILE;
-          const int k = wr, key = j0 + k;
-          const int u = key - sc.len;
-          const bool gone = key >= n || !(boxes >> (k / a.box_rows) & 1) || (u >= 0 && (sh->bad[u >> 5] >> (u & 31) & 1));
-          if (gone)
+          const uint32_t boxes = *(volatile uint32_t*)&sh->vmask[stv];
+          const int u = j0 + wr - sc.len;
+          const bool isbad = any_bad && u >= 0 && u < TREE_MAX_NODES && (sh->bad[u >> 5] >> (u & 31) & 1);
+          if (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad) {
+            unsigned char* vt = smem + C::RING + stv * TILE;
+#pragma unroll 1
             for (int c = 0; c < DH / 8; ++c)
-              *reinterpret_cast<uint4*>(vt + (c >> 3) * SLICE + sw128(k, c & 7)) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(vt + (c >> 3) * SLICE + sw128(wr, c & 7)) = make_uint4(0, 0, 0, 0);
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (live_warp) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t x = !odd ? 0xffffffffu : c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+              for (int e = 0; e < 32; e += 8)                // a box has at least 8 rows
+                if (!(boxes >> ((32 * c + e) >> a.box_shift) & 1)) x &= ~(0xffu << e);
+              if (any_bad)                                   // not the nodes that are added at the end
+                for (int e = 0; e < 32; ++e) {
+                  const int n = j0 + 32 * c + e - sc.len;
+                  if (n >= 0 && n < TREE_MAX_NODES && (sh->bad[n >> 5] >> (n & 31) & 1)) x &= ~(1u << e);
+                }
+              if (__all_sync(0xffffffffu, x == 0xffffffffu)) continue;
+              uint32_t v[32];
+              tmem_ld32(scol + 32 * c, v);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = x >> e & 1 ? v[e] : 0xff800000u;
+              tmem_st32(scol + 32 * c, v);
+            }
+          }
         }
         if (live_warp) {
           uint32_t v[128];
-          tmem_ld128(lanes + S_COL + 128 * w, v);
-          if (odd) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int k0 = j0 + 32 * c, u0 = k0 - sc.len;
-              uint32_t vis = see32(mrow, a.mask_words, t, u0) & ones_below(n - k0);
-              if (u0 > -32) {                                // not the nodes that are added at the end
-                const int bw = u0 >> 5, bs = u0 & 31;
-                const uint32_t lo = bw >= 0 && bw < MAXW ? sh->bad[bw] : 0u, hi = bw + 1 >= 0 && bw + 1 < MAXW ? sh->bad[bw + 1] : 0u;
-                vis &= ~(bs ? __funnelshift_r(lo, hi, bs) : lo);
-              }
-              for (int e = 0; e < 32; e += a.box_rows)       // box_rows >= 8
-                if (!(boxes >> ((32 * c + e) / a.box_rows) & 1))
-                  vis &= ~((a.box_rows >= 32 ? 0xffffffffu : (1u << a.box_rows) - 1) << e);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(vis >> e & 1)) v[32 * c + e] = 0xff800000u;
-            }
-          }
+          tmem_ld128(scol, v);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int e = 0; e < 128; e += 4)
@@ -435,31 +586,32 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
             if (!first) {
               // s_full came after the products before it, so O is at rest
 #pragma unroll 1
-              for (int c0 = 0; c0 < DH; c0 += 32) {
-                uint32_t o[32];
-                tmem_ld32(lanes + O_COL + 128 * w + c0, o);
+              for (int c0 = 0; c0 < DH; c0 += 16) {
+                uint32_t o[16];
+                tmem_ld16(ocol + c0, o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                tmem_st32(lanes + O_COL + 128 * w + c0, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                tmem_st16(ocol + c0, o);
               }
             }
           }
           const float mb = m == -INFINITY ? 0.f : m - SHIFT;
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[32];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float p0 = tt_ex2(fmaf(__uint_as_float(v[64 * c + 2 * e]), sl2, -mb));
-              const float p1 = tt_ex2(fmaf(__uint_as_float(v[64 * c + 2 * e + 1]), sl2, -mb));
+            for (int e = 0; e < 16; ++e) {
+              const float p0 = tt_ex2(fmaf(__uint_as_float(v[32 * c + 2 * e]), sl2, -mb));
+              const float p1 = tt_ex2(fmaf(__uint_as_float(v[32 * c + 2 * e + 1]), sl2, -mb));
               ps[(e & 1) * 2] += p0;
               ps[(e & 1) * 2 + 1] += p1;
               const __half2 hp = __floats2half2_rn(p0, p1);
               pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
             }
-            tmem_st32(lanes + S_COL + 128 * w + 32 * c, pk);
+            tmem_st16_async(scol + 16 * c, pk);
           }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
         }
         first = false;
@@ -471,8 +623,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       ok = ok && tt_wait_warp(&sh->o_full[w], (uint32_t)(nseg & 1), abort);
       if (!TWO) ok = ok && tt_wait_warp(&sh->o_full[w ^ 1], (uint32_t)(nseg & 1), abort);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float f0 = 1.f, f1 = 0.f;                              // weights of O and of the other stream's O
-      bool have0 = !first, have1 = false;
+      float f0 = first ? 0.f : 1.f, f1 = 0.f;                // weights of O and of the other stream's O
       if (!TWO) {
         sh->ml[w][wr] = make_float2(m, l);
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -482,109 +633,21 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         f1 = o.x == -INFINITY ? 0.f : tt_ex2(o.x - M);
         l = l * f0 + o.y * f1;
         m = M;
-        have1 = nt > (w ? 0 : 1);
       }
-      // nodes that are not finite, for the segment that ends with the sequence
-      const bool ends = sc.ends();
-      bool any_bad = false;
-      if (tail && ends)
-        for (int k = 0; k < MAXW; ++k) any_bad |= sh->bad[k] != 0;
-      auto visible = [&](int u) { return mrow ? (__ldg(mrow + (u >> 5)) >> (u & 31)) & 1 : u <= t; };
-      auto node_row = [&](const __half* c, int u) {
-        const int row = sc.len + u, p = __ldg(a.table + (size_t)sc.b * a.W + row / a.page);
-        return p < 0 || p >= a.P ? nullptr : c + (size_t)p * a.page_stride + ((size_t)sc.h * a.page + row % a.page) * DH;
-      };
-      auto node_score = [&](const __half* kr) {
-        const __half* q = a.q + (((size_t)sc.b * a.KV + sc.h) * R + r) * DH;
-        float s = 0.f;
-        for (int d = 0; d < DH; ++d) s = fmaf(h2f(__ldcg(q + d)), h2f(__ldcg(kr + d)), s);
-        return s * sl2;
-      };
-      float m2 = m;
-      if (any_bad && in) {
-        for (int u = 0; u < sc.nodes; ++u)
-          if ((sh->bad[u >> 5] >> (u & 31) & 1) && visible(u)) {
-            const __half* kr = node_row(a.kc, u);
-            if (kr) m2 = fmaxf(m2, node_score(kr));
-          }
-        const float c = m == -INFINITY ? 0.f : tt_ex2(m - m2);
-        f0 *= c; f1 *= c; l *= c;
-        m = m2;
-        for (int u = 0; u < sc.nodes; ++u)
-          if ((sh->bad[u >> 5] >> (u & 31) & 1) && visible(u)) {
-            const __half* kr = node_row(a.kc, u);
-            if (kr) l += tt_ex2(node_score(kr) - (m - SHIFT));
-          }
+      TreeEnd e;
+      e.o0 = ocol;
+      e.o1 = lanes + O_COL + 128 * (w ^ 1);
+      e.have0 = !first;
+      e.have1 = !TWO && nt > (w ? 0 : 1);
+      e.f0 = f0; e.f1 = f1; e.m = m; e.l = l;
+      e.c0 = TWO ? 0 : w * (DH / 2);                         // split streams: each group writes half of the columns
+      e.r = r; e.t = t;
+      e.pr = (TWO ? 128 * w : 0) + wr;
+      e.part = sc.whole() ? nullptr : a.part + (size_t)(blockIdx.x * 2 + sc.slot()) * a.part_rows * (DH + 2);
+      if (ok && live_warp) {
+        if (any_bad && sc.ends()) tree_bad_nodes<DH, TWO>(a, sc.b, sc.h, sc.len, sc.nodes, sh->bad, mrow, e);
+        else tree_store<DH, TWO>(a, sc.b, sc.h, sc.nodes, e);
       }
-      const bool whole = sc.whole();
-      const float il = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);       // NaN stays
-      // split streams: each group writes half of the columns
-      constexpr int CW = TWO ? DH : DH / 2;
-      const int cb = TWO ? 0 : w * CW;
-      float* part = nullptr;
-      if (!whole) {
-        part = a.part + (size_t)(blockIdx.x * 2 + sc.slot()) * a.part_rows * (DH + 2);
-        if ((TWO || w == 0) && ok && in) {
-          const int pr = (TWO ? 128 * w : 0) + wr;
-          reinterpret_cast<float2*>(part + (size_t)a.part_rows * DH)[pr] = make_float2(m, l);
-        }
-      }
-      if (ok && live_warp)
-#pragma unroll 1
-        for (int c0 = cb; c0 < cb + CW; c0 += 32) {
-          float x[32];
-          uint32_t o[32];
-          if (have0) {
-            tmem_ld32(lanes + O_COL + 128 * w + c0, o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * f0;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = 0.f;
-          }
-          if (have1) {
-            tmem_ld32(lanes + O_COL + 128 * (w ^ 1) + c0, o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = fmaf(__uint_as_float(o[e]), f1, x[e]);
-          }
-          if (any_bad && in)
-            for (int u = 0; u < sc.nodes; ++u)
-              if ((sh->bad[u >> 5] >> (u & 31) & 1) && visible(u)) {
-                const __half* kr = node_row(a.kc, u);
-                const __half* vr = node_row(a.vc, u);
-                if (!kr) continue;
-                const float p = tt_ex2(node_score(kr) - (m - SHIFT));
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = fmaf(p, h2f(__ldcg(vr + c0 + e)), x[e]);
-              }
-          if (!in) continue;
-          if (whole) {
-            const int g = r - t * G;
-            __half* dst = a.out + ((size_t)sc.b * a.T + t) * a.ld_out + (size_t)(sc.h * G + g) * DH + c0;
-            const bool live = t < sc.nodes;
-            if (a.out16) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t o4[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const __half2 hv = live ? __floats2half2_rn(x[8 * q + 2 * i] * il, x[8 * q + 2 * i + 1] * il) : __half2();
-                  o4[i] = *reinterpret_cast<const uint32_t*>(&hv);
-                }
-                *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) dst[e] = live ? f2h(x[e] * il) : __half();
-            }
-          } else {
-            const int pr = (TWO ? 128 * w : 0) + wr;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              __stcg(reinterpret_cast<float4*>(part) + (size_t)(c0 / 4 + q) * a.part_rows + pr,
-                     make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
-          }
-        }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(&sh->acc_free);
     }
@@ -725,7 +788,7 @@ static cudaError_t tc_launch(const AttnTreeArgs& a, cudaStream_t st) {
 cudaError_t attn_tree_tc_launch(AttnTreeArgs a, cudaStream_t st) {
   const int R = a.T * (a.H / a.KV);
   a.box_rows = box_rows(a);
-  a.paged = a.W > 1;
+  a.box_shift = 31 - __builtin_clz((unsigned)a.box_rows);
   a.row_groups = (R + 255) / 256;
   a.out16 = a.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
   if (R <= 128) return a.dh == 128 ? tc_launch<128, false>(a, st) : tc_launch<64, false>(a, st);
