@@ -102,23 +102,18 @@ AF_DEV float tt_ex2(float x) {
 
 #define TT_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
 #define TT_R32(v, o) TT_R8(v, o), TT_R8(v, o + 8), TT_R8(v, o + 16), TT_R8(v, o + 24)
-// 128 columns of this warp's 32 lanes
-AF_DEV void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
+#define TT_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+// 32 columns of this warp's 32 lanes, on their way until tmem_ld_wait; the registers are touched after it only
+AF_DEV void tmem_ld32_async(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
-      "{\n"
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n"
-      "tcgen05.wait::ld.sync.aligned;\n}\n"
-      : TT_R32(v, 0), TT_R32(v, 32), TT_R32(v, 64), TT_R32(v, 96)
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : TT_R32(v, 0)
       : "r"(taddr)
       : "memory");
 }
+AF_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+AF_DEV void after_wait(uint32_t (&v)[32]) { asm volatile("" : TT_RW8(v, 0), TT_RW8(v, 8), TT_RW8(v, 16), TT_RW8(v, 24)); }
 
 #define TT_IN16(v) "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), \
                    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
@@ -160,17 +155,25 @@ AF_DEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, 
 template <bool TWO> AF_DEV int seq_k(int j) { return TWO ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
 template <bool TWO> AF_DEV int seq_v(int j, int nt) { return TWO ? 2 * j + 1 : (j == nt - 1 ? 2 * nt - 1 : 2 * j + 2); }
 
-// visibility of 32 nodes from node number u0 (may be negative: prefix rows) for a node's mask row
-AF_DEV uint32_t see32(const int* mask, int words, int t, int u0) {
-  if (u0 <= -32) return 0xffffffffu;
-  auto word = [&](int w) -> uint32_t {
-    if (w < 0) return 0xffffffffu;
-    if (mask) return w < words ? (uint32_t)__ldg(mask + w) : 0u;
-    const int k = t - 32 * w;                  // chain: nodes 0..t
-    return k < 0 ? 0u : k >= 31 ? 0xffffffffu : (2u << k) - 1;
-  };
-  const int w = u0 >> 5, s = u0 & 31;          // floor division: u0 = 32 w + s
-  return s ? __funnelshift_r(word(w), word(w + 1), s) : word(w);
+// visibility of the 128 nodes from node number u0 (may be negative: prefix rows) for a node's mask row; the
+// five words that this can reach are loaded together
+AF_DEV void see128(const int* mask, int words, int t, int u0, uint32_t (&vis)[4]) {
+  const int w0 = u0 >> 5, s = u0 & 31;         // floor division: u0 = 32 w0 + s
+  uint32_t x[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const int w = w0 + k;
+    x[k] = 0;
+    if (mask && w >= 0 && w < words) x[k] = (uint32_t)__ldg(mask + w);
+  }
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const int w = w0 + k, n = t - 32 * w;      // chain: nodes 0..t
+    if (w < 0) x[k] = 0xffffffffu;
+    else if (!mask) x[k] = n < 0 ? 0u : n >= 31 ? 0xffffffffu : (2u << n) - 1;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) vis[k] = __funnelshift_r(x[k], x[k + 1], s);
 }
 AF_DEV uint32_t ones_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
@@ -308,8 +311,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
   const int G = a.H / a.KV, R = a.T * G;
   pdl_trigger();
   TreeSched sc;
-  sc.init(a, blockIdx.x, gridDim.x, lane);
-  if (sc.u >= sc.u1) return;                   // fewer tiles than blocks
+  if (!sc.init(a, blockIdx.x, gridDim.x, lane)) return;      // fewer tiles than blocks
 
   if (threadIdx.x == 0) {
     mbar_init(&sh->q_full, 1);
@@ -527,8 +529,9 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         const bool odd = j0 + BK > sc.len;                   // reaches past the prefix
         uint32_t vis[4];                                     // visible keys, while the scores are on their way
         if (odd) {
+          see128(mrow, a.mask_words, t, j0 - sc.len, vis);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) vis[c] = see32(mrow, a.mask_words, t, j0 + 32 * c - sc.len) & ones_below(sc.len + sc.nodes - j0 - 32 * c);
+          for (int c = 0; c < 4; ++c) vis[c] &= ones_below(sc.len + sc.nodes - j0 - 32 * c);
         }
         if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
         ++ns;
@@ -569,13 +572,17 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
         }
         if (live_warp) {
-          uint32_t v[128];
-          tmem_ld128(scol, v);
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32_async(scol + 32 * c, v[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) after_wait(v[c]);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 128; e += 4)
+          for (int e = 0; e < 32; ++e)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(v[e + k]));
+            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(v[k][e]));
           const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
           const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY;
           if (__any_sync(0xffffffffu, rise)) {
@@ -602,8 +609,8 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float p0 = tt_ex2(fmaf(__uint_as_float(v[32 * c + 2 * e]), sl2, -mb));
-              const float p1 = tt_ex2(fmaf(__uint_as_float(v[32 * c + 2 * e + 1]), sl2, -mb));
+              const float p0 = tt_ex2(fmaf(__uint_as_float(v[c][2 * e]), sl2, -mb));
+              const float p1 = tt_ex2(fmaf(__uint_as_float(v[c][2 * e + 1]), sl2, -mb));
               ps[(e & 1) * 2] += p0;
               ps[(e & 1) * 2 + 1] += p1;
               const __half2 hp = __floats2half2_rn(p0, p1);
@@ -672,43 +679,56 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
   }
 }
 
-// joins the parts of the pairs that were cut: grid (row blocks, KV, B), a thread per 4 output elements
+// joins the parts of the pairs that were cut: grid (row blocks, KV, B), a thread per 4 output elements. The
+// parts are found by a thread each, their m and l brought to shared memory together, so that a part costs
+// one load of O.
 template <int DH>
 __global__ void __launch_bounds__(256) tree_combine_kernel(AttnTreeArgs a, int blocks) {
-  constexpr int C4 = DH / 4, ROWS = 256 / C4;
-  const int lane = threadIdx.x & 31;
-  const int G = a.H / a.KV, R = a.T * G;
-  const int r = blockIdx.x * ROWS + threadIdx.x % ROWS, c4 = threadIdx.x / ROWS;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int rg = a.row_groups > 1 ? r / 256 : 0;
+  constexpr int C4 = DH / 4, ROWS = 256 / C4, MAXP = 160;
+  __shared__ int part_s[MAXP];
+  __shared__ float2 ml_s[MAXP][ROWS];
+  const int tid = threadIdx.x, G = a.H / a.KV, R = a.T * G;
+  const int row0 = blockIdx.x * ROWS, h = blockIdx.y, b = blockIdx.z;
+  const int rg = row0 / 256;                   // ROWS divides 256: one group a block
   TreeSched sc;
   long long first, total;
-  sc.find(a, b, lane, first, total);
-  const int rg0 = a.row_groups > 1 ? blockIdx.x * ROWS / 256 : 0;    // ROWS divides 256: one group a block
-  const long long u0 = first + (long long)(h * a.row_groups + rg0) * sc.nt, u1 = u0 + sc.nt;
+  sc.find(a, b, tid & 31, first, total);
+  blocks = (int)min((long long)blocks, total);
+  const long long u0 = first + (long long)(h * a.row_groups + rg) * sc.nt, u1 = u0 + sc.nt;
   const int c0 = tree_block_of(u0, total, blocks), c1 = tree_block_of(u1 - 1, total, blocks);
+  if (c0 == c1) return;                        // the pair is whole
+  const int lr = tid % ROWS, c4 = tid / ROWS, r = row0 + lr, pr = r - rg * 256;
+  const int n = c1 - c0 + 1;
+  for (int k = tid; k < n; k += 256) part_s[k] = (c0 + k) * 2 + (tree_unit(c0 + k, total, blocks) > u0 ? 0 : 1);
   pdl_wait();
-  if (c0 == c1 || r >= R) return;
-  const int pr = r - rg * 256, t = r / G, g = r - t * G;
-  float M = -INFINITY;
-  for (int c = c0; c <= c1; ++c) {
-    const int slot = tree_unit(c, total, blocks) > u0 ? 0 : 1;
-    const float* part = a.part + (size_t)(c * 2 + slot) * a.part_rows * (DH + 2);
-    M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part + (size_t)a.part_rows * DH) + pr).x);
+  __syncthreads();
+  const size_t psize = (size_t)a.part_rows * (DH + 2);
+  for (int k = tid; k < n * ROWS; k += 256) {
+    const int q = k % ROWS;
+    ml_s[k / ROWS][q] = row0 + q < R
+        ? __ldcg(reinterpret_cast<const float2*>(a.part + part_s[k / ROWS] * psize + (size_t)a.part_rows * DH) + row0 - rg * 256 + q)
+        : make_float2(-INFINITY, 0.f);
   }
+  __syncthreads();
+  if (r >= R) return;
+  float M = -INFINITY;
+  for (int k = 0; k < n; ++k) M = fmaxf(M, ml_s[k][lr].x);
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0; c <= c1; ++c) {
-    const int slot = tree_unit(c, total, blocks) > u0 ? 0 : 1;
-    const float* part = a.part + (size_t)(c * 2 + slot) * a.part_rows * (DH + 2);
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + (size_t)a.part_rows * DH) + pr);
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float f = tt_ex2(ml.x - M);
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(part) + (size_t)c4 * a.part_rows + pr);
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) {
+    const float2 ml = ml_s[k][lr];
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part + part_s[k] * psize) + (size_t)c4 * a.part_rows + pr);
+    const bool any = ml.x != -INFINITY || ml.y != 0.f;       // a part in which the row saw nothing
+    const float f = any ? tt_ex2(ml.x - M) : 0.f;
     l = fmaf(ml.y, f, l);
-    o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+    o.x = any ? fmaf(x.x, f, o.x) : o.x;
+    o.y = any ? fmaf(x.y, f, o.y) : o.y;
+    o.z = any ? fmaf(x.z, f, o.z) : o.z;
+    o.w = any ? fmaf(x.w, f, o.w) : o.w;
   }
-  float il = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int t = r / G, g = r - t * G;
+  float il = l == 0.f ? 0.f : 1.f / l;         // NaN stays
   if (t >= sc.nodes) { il = 0.f; o = make_float4(0.f, 0.f, 0.f, 0.f); }
   __half2 x[2] = {__floats2half2_rn(o.x * il, o.y * il), __floats2half2_rn(o.z * il, o.w * il)};
   __half* dst = a.out + ((size_t)b * a.T + t) * a.ld_out + (size_t)(h * G + g) * DH + 4 * c4;
@@ -743,7 +763,8 @@ static bool q_map(CUtensorMap* map, const AttnTreeArgs& a, int rows) {
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int attn_tree_tc_blocks() { return device_attr(cudaDevAttrMultiProcessorCount, 148); }
+// one block an SM (the parts of a pair are listed in shared memory when they are joined: at most 160)
+int attn_tree_tc_blocks() { const int n = device_attr(cudaDevAttrMultiProcessorCount, 148); return n < 160 ? n : 160; }
 
 // rows of a page that one box can cover: a box never crosses a page (unless the sequence is one page,
 // where it ends at the map's bound), and starts at a multiple of 8 rows, the swizzle's period

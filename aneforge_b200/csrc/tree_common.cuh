@@ -13,7 +13,7 @@ AF_DEV void tree_extent(const AttnTreeArgs& a, int b, int& len, int& nodes) {
   nodes = min(nodes, a.W * a.page - len);
 }
 
-// block c of `blocks` takes the units from tree_unit(c) to tree_unit(c + 1) of `total`
+// block c of `blocks` (no more than there are units) takes the units from tree_unit(c) to tree_unit(c + 1) of `total`
 AF_DEV long long tree_unit(long long c, long long total, int blocks) { return c * total / blocks; }
 // the block that takes unit u
 AF_DEV int tree_block_of(long long u, long long total, int blocks) {
@@ -53,7 +53,8 @@ struct TreeSched {
       total += __reduce_add_sync(0xffffffffu, mine);
     }
     total *= per;
-    const long long at = want < 0 ? tree_unit(c, total, blocks) : 0;
+    const int act = (int)min((long long)blocks, total);
+    const long long at = want < 0 ? tree_unit(c < act ? c : 0, total, act) : 0;
     long long before = 0;
     b = 0;
     first = 0;
@@ -76,9 +77,12 @@ struct TreeSched {
       before += __shfl_sync(0xffffffffu, x, 31);
     }
   }
-  AF_DEV void init(const AttnTreeArgs& a, int c, int blocks, int lane) {
+  // false: nothing for this block
+  AF_DEV bool init(const AttnTreeArgs& a, int c, int blocks, int lane) {
     long long first, total;
     scan(a, -1, c, blocks, lane, first, total);
+    blocks = (int)min((long long)blocks, total);
+    if (c >= blocks) return false;
     u = tree_unit(c, total, blocks);
     u1 = tree_unit(c + 1, total, blocks);
     load(a);
@@ -87,6 +91,7 @@ struct TreeSched {
     rg = pair - h * a.row_groups;
     item0 = first + (long long)pair * nt;
     t0 = (int)(u - item0);
+    return true;
   }
   AF_DEV void find(const AttnTreeArgs& a, int want, int lane, long long& first, long long& total) {
     scan(a, want, 0, 1, lane, first, total);
