@@ -335,7 +335,7 @@ struct AttnTreeArgs {
   __half* q = nullptr;                 // [B][KV][T * G][dh]
   unsigned char* flags = nullptr;      // [B][KV][T] 1: the node's k or v is not finite
   float* part = nullptr;               // [blocks][2][part_rows * (dh + 2)] partial O, (m, l)
-  int part_rows = 0, box_rows = 0, box_shift = 0, row_groups = 1, out16 = 0;
+  int part_rows = 0, box_rows = 0, box_shift = 0, page_shift = -1, row_groups = 1, out16 = 0;
 };
 size_t attn_tree_scratch_bytes(int B, int T, int H, int KV, int dh);
 // the tensor-core form (attn_tree_tc.cu), after tree_append

@@ -26,8 +26,8 @@
 // in V; nodes whose k or v is not finite are taken out of the products too and added by the row's thread
 // at the end, for the rows that see them only.
 //
-// Roles (320 threads): warps 0-3 and 4-7 the streams' rows, warp 8 tensor memory and the products
-// (one thread), warp 9 the copies. Every wait is bounded; a block that gives up records
+// Roles (352 threads): warps 0-3 and 4-7 the streams' rows, warp 8 tensor memory and the products
+// (one thread), warps 9 and 10 the copies of K (and Q) and of V. Every wait is bounded; a block that gives up records
 // AF_DEV_WAIT_TIMEOUT, waits for its copies and products in flight, frees its tensor memory and returns.
 #include <cuda.h>
 
@@ -40,12 +40,13 @@ namespace af {
 
 namespace tt {
 constexpr int BK = 128;                        // keys per tile
-constexpr int THREADS = 320;
+constexpr int THREADS = 352;
 constexpr int MMA_WARP = 8, TMA_WARP = 9;
 constexpr int SLICE = 128 * 64 * 2;            // 128 rows x 64 fp16, 128-byte swizzled
 constexpr long long LIMIT = 1ll << 26;
 constexpr float SHIFT = 6.f, RISE = 8.f;       // log2 of the weights' factor; rise of the maximum that is let pass
 constexpr int MAXW = TREE_MAX_NODES / 32;
+constexpr int AHEAD = 8;                       // segments that the copies can be ahead: under NS
 template <int DH, bool TWO> struct Cfg {
   static constexpr int TILE = SLICE * (DH / 64);
   static constexpr int QT = TWO ? 2 : 1;       // row tiles
@@ -68,7 +69,7 @@ struct TreeShared {
   uint64_t done;
   float2 ml[2][128];                           // split streams: (m, l) of the other half
   uint32_t vmask[8];                           // boxes of the tile that have a page
-  uint32_t bad[tt::MAXW];                      // nodes whose k or v is not finite
+  uint32_t bad[tt::AHEAD][tt::MAXW];           // nodes whose k or v is not finite, of a segment (modulo AHEAD)
   uint32_t tmem;
   int holes;                                   // some row of the segments so far has no page
   int abort;
@@ -84,6 +85,14 @@ AF_DEV bool tt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
 }
 AF_DEV bool tt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, tt_wait(bar, parity, abort));
+}
+
+// whether the phase is over, without waiting; one answer for the warp
+AF_DEV bool tt_done_warp(uint64_t* bar, uint32_t parity) {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(r) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, r != 0);
 }
 
 // barrier of the 256 row threads; true if `ok` holds in all of them
@@ -144,10 +153,11 @@ AF_DEV void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, u
       ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-AF_DEV void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+// a box of a page: rows from `row`, 64 columns from 64 * half (or all 128 columns, as two slices)
+AF_DEV void tma_load_5d(void* dst, const CUtensorMap* map, int row, int half, int h, int page, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(0), "r"(row), "r"(half), "r"(h), "r"(page), "r"(smem_u32(bar)) : "memory");
 }
 
 // where a tile's K and V stand in the order in which they are loaded and used: two row tiles K0 V0 K1 V1
@@ -230,8 +240,9 @@ AF_DEV void tree_put(const AttnTreeArgs& a, int b, int h, int nodes, const TreeE
   }
 }
 
+// (not inlined, as the next one: once a segment, and its registers would be the tile loop's spills)
 template <int DH, bool TWO>
-AF_DEV void tree_store(const AttnTreeArgs& a, int b, int h, int nodes, const TreeEnd& e) {
+__device__ __noinline__ void tree_store(const AttnTreeArgs& a, int b, int h, int nodes, TreeEnd e) {
   if (e.part && (TWO || e.c0 == 0) && e.r < a.T * (a.H / a.KV))
     __stcg(reinterpret_cast<float2*>(e.part + (size_t)a.part_rows * DH) + e.pr, make_float2(e.m, e.l));
 #pragma unroll 1
@@ -294,7 +305,7 @@ __device__ __noinline__ void tree_bad_nodes(const AttnTreeArgs& a, int b, int h,
 
 template <int DH, bool TWO>
 __global__ void __launch_bounds__(tt::THREADS, 1)
-    attn_tree_tc_kernel(AttnTreeArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+    attn_tree_tc_kernel(const __grid_constant__ AttnTreeArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap) {
   using namespace tt;
   using C = Cfg<DH, TWO>;
@@ -322,10 +333,10 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh->s_full[w], 1);
-      mbar_init(&sh->p_full[w], 128);
+      mbar_init(&sh->p_full[w], 4);
       mbar_init(&sh->o_full[w], 1);
     }
-    mbar_init(&sh->acc_free, 256);
+    mbar_init(&sh->acc_free, 8);
     mbar_init(&sh->done, 1);
     sh->abort = 0;
     sh->holes = 0;
@@ -342,13 +353,13 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
   const uint32_t tmem = sh->tmem;
   volatile int* abort = &sh->abort;
 
-  if (warp == TMA_WARP) {
-    // ------------------------------------------------------------- copies (a lane per box)
-    const int nbox = BK / a.box_rows;                        // boxes of a tile, for each 64 columns
-    const int half = lane / nbox, box = lane - half * nbox;
-    const bool mine = half < DH / 64;
+  if (warp >= TMA_WARP) {
+    // ------------------------------------------------------------- copies: a warp for K (and Q), one for V
+    const bool is_v = warp == TMA_WARP + 1;
+    const int nbox = BK >> a.box_shift, per = 32 / nbox;     // boxes of a tile (at most 16), tiles of a page read
     bool waited = false, ok = true;
-    int seq0 = 0, nseg = 0, issued = 0, nq = 0;              // issued: ring slots, nq: Q tiles
+    int seq0 = 0, nseg = 0, nq = 0;
+    uint32_t armed = 0, phase = 0;                           // slots that were filled here, and their last phase
     auto dependency = [&] {                                  // q and the nodes' rows come from tree_append
       if (waited) return;
       pdl_wait();
@@ -357,7 +368,20 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
     };
     for (; ok && sc.u < sc.u1; sc.next(a), ++nseg) {
       const int nt = sc.tiles();
-      bool have_q = false;
+      bool have_q = is_v;
+      if (!is_v) {
+        // only a segment that meets the nodes has any that are not finite
+        const bool tail = (sc.t0 + nt) * BK > sc.len && sc.nodes > 0;
+        if (tail) dependency();
+        for (int k = 0; k < MAXW; ++k) {
+          unsigned m = 0;
+          if (tail && 32 * k < sc.nodes) {
+            const int u = 32 * k + lane;
+            m = __ballot_sync(0xffffffffu, u < sc.nodes && __ldcg(a.flags + ((size_t)sc.b * a.KV + sc.h) * a.T + u));
+          }
+          if (lane == 0) *(volatile uint32_t*)&sh->bad[nseg % AHEAD][k] = m;
+        }
+      }
       auto load_q = [&]() -> bool {
         dependency();
         if (nseg && !tt_wait_warp(&sh->q_empty, (uint32_t)((nseg - 1) & 1), abort)) return false;
@@ -371,51 +395,62 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         ++nq;
         return true;
       };
-      // the loads in the order of their use
-      for (int i = 0; ok && i < 2 * nt; ++i) {
-        int j;
-        bool is_v;
-        if (TWO) { j = i >> 1; is_v = i & 1; }
-        else if (i == 0) { j = 0; is_v = false; }
-        else if (i == 2 * nt - 1) { j = nt - 1; is_v = true; }
-        else { is_v = !(i & 1); j = is_v ? (i - 2) >> 1 : (i + 1) >> 1; }
-        const int seq = seq0 + i, st = seq % NS;
-        const int row = (sc.t0 + j) * BK + box * a.box_rows;
-        if (!have_q && (waited || seq >= NS || (sc.t0 + j + 1) * BK > sc.len)) {
-          if (!load_q()) { ok = false; break; }
-        }
-        if (seq >= NS && !tt_wait_warp(&sh->empty[st], (uint32_t)((seq / NS - 1) & 1), abort)) { ok = false; break; }
-        int p = -1;
-        if (mine && row < sc.len + sc.nodes) {
-          p = __ldg(a.table + (size_t)sc.b * a.W + row / a.page);
-          if (p < 0 || p >= a.P) {
-            p = -1;
+      // the pages of `per` tiles at a time, a lane each; -2: no row in the box
+      auto pages_of = [&](int j) {
+        const int row = (sc.t0 + j) * BK + lane * a.box_rows;
+        const int w = a.page_shift >= 0 ? row >> a.page_shift : row / a.page;
+        return j < nt && row < sc.len + sc.nodes ? __ldg(a.table + (size_t)sc.b * a.W + w) : -2;
+      };
+      int pages = -2, pages1 = pages_of(0);
+      for (int j = 0; j < nt; ++j) {
+        const int i = is_v ? seq_v<TWO>(j, nt) : seq_k<TWO>(j), seq = seq0 + i, st = seq % NS;
+        const int g = j % per;
+        if (g == 0) {
+          pages = pages1;
+          pages1 = pages_of(j + per);
+          if (pages != -2 && (pages < 0 || pages >= a.P)) {
+            pages = -1;
             *(volatile int*)&sh->holes = 1;
             af_set_err(a.err, AF_DEV_BAD_POS);
           }
         }
-        const unsigned live = __ballot_sync(0xffffffffu, p >= 0);
-        __syncwarp();
-        if (lane == 0) {
-          sh->vmask[st] = live & (nbox == 32 ? 0xffffffffu : (1u << nbox) - 1);
-          mbar_arrive_expect_tx(&sh->full[st], (uint32_t)(__popc(live) * a.box_rows * 128));
+        const unsigned live = (__ballot_sync(0xffffffffu, pages >= 0) >> (g * nbox)) & ((1u << nbox) - 1);
+        if ((sc.t0 + j + 1) * BK > sc.len) dependency();     // the nodes' rows
+        // Q at the latest when the ring is full of this segment; before, once the last one's scores are done
+        if (!have_q && (i >= NS || (waited && (!nseg || tt_done_warp(&sh->q_empty, (uint32_t)((nseg - 1) & 1))))) && !load_q()) {
+          ok = false;
+          break;
         }
-        __syncwarp();
-        if (p >= 0)
-          tma_load_4d(smem + C::RING + st * TILE + half * SLICE + box * a.box_rows * 128, is_v ? &vmap : &kmap, 64 * half,
-                      row % a.page, sc.h, p, &sh->full[st]);
-        issued = seq + 1;
+        if (seq >= NS && !tt_wait_warp(&sh->empty[st], (uint32_t)((seq / NS - 1) & 1), abort)) { ok = false; break; }
+        if (lane == 0) {
+          sh->vmask[st] = live;
+          mbar_arrive_expect_tx(&sh->full[st], (uint32_t)(__popc(live) * a.box_rows * (DH * 2)));
+        }
+        // one lane issues all copies: their operands are the warp's, several lanes would take turns
+        const int row = (sc.t0 + j) * BK;
+        unsigned char* slot = smem + C::RING + st * TILE;
+        const CUtensorMap* map = is_v ? &vmap : &kmap;
+        for (int k = 0; k < nbox; ++k) {
+          const int pk = __shfl_sync(0xffffffffu, pages, g * nbox + k);
+          if (pk >= 0 && lane == 0) {
+            const int y = row + k * a.box_rows, in = a.page_shift >= 0 ? y & (a.page - 1) : y % a.page;
+            tma_load_5d(slot + k * a.box_rows * 128, map, in, 0, sc.h, pk, &sh->full[st]);
+            if (DH == 128 && nbox > 1) tma_load_5d(slot + SLICE + k * a.box_rows * 128, map, in, 1, sc.h, pk, &sh->full[st]);
+          }
+        }
+        armed |= 1u << st;
+        phase = (phase & ~(1u << st)) | (uint32_t)((seq / NS) & 1) << st;
       }
       if (ok && !have_q) ok = load_q();
-      if (ok) seq0 += 2 * nt;
+      seq0 += 2 * nt;
     }
     if (!ok) *abort = 1;
     dependency();
     // shared memory must outlive every copy issued: a block that gave up waits (bounded) for the last ones
     if (!ok) {
-      for (int s = max(0, issued - NS); s < issued; ++s) {
+      for (int st = 0; st < NS; ++st) {
         SpinBudget b;
-        while (!mbar_try_wait(&sh->full[s % NS], (uint32_t)((s / NS) & 1)) && !b.spent()) {
+        while ((armed >> st & 1) && !mbar_try_wait(&sh->full[st], phase >> st & 1) && !b.spent()) {
         }
       }
       SpinBudget b;
@@ -493,12 +528,12 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
     // ------------------------------------------------------------- rows (two groups of four warps)
     const int w = warp >> 2, wr = (warp & 3) * 32 + lane;    // stream, row of the tile = TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t scol = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
+    const uint32_t scol0 = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
     const float sl2 = a.scale * 1.4426950408889634f;
     bool ok = true;
     int seq0 = 0, nseg = 0;
     uint32_t ns = 0;                                         // tiles of this stream so far
-    pdl_wait();                                              // the flags of nodes that are not finite
+    pdl_wait();                                              // q, for the nodes that are added at the end
     for (; sc.u < sc.u1; sc.next(a), ++nseg) {
       // all rows go on, or none (barriers lie ahead); `bad` is free from here
       ok = rows_all(ok);
@@ -508,43 +543,39 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       const bool live_warp = r - lane < R, in = r < R;
       const int t = in ? r / G : 0;
       const int* mrow = a.mask ? a.mask + ((size_t)sc.b * a.T + t) * a.mask_words : nullptr;
-      // nodes that are not finite: only a segment that meets the nodes looks
-      const bool tail = (sc.t0 + nt) * BK > sc.len;
-      bool any_bad = false;
-      if (tail) {
-        if (warp < MAXW) {
-          const int u = 32 * warp + lane;
-          const bool b = u < sc.nodes && __ldcg(a.flags + ((size_t)sc.b * a.KV + sc.h) * a.T + u);
-          const unsigned m = __ballot_sync(0xffffffffu, b);
-          if (lane == 0) sh->bad[warp] = m;
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-#pragma unroll
-        for (int k = 0; k < MAXW; ++k) any_bad |= sh->bad[k] != 0;
-      }
+      const uint32_t* bad = sh->bad[nseg % AHEAD];           // written before the segment's first copy
       float m = -INFINITY, l = 0.f;
       bool first = true;
-      for (int j = TWO ? 0 : w; j < nt; j += TWO ? 1 : 2) {
+      // The block's first tile is preceded by a dry one, while Q is on its way: the same instructions on columns of
+      // O that nothing uses yet, so that they are fetched (from an L2 full of K and V) before they are waited for.
+      for (int j = (TWO ? 0 : w) - (nseg ? 0 : TWO ? 1 : 2); j < nt; j += TWO ? 1 : 2) {
+        const bool dry = j < 0;
+        const uint32_t scol = dry ? ocol : scol0;
         const int j0 = (sc.t0 + j) * BK;
-        const bool odd = j0 + BK > sc.len;                   // reaches past the prefix
+        const bool odd = j0 + BK > sc.len || dry;            // reaches past the prefix
         uint32_t vis[4];                                     // visible keys, while the scores are on their way
         if (odd) {
           see128(mrow, a.mask_words, t, j0 - sc.len, vis);
 #pragma unroll
           for (int c = 0; c < 4; ++c) vis[c] &= ones_below(sc.len + sc.nodes - j0 - 32 * c);
         }
-        if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
-        ++ns;
+        if (!dry) {
+          if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
+          ++ns;
+        }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        bool any_bad = false;
         if (odd || *(volatile int*)&sh->holes) {
+#pragma unroll
+          for (int k = 0; k < MAXW; ++k) any_bad |= bad[k] != 0;
           // keys that are not there: out of the scores; rows of V that nobody may see become zeros (whatever
           // lies there times a weight of 0 must be 0)
-          const int seqv = seq0 + seq_v<TWO>(j, nt), stv = seqv % NS;
-          if (!tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
+          const int seqv = seq0 + (dry ? 0 : seq_v<TWO>(j, nt)), stv = seqv % NS;
+          if (!dry && !tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
           const uint32_t boxes = *(volatile uint32_t*)&sh->vmask[stv];
           const int u = j0 + wr - sc.len;
-          const bool isbad = any_bad && u >= 0 && u < TREE_MAX_NODES && (sh->bad[u >> 5] >> (u & 31) & 1);
-          if (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad) {
+          const bool isbad = any_bad && u >= 0 && u < TREE_MAX_NODES && (bad[u >> 5] >> (u & 31) & 1);
+          if (!dry && (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad)) {
             unsigned char* vt = smem + C::RING + stv * TILE;
 #pragma unroll 1
             for (int c = 0; c < DH / 8; ++c)
@@ -560,7 +591,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
               if (any_bad)                                   // not the nodes that are added at the end
                 for (int e = 0; e < 32; ++e) {
                   const int n = j0 + 32 * c + e - sc.len;
-                  if (n >= 0 && n < TREE_MAX_NODES && (sh->bad[n >> 5] >> (n & 31) & 1)) x &= ~(1u << e);
+                  if (n >= 0 && n < TREE_MAX_NODES && (bad[n >> 5] >> (n & 31) & 1)) x &= ~(1u << e);
                 }
               if (__all_sync(0xffffffffu, x == 0xffffffffu)) continue;
               uint32_t v[32];
@@ -572,25 +603,28 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
         }
         if (live_warp) {
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32_async(scol + 32 * c, v[c]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) after_wait(v[c]);
+          // the scores are read twice, 32 columns at a time with the next ones on their way: holding all 128
+          // costs spills whose first touches stalled whole tiles
+          uint32_t v[2][32];
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_ld32_async(scol, v[0]);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            after_wait(v[c & 1]);
+            if (c < 3) tmem_ld32_async(scol + 32 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(v[k][e]));
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[c & 1][e]));
+          }
+          tmem_ld32_async(scol, v[0]);
           const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-          const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY;
+          const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY || dry;
           if (__any_sync(0xffffffffu, rise)) {
             const float mn = fmaxf(m, tm);
             const float corr = m == -INFINITY ? 0.f : tt_ex2(m - mn);
             m = mn;
             l *= corr;
-            if (!first) {
+            if (!first || dry) {
               // s_full came after the products before it, so O is at rest
 #pragma unroll 1
               for (int c0 = 0; c0 < DH; c0 += 16) {
@@ -605,12 +639,15 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           const float mb = m == -INFINITY ? 0.f : m - SHIFT;
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 4; ++c) {                      // P's columns 16 c.. lie in scores that were read
+            tmem_ld_wait();
+            after_wait(v[c & 1]);
+            if (c < 3) tmem_ld32_async(scol + 32 * (c + 1), v[(c + 1) & 1]);
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float p0 = tt_ex2(fmaf(__uint_as_float(v[c][2 * e]), sl2, -mb));
-              const float p1 = tt_ex2(fmaf(__uint_as_float(v[c][2 * e + 1]), sl2, -mb));
+              const float p0 = tt_ex2(fmaf(__uint_as_float(v[c & 1][2 * e]), sl2, -mb));
+              const float p1 = tt_ex2(fmaf(__uint_as_float(v[c & 1][2 * e + 1]), sl2, -mb));
               ps[(e & 1) * 2] += p0;
               ps[(e & 1) * 2 + 1] += p1;
               const __half2 hp = __floats2half2_rn(p0, p1);
@@ -621,9 +658,15 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
         }
+        if (dry) {
+          m = -INFINITY;
+          l = 0.f;
+          continue;
+        }
         first = false;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        mbar_arrive(&sh->p_full[w]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full[w]);
       }
       seq0 += 2 * nt;
       // ---- the segment's end
@@ -652,11 +695,16 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       e.pr = (TWO ? 128 * w : 0) + wr;
       e.part = sc.whole() ? nullptr : a.part + (size_t)(blockIdx.x * 2 + sc.slot()) * a.part_rows * (DH + 2);
       if (ok && live_warp) {
-        if (any_bad && sc.ends()) tree_bad_nodes<DH, TWO>(a, sc.b, sc.h, sc.len, sc.nodes, sh->bad, mrow, e);
+        bool any_bad = false;
+        if (sc.ends())
+#pragma unroll
+          for (int k = 0; k < MAXW; ++k) any_bad |= bad[k] != 0;
+        if (any_bad) tree_bad_nodes<DH, TWO>(a, sc.b, sc.h, sc.len, sc.nodes, bad, mrow, e);
         else tree_store<DH, TWO>(a, sc.b, sc.h, sc.nodes, e);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      mbar_arrive(&sh->acc_free);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->acc_free);
     }
     if (!ok) {
       *abort = 1;
@@ -739,15 +787,16 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(AttnTreeArgs a, int b
   }
 }
 
-// K / V [P][KV][page][dh]: boxes of 64 columns and box_rows rows of one head's page
+// K / V [P][KV][page][dh] as [P][KV][dh / 64][page][64]: boxes of box_rows rows of one head's page and 64
+// columns; a box of 128 rows takes both halves of a head of 128, which land as two slices
 static bool cache_map(CUtensorMap* map, const AttnTreeArgs& a, const __half* base) {
   const EncodeTiledFn enc = encode_tiled();
   if (!enc) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)a.dh, (cuuint64_t)a.page, (cuuint64_t)a.KV, (cuuint64_t)a.P};
-  const cuuint64_t strides[3] = {(cuuint64_t)a.dh * 2, (cuuint64_t)a.page * a.dh * 2, (cuuint64_t)a.page_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)a.box_rows, 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dims, strides, box, estr,
+  const cuuint64_t dims[5] = {64, (cuuint64_t)a.page, (cuuint64_t)a.dh / 64, (cuuint64_t)a.KV, (cuuint64_t)a.P};
+  const cuuint64_t strides[4] = {(cuuint64_t)a.dh * 2, 128, (cuuint64_t)a.page * a.dh * 2, (cuuint64_t)a.page_stride * 2};
+  const cuuint32_t box[5] = {64, (cuuint32_t)a.box_rows, a.box_rows == 128 ? (cuuint32_t)a.dh / 64 : 1u, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<__half*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -809,6 +858,7 @@ static cudaError_t tc_launch(const AttnTreeArgs& a, cudaStream_t st) {
 cudaError_t attn_tree_tc_launch(AttnTreeArgs a, cudaStream_t st) {
   const int R = a.T * (a.H / a.KV);
   a.box_rows = box_rows(a);
+  a.page_shift = a.page & (a.page - 1) ? -1 : 31 - __builtin_clz((unsigned)a.page);
   a.box_shift = 31 - __builtin_clz((unsigned)a.box_rows);
   a.row_groups = (R + 255) / 256;
   a.out16 = a.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;

@@ -30,11 +30,16 @@ struct TreeSched {
   long long u, u1, item0;                      // next unit, end, the current pair's first unit
   int b, h, rg, nt;                            // the pair; its tiles
   int len, nodes;
+  int len1, nodes1;                            // the next sequence's, read ahead
   int t0;                                      // the segment's first tile
 
   AF_DEV void load(const AttnTreeArgs& a) {
     tree_extent(a, b, len, nodes);
+    ahead(a);
     nt = max(1, (len + nodes + 127) / 128);
+  }
+  AF_DEV void ahead(const AttnTreeArgs& a) {
+    if (b + 1 < a.B) tree_extent(a, b + 1, len1, nodes1);
   }
   // a whole warp: `first` unit of sequence `want`, `total` units; with want < 0 the sequence that holds
   // unit c * total / blocks
@@ -112,7 +117,10 @@ struct TreeSched {
       if (++h == a.KV) {
         h = 0;
         ++b;
-        load(a);
+        len = len1;
+        nodes = nodes1;
+        nt = max(1, (len + nodes + 127) / 128);
+        ahead(a);
       }
     }
   }
