@@ -50,8 +50,9 @@ constexpr int AHEAD = 8;                       // segments that the copies can b
 template <int DH, bool TWO> struct Cfg {
   static constexpr int TILE = SLICE * (DH / 64);
   static constexpr int QT = TWO ? 2 : 1;       // row tiles
-  static constexpr int NS = DH == 128 ? (TWO ? 5 : 6) : 8;   // ring slots (K or V tiles)
-  static constexpr int RING = QT * TILE;
+  static constexpr int QB = TWO ? 1 : 2;       // Q buffers: few rows come with short segments, whose Q is fetched ahead
+  static constexpr int NS = DH == 128 ? 5 : 8; // ring slots (K or V tiles)
+  static constexpr int RING = 2 * TILE;
   static constexpr int SH = RING + NS * TILE;
 };
 constexpr uint32_t S_COL = 0, O_COL = 256;     // S / P of stream w at 128 w, O at 256 + 128 w
@@ -62,7 +63,7 @@ template <int DH> struct IdescPV {
 }  // namespace tt
 
 struct TreeShared {
-  uint64_t q_full, q_empty;
+  uint64_t q_full[2], q_empty[2];
   uint64_t full[8], empty[8];
   uint64_t s_full[2], p_full[2], o_full[2];
   uint64_t acc_free;                           // both streams' O read out
@@ -325,13 +326,13 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
   if (!sc.init(a, blockIdx.x, gridDim.x, lane)) return;      // fewer tiles than blocks
 
   if (threadIdx.x == 0) {
-    mbar_init(&sh->q_full, 1);
-    mbar_init(&sh->q_empty, 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
     }
     for (int w = 0; w < 2; ++w) {
+      mbar_init(&sh->q_full[w], 1);
+      mbar_init(&sh->q_empty[w], 1);
       mbar_init(&sh->s_full[w], 1);
       mbar_init(&sh->p_full[w], 4);
       mbar_init(&sh->o_full[w], 1);
@@ -382,14 +383,17 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           if (lane == 0) *(volatile uint32_t*)&sh->bad[nseg % AHEAD][k] = m;
         }
       }
+      // Q of segment n lies in buffer n mod QB, free once the scores of segment n - QB are done
+      const int qb = nseg % C::QB, qn = nseg / C::QB;
       auto load_q = [&]() -> bool {
         dependency();
-        if (nseg && !tt_wait_warp(&sh->q_empty, (uint32_t)((nseg - 1) & 1), abort)) return false;
+        if (qn && !tt_wait_warp(&sh->q_empty[qb], (uint32_t)((qn - 1) & 1), abort)) return false;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&sh->q_full, C::QT * TILE);
+          mbar_arrive_expect_tx(&sh->q_full[qb], C::QT * TILE);
           for (int w = 0; w < C::QT; ++w)
             for (int k = 0; k < DH / 64; ++k)
-              tma_load_3d(smem + w * TILE + k * SLICE, &qmap, 64 * k, sc.rg * 256 + 128 * w, sc.b * a.KV + sc.h, &sh->q_full);
+              tma_load_3d(smem + (qb + w) * TILE + k * SLICE, &qmap, 64 * k, sc.rg * 256 + 128 * w, sc.b * a.KV + sc.h,
+                          &sh->q_full[qb]);
         }
         have_q = true;
         ++nq;
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         const unsigned live = (__ballot_sync(0xffffffffu, pages >= 0) >> (g * nbox)) & ((1u << nbox) - 1);
         if ((sc.t0 + j + 1) * BK > sc.len) dependency();     // the nodes' rows
         // Q at the latest when the ring is full of this segment; before, once the last one's scores are done
-        if (!have_q && (i >= NS || (waited && (!nseg || tt_done_warp(&sh->q_empty, (uint32_t)((nseg - 1) & 1))))) && !load_q()) {
+        if (!have_q && (i >= NS || (waited && (!qn || tt_done_warp(&sh->q_empty[qb], (uint32_t)((qn - 1) & 1))))) && !load_q()) {
           ok = false;
           break;
         }
@@ -454,8 +458,9 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         }
       }
       SpinBudget b;
-      while (nq && !mbar_try_wait(&sh->q_full, (uint32_t)((nq - 1) & 1)) && !b.spent()) {
-      }
+      for (int k = max(0, nq - C::QB); k < nq; ++k)
+        while (!mbar_try_wait(&sh->q_full[k % C::QB], (uint32_t)((k / C::QB) & 1)) && !b.spent()) {
+        }
     }
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------- products (one thread)
@@ -465,7 +470,8 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       uint32_t np[2] = {0, 0};                               // tiles of each stream so far
       for (; ok && sc.u < sc.u1; sc.next(a), ++nseg) {
         const int nt = sc.tiles();
-        const uint32_t qa = smem_u32(smem);
+        const int qb = nseg % C::QB;
+        const uint32_t qa = smem_u32(smem + qb * TILE);
         auto scores = [&](int w, int j, bool last_use) -> bool {
           const int seq = seq0 + seq_k<TWO>(j), st = seq % NS;
           if (!tt_wait(&sh->full[st], (uint32_t)((seq / NS) & 1), abort)) return false;
@@ -494,28 +500,28 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           if (last_use) mma_commit(&sh->empty[st]);
           return true;
         };
-        ok = tt_wait(&sh->q_full, (uint32_t)(nseg & 1), abort);
+        ok = tt_wait(&sh->q_full[qb], (uint32_t)((nseg / C::QB) & 1), abort);
         if (TWO) {
           ok = ok && scores(0, 0, false) && scores(1, 0, true);
-          if (ok && nt == 1) mma_commit(&sh->q_empty);
+          if (ok && nt == 1) mma_commit(&sh->q_empty[qb]);
           if (ok && nseg) ok = tt_wait(&sh->acc_free, (uint32_t)((nseg - 1) & 1), abort);
           for (int j = 0; ok && j < nt; ++j)
             for (int w = 0; ok && w < 2; ++w) {
               ok = values(w, j, j == 0, w == 1);
               if (ok && j == nt - 1) mma_commit(&sh->o_full[w]);
               if (ok && j + 1 < nt) ok = scores(w, j + 1, w == 1);
-              if (ok && j + 2 == nt && w == 1) mma_commit(&sh->q_empty);
+              if (ok && j + 2 == nt && w == 1) mma_commit(&sh->q_empty[qb]);
             }
         } else {
           ok = ok && scores(0, 0, true) && (nt < 2 || scores(1, 1, true));
-          if (ok && nt <= 2) mma_commit(&sh->q_empty);
+          if (ok && nt <= 2) mma_commit(&sh->q_empty[qb]);
           if (ok && nseg) ok = tt_wait(&sh->acc_free, (uint32_t)((nseg - 1) & 1), abort);
           for (int j = 0; ok && j < nt; ++j) {
             const int w = j & 1;
             ok = values(w, j, j < 2, true);
             if (ok && j + 2 >= nt) mma_commit(&sh->o_full[w]);
             if (ok && j + 2 < nt) ok = scores(w, j + 2, true);
-            if (ok && j + 3 == nt) mma_commit(&sh->q_empty);
+            if (ok && j + 3 == nt) mma_commit(&sh->q_empty[qb]);
           }
           if (ok && nt == 1) mma_commit(&sh->o_full[1]);     // the second stream had nothing
         }
@@ -528,7 +534,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
     // ------------------------------------------------------------- rows (two groups of four warps)
     const int w = warp >> 2, wr = (warp & 3) * 32 + lane;    // stream, row of the tile = TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t scol0 = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
+    const uint32_t scol = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
     const float sl2 = a.scale * 1.4426950408889634f;
     bool ok = true;
     int seq0 = 0, nseg = 0;
@@ -546,23 +552,17 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       const uint32_t* bad = sh->bad[nseg % AHEAD];           // written before the segment's first copy
       float m = -INFINITY, l = 0.f;
       bool first = true;
-      // The block's first tile is preceded by a dry one, while Q is on its way: the same instructions on columns of
-      // O that nothing uses yet, so that they are fetched (from an L2 full of K and V) before they are waited for.
-      for (int j = (TWO ? 0 : w) - (nseg ? 0 : TWO ? 1 : 2); j < nt; j += TWO ? 1 : 2) {
-        const bool dry = j < 0;
-        const uint32_t scol = dry ? ocol : scol0;
+      for (int j = TWO ? 0 : w; j < nt; j += TWO ? 1 : 2) {
         const int j0 = (sc.t0 + j) * BK;
-        const bool odd = j0 + BK > sc.len || dry;            // reaches past the prefix
+        const bool odd = j0 + BK > sc.len;                   // reaches past the prefix
         uint32_t vis[4];                                     // visible keys, while the scores are on their way
         if (odd) {
           see128(mrow, a.mask_words, t, j0 - sc.len, vis);
 #pragma unroll
           for (int c = 0; c < 4; ++c) vis[c] &= ones_below(sc.len + sc.nodes - j0 - 32 * c);
         }
-        if (!dry) {
-          if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
-          ++ns;
-        }
+        if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
+        ++ns;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool any_bad = false;
         if (odd || *(volatile int*)&sh->holes) {
@@ -570,12 +570,12 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           for (int k = 0; k < MAXW; ++k) any_bad |= bad[k] != 0;
           // keys that are not there: out of the scores; rows of V that nobody may see become zeros (whatever
           // lies there times a weight of 0 must be 0)
-          const int seqv = seq0 + (dry ? 0 : seq_v<TWO>(j, nt)), stv = seqv % NS;
-          if (!dry && !tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
+          const int seqv = seq0 + seq_v<TWO>(j, nt), stv = seqv % NS;
+          if (!tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
           const uint32_t boxes = *(volatile uint32_t*)&sh->vmask[stv];
           const int u = j0 + wr - sc.len;
           const bool isbad = any_bad && u >= 0 && u < TREE_MAX_NODES && (bad[u >> 5] >> (u & 31) & 1);
-          if (!dry && (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad)) {
+          if (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad) {
             unsigned char* vt = smem + C::RING + stv * TILE;
 #pragma unroll 1
             for (int c = 0; c < DH / 8; ++c)
@@ -589,6 +589,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
               for (int e = 0; e < 32; e += 8)                // a box has at least 8 rows
                 if (!(boxes >> ((32 * c + e) >> a.box_shift) & 1)) x &= ~(0xffu << e);
               if (any_bad)                                   // not the nodes that are added at the end
+#pragma unroll 1
                 for (int e = 0; e < 32; ++e) {
                   const int n = j0 + 32 * c + e - sc.len;
                   if (n >= 0 && n < TREE_MAX_NODES && (bad[n >> 5] >> (n & 31) & 1)) x &= ~(1u << e);
@@ -603,28 +604,30 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
         }
         if (live_warp) {
-          // the scores are read twice, 32 columns at a time with the next ones on their way: holding all 128
-          // costs spills whose first touches stalled whole tiles
+          // The scores are read twice, 32 columns at a time with the next ones on their way (holding all 128
+          // spills), in loops of two: a block meets this code cold, with the memory busy, and pays for its length.
           uint32_t v[2][32];
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           tmem_ld32_async(scol, v[0]);
+#pragma unroll 1
+          for (int c = 0; c < 4; c += 2) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld_wait();
-            after_wait(v[c & 1]);
-            if (c < 3) tmem_ld32_async(scol + 32 * (c + 1), v[(c + 1) & 1]);
+            for (int h = 0; h < 2; ++h) {
+              tmem_ld_wait();
+              after_wait(v[h]);
+              tmem_ld32_async(scol + 32 * ((c + h + 1) & 3), v[h ^ 1]);    // the last one: the first again
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[c & 1][e]));
+              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[h][e]));
+            }
           }
-          tmem_ld32_async(scol, v[0]);
           const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-          const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY || dry;
+          const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY;
           if (__any_sync(0xffffffffu, rise)) {
             const float mn = fmaxf(m, tm);
             const float corr = m == -INFINITY ? 0.f : tt_ex2(m - mn);
             m = mn;
             l *= corr;
-            if (!first || dry) {
+            if (!first) {
               // s_full came after the products before it, so O is at rest
 #pragma unroll 1
               for (int c0 = 0; c0 < DH; c0 += 16) {
@@ -638,30 +641,28 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
           const float mb = m == -INFINITY ? 0.f : m - SHIFT;
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int c = 0; c < 4; c += 2) {                   // P's columns 16 c.. lie in scores that were read
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {                      // P's columns 16 c.. lie in scores that were read
-            tmem_ld_wait();
-            after_wait(v[c & 1]);
-            if (c < 3) tmem_ld32_async(scol + 32 * (c + 1), v[(c + 1) & 1]);
-            uint32_t pk[16];
+            for (int h = 0; h < 2; ++h) {
+              tmem_ld_wait();
+              after_wait(v[h]);
+              if (c + h < 3) tmem_ld32_async(scol + 32 * (c + h + 1), v[h ^ 1]);
+              uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float p0 = tt_ex2(fmaf(__uint_as_float(v[c & 1][2 * e]), sl2, -mb));
-              const float p1 = tt_ex2(fmaf(__uint_as_float(v[c & 1][2 * e + 1]), sl2, -mb));
-              ps[(e & 1) * 2] += p0;
-              ps[(e & 1) * 2 + 1] += p1;
-              const __half2 hp = __floats2half2_rn(p0, p1);
-              pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
+              for (int e = 0; e < 16; ++e) {
+                const float p0 = tt_ex2(fmaf(__uint_as_float(v[h][2 * e]), sl2, -mb));
+                const float p1 = tt_ex2(fmaf(__uint_as_float(v[h][2 * e + 1]), sl2, -mb));
+                ps[(e & 1) * 2] += p0;
+                ps[(e & 1) * 2 + 1] += p1;
+                const __half2 hp = __floats2half2_rn(p0, p1);
+                pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
+              }
+              tmem_st16_async(scol + 16 * (c + h), pk);
             }
-            tmem_st16_async(scol + 16 * c, pk);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-        }
-        if (dry) {
-          m = -INFINITY;
-          l = 0.f;
-          continue;
         }
         first = false;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
