@@ -241,9 +241,8 @@ AF_DEV void tree_put(const AttnTreeArgs& a, int b, int h, int nodes, const TreeE
   }
 }
 
-// (not inlined, as the next one: once a segment, and its registers would be the tile loop's spills)
 template <int DH, bool TWO>
-__device__ __noinline__ void tree_store(const AttnTreeArgs& a, int b, int h, int nodes, TreeEnd e) {
+AF_DEV void tree_store(const AttnTreeArgs& a, int b, int h, int nodes, const TreeEnd& e) {
   if (e.part && (TWO || e.c0 == 0) && e.r < a.T * (a.H / a.KV))
     __stcg(reinterpret_cast<float2*>(e.part + (size_t)a.part_rows * DH) + e.pr, make_float2(e.m, e.l));
 #pragma unroll 1
