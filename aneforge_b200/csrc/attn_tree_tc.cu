@@ -1,9 +1,9 @@
 // Tree attention over a paged cache on the 5th-generation tensor cores (head dims 64 and 128).
 //
 // The T * G query rows that share a key head are the rows of one product; keys go through in tiles of
-// 128. A block (one per SM) holds two streams, each with its own scores S, running maximum and sum, and
-// output O in tensor memory, so that the tensor cores work on one stream while the other takes its
-// exponentials:
+// 64. A block (one per SM) holds two streams, each with its own scores S (two buffers: the next tile's
+// scores are formed while this one's exponentials are taken), running maximum and sum, and output O in
+// tensor memory:
 //   more than 128 rows   the streams are two tiles of 128 rows over the same keys (K and V read once)
 //   at most 128 rows     the streams take the even and the odd key tiles of the same rows, joined at the
 //                        end: O and O' = O e^(m - M) + O' e^(m' - M)
@@ -20,14 +20,14 @@
 // tree_combine joins in the order of the keys, so the result does not depend on timing. The cut comes
 // from lens on the device.
 //
-// K and V arrive by TMA in boxes of as many rows as divide the page (8..128, or 128 where a sequence is
+// K and V arrive by TMA in boxes of as many rows as divide the page (8..64, or 64 where a sequence is
 // one page) into a ring of tiles. Rows before the prefix's end are loaded while tree_append still runs.
 // Rows that hold nothing (past the last node, or without a page) are taken out of the scores and zeroed
 // in V; nodes whose k or v is not finite are taken out of the products too and added by the row's thread
 // at the end, for the rows that see them only.
 //
-// Roles (352 threads): warps 0-3 and 4-7 the streams' rows, warp 8 tensor memory and the products
-// (one thread), warps 9 and 10 the copies of K (and Q) and of V. Every wait is bounded; a block that gives up records
+// Roles (384 threads): warps 0-3 and 4-7 the streams' rows, warps 8 and 9 the streams' products (warp 8
+// owns the tensor memory), warps 10 and 11 the copies of K (and Q) and of V. Every wait is bounded; a block that gives up records
 // AF_DEV_WAIT_TIMEOUT, waits for its copies and products in flight, frees its tensor memory and returns.
 #include <cuda.h>
 
@@ -39,24 +39,29 @@
 namespace af {
 
 namespace tt {
-constexpr int BK = 128;                        // keys per tile
-constexpr int THREADS = 352;
-constexpr int MMA_WARP = 8, TMA_WARP = 9;
-constexpr int SLICE = 128 * 64 * 2;            // 128 rows x 64 fp16, 128-byte swizzled
+constexpr int BK = TREE_BK;                    // keys per tile
+constexpr int THREADS = 384;
+constexpr int MMA_WARP = 8, TMA_WARP = 10;     // two warps each
+constexpr int QSLICE = 128 * 64 * 2;           // 128 rows x 64 fp16, 128-byte swizzled
+constexpr int SLICE = BK * 64 * 2;             // a tile's keys x 64 fp16
 constexpr long long LIMIT = 1ll << 26;
 constexpr float SHIFT = 6.f, RISE = 8.f;       // log2 of the weights' factor; rise of the maximum that is let pass
 constexpr int MAXW = TREE_MAX_NODES / 32;
-constexpr int AHEAD = 8;                       // segments that the copies can be ahead: under NS
+constexpr int NS = 10;                         // ring slots (K or V tiles)
+constexpr int AHEAD = 16;                      // segments that the copies can be ahead: under NS
 template <int DH, bool TWO> struct Cfg {
-  static constexpr int TILE = SLICE * (DH / 64);
+  static constexpr int TILE = SLICE * (DH / 64), QTILE = QSLICE * (DH / 64);
   static constexpr int QT = TWO ? 2 : 1;       // row tiles
   static constexpr int QB = TWO ? 1 : 2;       // Q buffers: few rows come with short segments, whose Q is fetched ahead
-  static constexpr int NS = DH == 128 ? 5 : 8; // ring slots (K or V tiles)
-  static constexpr int RING = 2 * TILE;
+  static constexpr int RING = 2 * QTILE;
   static constexpr int SH = RING + NS * TILE;
+  // Split streams have half of the ring each: a slot's fills are waited for by one warp, in order. (A parity
+  // cannot tell a fill from the one before the last, so nobody may wait for a fill before the last one of its
+  // slot has landed.)
+  static constexpr int HS = TWO ? NS : NS / 2;
 };
-constexpr uint32_t S_COL = 0, O_COL = 256;     // S / P of stream w at 128 w, O at 256 + 128 w
-constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+constexpr uint32_t S_COL = 0, O_COL = 256;     // S / P of stream w at 128 w (two buffers of 64), O at 256 + 128 w
+constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 template <int DH> struct IdescPV {
   static constexpr uint32_t v = (1u << 4) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 };
@@ -64,12 +69,13 @@ template <int DH> struct IdescPV {
 
 struct TreeShared {
   uint64_t q_full[2], q_empty[2];
-  uint64_t full[8], empty[8];
-  uint64_t s_full[2], p_full[2], o_full[2];
-  uint64_t acc_free;                           // both streams' O read out
+  uint64_t full[tt::NS], empty[tt::NS];
+  uint64_t s_full[2][2], p_full[2][2];         // of a stream's buffers
+  uint64_t pv_done[2];                         // a stream's O += P V is done (every tile)
+  uint64_t o_full[2], acc_free[2];             // a stream's O is complete; read out (every segment with tiles for it)
   uint64_t done;
   float2 ml[2][128];                           // split streams: (m, l) of the other half
-  uint32_t vmask[8];                           // boxes of the tile that have a page
+  uint32_t vmask[tt::NS];                      // boxes of the tile that have a page
   uint32_t bad[tt::AHEAD][tt::MAXW];           // nodes whose k or v is not finite, of a segment (modulo AHEAD)
   uint32_t tmem;
   int holes;                                   // some row of the segments so far has no page
@@ -154,6 +160,25 @@ AF_DEV void mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, u
       ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// the same with the accumulation known beforehand
+AF_DEV void mma_f16_c(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  if (accumulate)
+    asm volatile("{\n .reg .pred p;\n setp.eq.u32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc) : "memory");
+}
+AF_DEV void mma_f16_ts_c(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc) {
+  asm volatile("{\n .reg .pred p;\n setp.eq.u32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc) : "memory");
+}
+AF_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // a box of a page: rows from `row`, 64 columns from 64 * half (or all 128 columns, as two slices)
 AF_DEV void tma_load_5d(void* dst, const CUtensorMap* map, int row, int half, int h, int page, uint64_t* bar) {
   asm volatile(
@@ -161,30 +186,30 @@ AF_DEV void tma_load_5d(void* dst, const CUtensorMap* map, int row, int half, in
       ::"r"(smem_u32(dst)), "l"(map), "r"(0), "r"(row), "r"(half), "r"(h), "r"(page), "r"(smem_u32(bar)) : "memory");
 }
 
-// where a tile's K and V stand in the order in which they are loaded and used: two row tiles K0 V0 K1 V1
-// ..., split streams K0 K1 V0 K2 V1 K3 ...
-template <bool TWO> AF_DEV int seq_k(int j) { return TWO ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
-template <bool TWO> AF_DEV int seq_v(int j, int nt) { return TWO ? 2 * j + 1 : (j == nt - 1 ? 2 * nt - 1 : 2 * j + 2); }
+// where a stream's K and V stand in the order in which they are loaded and used: K0 K1 V0 K2 V1 ... (the
+// scores are formed two tiles ahead)
+AF_DEV int seq_k(int i) { return i < 2 ? i : 2 * i - 1; }
+AF_DEV int seq_v(int i, int n) { return i < n - 2 ? 2 + 2 * i : n + i; }
 
-// visibility of the 128 nodes from node number u0 (may be negative: prefix rows) for a node's mask row; the
-// five words that this can reach are loaded together
-AF_DEV void see128(const int* mask, int words, int t, int u0, uint32_t (&vis)[4]) {
+// visibility of the 64 nodes from node number u0 (may be negative: prefix rows) for a node's mask row; the
+// three words that this can reach are loaded together
+AF_DEV void see64(const int* mask, int words, int t, int u0, uint32_t (&vis)[2]) {
   const int w0 = u0 >> 5, s = u0 & 31;         // floor division: u0 = 32 w0 + s
-  uint32_t x[5];
+  uint32_t x[3];
 #pragma unroll
-  for (int k = 0; k < 5; ++k) {
+  for (int k = 0; k < 3; ++k) {
     const int w = w0 + k;
     x[k] = 0;
     if (mask && w >= 0 && w < words) x[k] = (uint32_t)__ldg(mask + w);
   }
 #pragma unroll
-  for (int k = 0; k < 5; ++k) {
+  for (int k = 0; k < 3; ++k) {
     const int w = w0 + k, n = t - 32 * w;      // chain: nodes 0..t
     if (w < 0) x[k] = 0xffffffffu;
     else if (!mask) x[k] = n < 0 ? 0u : n >= 31 ? 0xffffffffu : (2u << n) - 1;
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) vis[k] = __funnelshift_r(x[k], x[k + 1], s);
+  for (int k = 0; k < 2; ++k) vis[k] = __funnelshift_r(x[k], x[k + 1], s);
 }
 AF_DEV uint32_t ones_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
@@ -309,7 +334,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
                         const __grid_constant__ CUtensorMap vmap) {
   using namespace tt;
   using C = Cfg<DH, TWO>;
-  constexpr int NS = C::NS, TILE = C::TILE;
+  constexpr int TILE = C::TILE, QTILE = C::QTILE, HS = C::HS;
   // the swizzle's period is 1024 bytes; there is no room to align by hand, so a wrong base is an error
   extern __shared__ __align__(1024) unsigned char tt_raw[];
   unsigned char* smem = tt_raw;
@@ -327,17 +352,20 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&sh->full[s], 1);
-      mbar_init(&sh->empty[s], 1);
+      mbar_init(&sh->empty[s], C::QT);         // every stream that reads it
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh->q_full[w], 1);
-      mbar_init(&sh->q_empty[w], 1);
-      mbar_init(&sh->s_full[w], 1);
-      mbar_init(&sh->p_full[w], 4);
+      mbar_init(&sh->q_empty[w], 2);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&sh->s_full[w][k], 1);
+        mbar_init(&sh->p_full[w][k], 4);
+      }
+      mbar_init(&sh->pv_done[w], 1);
       mbar_init(&sh->o_full[w], 1);
+      mbar_init(&sh->acc_free[w], 8);
     }
-    mbar_init(&sh->acc_free, 8);
-    mbar_init(&sh->done, 1);
+    mbar_init(&sh->done, 2);
     sh->abort = 0;
     sh->holes = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -356,9 +384,9 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
   if (warp >= TMA_WARP) {
     // ------------------------------------------------------------- copies: a warp for K (and Q), one for V
     const bool is_v = warp == TMA_WARP + 1;
-    const int nbox = BK >> a.box_shift, per = 32 / nbox;     // boxes of a tile (at most 16), tiles of a page read
+    const int nbox = BK >> a.box_shift, per = 32 / nbox;     // boxes of a tile (at most 8), tiles of a page read
     bool waited = false, ok = true;
-    int seq0 = 0, nseg = 0, nq = 0;
+    int seq0[2] = {0, 0}, nseg = 0, nq = 0;                  // loads of each stream so far (two row tiles: of both)
     uint32_t armed = 0, phase = 0;                           // slots that were filled here, and their last phase
     auto dependency = [&] {                                  // q and the nodes' rows come from tree_append
       if (waited) return;
@@ -366,7 +394,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       asm volatile("fence.proxy.async.global;" ::: "memory");
       waited = true;
     };
-    for (; ok && sc.u < sc.u1; sc.next(a), ++nseg) {
+    for (bool more = true; ok && more; more = sc.next(a), ++nseg) {
       const int nt = sc.tiles();
       bool have_q = is_v;
       if (!is_v) {
@@ -388,10 +416,10 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         dependency();
         if (qn && !tt_wait_warp(&sh->q_empty[qb], (uint32_t)((qn - 1) & 1), abort)) return false;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&sh->q_full[qb], C::QT * TILE);
+          mbar_arrive_expect_tx(&sh->q_full[qb], C::QT * QTILE);
           for (int w = 0; w < C::QT; ++w)
             for (int k = 0; k < DH / 64; ++k)
-              tma_load_3d(smem + (qb + w) * TILE + k * SLICE, &qmap, 64 * k, sc.rg * 256 + 128 * w, sc.b * a.KV + sc.h,
+              tma_load_3d(smem + (qb + w) * QTILE + k * QSLICE, &qmap, 64 * k, sc.rg * 256 + 128 * w, sc.b * a.KV + sc.h,
                           &sh->q_full[qb]);
         }
         have_q = true;
@@ -406,7 +434,8 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       };
       int pages = -2, pages1 = pages_of(0);
       for (int j = 0; j < nt; ++j) {
-        const int i = is_v ? seq_v<TWO>(j, nt) : seq_k<TWO>(j), seq = seq0 + i, st = seq % NS;
+        const int w = TWO ? 0 : j & 1, n = TWO ? nt : (nt + 1 - w) >> 1, i = TWO ? j : j >> 1;
+        const int local = is_v ? seq_v(i, n) : seq_k(i), seq = (w ? seq0[1] : seq0[0]) + local, st = w * HS + seq % HS;
         const int g = j % per;
         if (g == 0) {
           pages = pages1;
@@ -420,11 +449,11 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         const unsigned live = (__ballot_sync(0xffffffffu, pages >= 0) >> (g * nbox)) & ((1u << nbox) - 1);
         if ((sc.t0 + j + 1) * BK > sc.len) dependency();     // the nodes' rows
         // Q at the latest when the ring is full of this segment; before, once the last one's scores are done
-        if (!have_q && (i >= NS || (waited && (!qn || tt_done_warp(&sh->q_empty[qb], (uint32_t)((qn - 1) & 1))))) && !load_q()) {
+        if (!have_q && (local >= HS || (waited && (!qn || tt_done_warp(&sh->q_empty[qb], (uint32_t)((qn - 1) & 1))))) && !load_q()) {
           ok = false;
           break;
         }
-        if (seq >= NS && !tt_wait_warp(&sh->empty[st], (uint32_t)((seq / NS - 1) & 1), abort)) { ok = false; break; }
+        if (seq >= HS && !tt_wait_warp(&sh->empty[st], (uint32_t)((seq / HS - 1) & 1), abort)) { ok = false; break; }
         if (lane == 0) {
           sh->vmask[st] = live;
           mbar_arrive_expect_tx(&sh->full[st], (uint32_t)(__popc(live) * a.box_rows * (DH * 2)));
@@ -442,10 +471,11 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
         }
         armed |= 1u << st;
-        phase = (phase & ~(1u << st)) | (uint32_t)((seq / NS) & 1) << st;
+        phase = (phase & ~(1u << st)) | (uint32_t)((seq / HS) & 1) << st;
       }
       if (ok && !have_q) ok = load_q();
-      seq0 += 2 * nt;
+      seq0[0] += 2 * (TWO ? nt : (nt + 1) >> 1);
+      seq0[1] += 2 * (nt >> 1);
     }
     if (!ok) *abort = 1;
     dependency();
@@ -461,85 +491,87 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         while (!mbar_try_wait(&sh->q_full[k % C::QB], (uint32_t)((k / C::QB) & 1)) && !b.spent()) {
         }
     }
-  } else if (warp == MMA_WARP) {
-    // ------------------------------------------------------------- products (one thread)
-    if (lane == 0) {
-      bool ok = true;
-      int seq0 = 0, nseg = 0;
-      uint32_t np[2] = {0, 0};                               // tiles of each stream so far
-      for (; ok && sc.u < sc.u1; sc.next(a), ++nseg) {
-        const int nt = sc.tiles();
-        const int qb = nseg % C::QB;
-        const uint32_t qa = smem_u32(smem + qb * TILE);
-        auto scores = [&](int w, int j, bool last_use) -> bool {
-          const int seq = seq0 + seq_k<TWO>(j), st = seq % NS;
-          if (!tt_wait(&sh->full[st], (uint32_t)((seq / NS) & 1), abort)) return false;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t kb = smem_u32(smem + C::RING + st * TILE), qw = qa + (TWO ? w * TILE : 0);
+  } else if (warp >= MMA_WARP) {
+    // ------------------------------------------------------------- products: a warp for each stream
+    // The whole warp walks through them, so that descriptors stay in uniform registers; one lane issues (in a
+    // branch of one lane alone every product cost about 70 cycles of moves to uniform registers).
+    const int w = warp - MMA_WARP;
+    const bool leader = elect_one();
+    bool ok = true;
+    int seq0 = 0, nseg = 0;
+    uint32_t cs = 0, cv = 0;                                 // tiles so far: scores, values
+    int nown = 0;                                            // segments with tiles for this stream
+    const uint64_t qdesc0 = smem_desc(smem_u32(smem)), kdesc0 = smem_desc(smem_u32(smem + C::RING));
+    const uint64_t vdesc0 = smem_desc_mn(smem_u32(smem + C::RING), SLICE, 1024);
+    for (bool more = true; ok && more; more = sc.next(a), ++nseg) {
+      const int nt = sc.tiles(), qb = nseg % C::QB;
+      const int n = TWO ? nt : (nt + 1 - w) >> 1;            // the stream's tiles
+      auto scores = [&](int i) -> bool {
+        const int seq = seq0 + seq_k(i), st = (TWO ? 0 : w * HS) + seq % HS;
+        if (!tt_wait_warp(&sh->full[st], (uint32_t)((seq / HS) & 1), abort)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t kd = kdesc0 + (uint32_t)(st * (TILE >> 4)), qd = qdesc0 + (uint32_t)((TWO ? w : qb) * (QTILE >> 4));
+        const uint32_t buf = cs & 1, d = tmem + S_COL + 128 * w + 64 * buf;
+        if (leader) {
 #pragma unroll
-          for (int ks = 0; ks < DH / 16; ++ks) {
-            const uint32_t off = (uint32_t)((ks >> 2) * SLICE + (ks & 3) * 32);
-            mma_f16(tmem + S_COL + 128 * w, smem_desc(qw + off), smem_desc(kb + off), IDESC_S, ks != 0);
-          }
-          mma_commit(&sh->s_full[w]);
-          if (last_use) mma_commit(&sh->empty[st]);
-          return true;
-        };
-        auto values = [&](int w, int j, bool first, bool last_use) -> bool {
-          const int seq = seq0 + seq_v<TWO>(j, nt), st = seq % NS;
-          if (!tt_wait(&sh->full[st], (uint32_t)((seq / NS) & 1), abort)) return false;
-          if (!tt_wait(&sh->p_full[w], np[w] & 1, abort)) return false;
-          ++np[w];
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t vb = smem_u32(smem + C::RING + st * TILE);
-#pragma unroll
-          for (int ks = 0; ks < BK / 16; ++ks)
-            mma_f16_ts(tmem + O_COL + 128 * w, tmem + S_COL + 128 * w + ks * 8, smem_desc_mn(vb + (uint32_t)(ks * 2048), SLICE, 1024),
-                       IdescPV<DH>::v, !(first && ks == 0));
-          if (last_use) mma_commit(&sh->empty[st]);
-          return true;
-        };
-        ok = tt_wait(&sh->q_full[qb], (uint32_t)((nseg / C::QB) & 1), abort);
-        if (TWO) {
-          ok = ok && scores(0, 0, false) && scores(1, 0, true);
-          if (ok && nt == 1) mma_commit(&sh->q_empty[qb]);
-          if (ok && nseg) ok = tt_wait(&sh->acc_free, (uint32_t)((nseg - 1) & 1), abort);
-          for (int j = 0; ok && j < nt; ++j)
-            for (int w = 0; ok && w < 2; ++w) {
-              ok = values(w, j, j == 0, w == 1);
-              if (ok && j == nt - 1) mma_commit(&sh->o_full[w]);
-              if (ok && j + 1 < nt) ok = scores(w, j + 1, w == 1);
-              if (ok && j + 2 == nt && w == 1) mma_commit(&sh->q_empty[qb]);
-            }
-        } else {
-          ok = ok && scores(0, 0, true) && (nt < 2 || scores(1, 1, true));
-          if (ok && nt <= 2) mma_commit(&sh->q_empty[qb]);
-          if (ok && nseg) ok = tt_wait(&sh->acc_free, (uint32_t)((nseg - 1) & 1), abort);
-          for (int j = 0; ok && j < nt; ++j) {
-            const int w = j & 1;
-            ok = values(w, j, j < 2, true);
-            if (ok && j + 2 >= nt) mma_commit(&sh->o_full[w]);
-            if (ok && j + 2 < nt) ok = scores(w, j + 2, true);
-            if (ok && j + 3 == nt) mma_commit(&sh->q_empty[qb]);
-          }
-          if (ok && nt == 1) mma_commit(&sh->o_full[1]);     // the second stream had nothing
+          for (int ks = 0; ks < DH / 16; ++ks)
+            mma_f16_c(d, qd + (uint32_t)(((ks >> 2) * QSLICE + (ks & 3) * 32) >> 4), kd + (uint32_t)(((ks >> 2) * SLICE + (ks & 3) * 32) >> 4),
+                      IDESC_S, ks != 0);
+          mma_commit(&sh->s_full[w][buf]);
+          mma_commit(&sh->empty[st]);
+          if (i == n - 1) mma_commit(&sh->q_empty[qb]);
         }
-        seq0 += 2 * nt;
+        __syncwarp();
+        ++cs;
+        return true;
+      };
+      ok = tt_wait_warp(&sh->q_full[qb], (uint32_t)((nseg / C::QB) & 1), abort);
+      for (int i = 0; ok && i < min(2, n); ++i) ok = scores(i);
+      if (n == 0 && leader) mbar_arrive(&sh->q_empty[qb]);   // no tile for this stream
+      __syncwarp();
+      if (ok && n) {                                         // O is free once the stream's last segment was read out
+        if (nown) ok = tt_wait_warp(&sh->acc_free[w], (uint32_t)((nown - 1) & 1), abort);
+        ++nown;
       }
+      for (int i = 0; ok && i < n; ++i) {
+        const int seq = seq0 + seq_v(i, n), st = (TWO ? 0 : w * HS) + seq % HS;
+        const uint32_t buf = cv & 1;
+        ok = tt_wait_warp(&sh->full[st], (uint32_t)((seq / HS) & 1), abort) &&
+             tt_wait_warp(&sh->p_full[w][buf], (cv >> 1) & 1, abort);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t vd = vdesc0 + (uint32_t)(st * (TILE >> 4));
+        const uint32_t d = tmem + O_COL + 128 * w, p = tmem + S_COL + 128 * w + 64 * buf;
+        if (leader) {
+          mma_f16_ts(d, p, vd, IdescPV<DH>::v, i != 0);      // the first tile begins O
+#pragma unroll
+          for (int ks = 1; ks < BK / 16; ++ks) mma_f16_ts_c(d, p + ks * 8, vd + (uint32_t)(ks * 2048 >> 4), IdescPV<DH>::v);
+          mma_commit(&sh->pv_done[w]);
+          mma_commit(&sh->empty[st]);
+          if (i == n - 1) mma_commit(&sh->o_full[w]);
+        }
+        __syncwarp();
+        ++cv;
+        if (i + 2 < n) ok = scores(i + 2);
+      }
+      seq0 += 2 * n;
+    }
+    if (leader) {
       if (!ok) *abort = 1;
       mma_commit(&sh->done);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------- rows (two groups of four warps)
     const int w = warp >> 2, wr = (warp & 3) * 32 + lane;    // stream, row of the tile = TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t scol = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
+    const uint32_t scol0 = lanes + S_COL + 128 * w, ocol = lanes + O_COL + 128 * w;
     const float sl2 = a.scale * 1.4426950408889634f;
     bool ok = true;
     int seq0 = 0, nseg = 0;
-    uint32_t ns = 0;                                         // tiles of this stream so far
+    uint32_t ns = 0, no0 = 0, no1 = 0;                       // tiles of this stream; segments with tiles for stream 0, 1
     pdl_wait();                                              // q, for the nodes that are added at the end
-    for (; sc.u < sc.u1; sc.next(a), ++nseg) {
+    for (bool more = true; more; more = sc.next(a), ++nseg) {
       // all rows go on, or none (barriers lie ahead); `bad` is free from here
       ok = rows_all(ok);
       if (!ok) break;
@@ -554,14 +586,14 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       for (int j = TWO ? 0 : w; j < nt; j += TWO ? 1 : 2) {
         const int j0 = (sc.t0 + j) * BK;
         const bool odd = j0 + BK > sc.len;                   // reaches past the prefix
-        uint32_t vis[4];                                     // visible keys, while the scores are on their way
+        uint32_t vis[2];                                     // visible keys, while the scores are on their way
         if (odd) {
-          see128(mrow, a.mask_words, t, j0 - sc.len, vis);
+          see64(mrow, a.mask_words, t, j0 - sc.len, vis);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) vis[c] &= ones_below(sc.len + sc.nodes - j0 - 32 * c);
+          for (int c = 0; c < 2; ++c) vis[c] &= ones_below(sc.len + sc.nodes - j0 - 32 * c);
         }
-        if (!tt_wait_warp(&sh->s_full[w], ns & 1, abort)) { ok = false; break; }
-        ++ns;
+        const uint32_t buf = ns & 1, scol = scol0 + 64 * buf;
+        if (!tt_wait_warp(&sh->s_full[w][buf], (ns >> 1) & 1, abort)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool any_bad = false;
         if (odd || *(volatile int*)&sh->holes) {
@@ -569,12 +601,12 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           for (int k = 0; k < MAXW; ++k) any_bad |= bad[k] != 0;
           // keys that are not there: out of the scores; rows of V that nobody may see become zeros (whatever
           // lies there times a weight of 0 must be 0)
-          const int seqv = seq0 + seq_v<TWO>(j, nt), stv = seqv % NS;
-          if (!tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / NS) & 1), abort)) { ok = false; break; }
+          const int seqv = seq0 + (TWO ? seq_v(j, nt) : seq_v(j >> 1, (nt + 1 - w) >> 1)), stv = (TWO ? 0 : w * HS) + seqv % HS;
+          if (!tt_wait_warp(&sh->full[stv], (uint32_t)((seqv / HS) & 1), abort)) { ok = false; break; }
           const uint32_t boxes = *(volatile uint32_t*)&sh->vmask[stv];
           const int u = j0 + wr - sc.len;
           const bool isbad = any_bad && u >= 0 && u < TREE_MAX_NODES && (bad[u >> 5] >> (u & 31) & 1);
-          if (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad) {
+          if (wr < BK && (u >= sc.nodes || !(boxes >> (wr >> a.box_shift) & 1) || isbad)) {
             unsigned char* vt = smem + C::RING + stv * TILE;
 #pragma unroll 1
             for (int c = 0; c < DH / 8; ++c)
@@ -583,8 +615,8 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           if (live_warp) {
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t x = !odd ? 0xffffffffu : c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+            for (int c = 0; c < 2; ++c) {
+              uint32_t x = !odd ? 0xffffffffu : c ? vis[1] : vis[0];
               for (int e = 0; e < 32; e += 8)                // a box has at least 8 rows
                 if (!(boxes >> ((32 * c + e) >> a.box_shift) & 1)) x &= ~(0xffu << e);
               if (any_bad)                                   // not the nodes that are added at the end
@@ -603,21 +635,17 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
         }
         if (live_warp) {
-          // The scores are read twice, 32 columns at a time with the next ones on their way (holding all 128
-          // spills), in loops of two: a block meets this code cold, with the memory busy, and pays for its length.
           uint32_t v[2][32];
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           tmem_ld32_async(scol, v[0]);
-#pragma unroll 1
-          for (int c = 0; c < 4; c += 2) {
+          tmem_ld32_async(scol + 32, v[1]);
+          tmem_ld_wait();
+          after_wait(v[0]);
+          after_wait(v[1]);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              tmem_ld_wait();
-              after_wait(v[h]);
-              tmem_ld32_async(scol + 32 * ((c + h + 1) & 3), v[h ^ 1]);    // the last one: the first again
-#pragma unroll
-              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[h][e]));
-            }
+          for (int e = 0; e < 32; ++e) {
+            mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(v[0][e]));
+            mx[2 + (e & 1)] = fmaxf(mx[2 + (e & 1)], __uint_as_float(v[1][e]));
           }
           const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
           const bool rise = tm > m + (first ? 0.f : RISE) || m == -INFINITY;
@@ -627,7 +655,9 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
             m = mn;
             l *= corr;
             if (!first) {
-              // s_full came after the products before it, so O is at rest
+              // once the products before this tile are done
+              if (!tt_wait_warp(&sh->pv_done[w], (ns - 1) & 1, abort)) { ok = false; break; }
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
               for (int c0 = 0; c0 < DH; c0 += 16) {
                 uint32_t o[16];
@@ -640,25 +670,19 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           }
           const float mb = m == -INFINITY ? 0.f : m - SHIFT;
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int c = 0; c < 4; c += 2) {                   // P's columns 16 c.. lie in scores that were read
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              tmem_ld_wait();
-              after_wait(v[h]);
-              if (c + h < 3) tmem_ld32_async(scol + 32 * (c + h + 1), v[h ^ 1]);
-              uint32_t pk[16];
+          for (int h = 0; h < 2; ++h) {                      // P takes the scores' first columns
+            uint32_t pk[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float p0 = tt_ex2(fmaf(__uint_as_float(v[h][2 * e]), sl2, -mb));
-                const float p1 = tt_ex2(fmaf(__uint_as_float(v[h][2 * e + 1]), sl2, -mb));
-                ps[(e & 1) * 2] += p0;
-                ps[(e & 1) * 2 + 1] += p1;
-                const __half2 hp = __floats2half2_rn(p0, p1);
-                pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
-              }
-              tmem_st16_async(scol + 16 * (c + h), pk);
+            for (int e = 0; e < 16; ++e) {
+              const float p0 = tt_ex2(fmaf(__uint_as_float(v[h][2 * e]), sl2, -mb));
+              const float p1 = tt_ex2(fmaf(__uint_as_float(v[h][2 * e + 1]), sl2, -mb));
+              ps[(e & 1) * 2] += p0;
+              ps[(e & 1) * 2 + 1] += p1;
+              const __half2 hp = __floats2half2_rn(p0, p1);
+              pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
             }
+            tmem_st16_async(scol + 16 * h, pk);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
@@ -666,12 +690,16 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         first = false;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[w]);
+        if (lane == 0) mbar_arrive(&sh->p_full[w][buf]);
+        ++ns;
       }
-      seq0 += 2 * nt;
+      seq0 += 2 * (TWO ? nt : (nt + 1 - w) >> 1);
       // ---- the segment's end
-      ok = ok && tt_wait_warp(&sh->o_full[w], (uint32_t)(nseg & 1), abort);
-      if (!TWO) ok = ok && tt_wait_warp(&sh->o_full[w ^ 1], (uint32_t)(nseg & 1), abort);
+      const bool both = TWO || nt > 1;                       // stream 1 has tiles too
+      if (!TWO || w == 0) ok = ok && tt_wait_warp(&sh->o_full[0], no0 & 1, abort);
+      if (both && (!TWO || w == 1)) ok = ok && tt_wait_warp(&sh->o_full[1], no1 & 1, abort);
+      ++no0;
+      no1 += both;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float f0 = first ? 0.f : 1.f, f1 = 0.f;                // weights of O and of the other stream's O
       if (!TWO) {
@@ -704,7 +732,10 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->acc_free);
+      if (lane == 0) {
+        mbar_arrive(&sh->acc_free[0]);
+        if (both) mbar_arrive(&sh->acc_free[1]);
+      }
     }
     if (!ok) {
       *abort = 1;
@@ -742,7 +773,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(AttnTreeArgs a, int b
   long long first, total;
   sc.find(a, b, tid & 31, first, total);
   blocks = (int)min((long long)blocks, total);
-  const long long u0 = first + (long long)(h * a.row_groups + rg) * sc.nt, u1 = u0 + sc.nt;
+  const long long u0 = first + (long long)(h * a.row_groups + rg) * (sc.nt + TREE_PAIR) + TREE_PAIR, u1 = u0 + sc.nt;
   const int c0 = tree_block_of(u0, total, blocks), c1 = tree_block_of(u1 - 1, total, blocks);
   if (c0 == c1) return;                        // the pair is whole
   const int lr = tid % ROWS, c4 = tid / ROWS, r = row0 + lr, pr = r - rg * 256;
@@ -788,13 +819,13 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(AttnTreeArgs a, int b
 }
 
 // K / V [P][KV][page][dh] as [P][KV][dh / 64][page][64]: boxes of box_rows rows of one head's page and 64
-// columns; a box of 128 rows takes both halves of a head of 128, which land as two slices
+// columns; a box of a whole tile takes both halves of a head of 128, which land as two slices
 static bool cache_map(CUtensorMap* map, const AttnTreeArgs& a, const __half* base) {
   const EncodeTiledFn enc = encode_tiled();
   if (!enc) return false;
   const cuuint64_t dims[5] = {64, (cuuint64_t)a.page, (cuuint64_t)a.dh / 64, (cuuint64_t)a.KV, (cuuint64_t)a.P};
   const cuuint64_t strides[4] = {(cuuint64_t)a.dh * 2, 128, (cuuint64_t)a.page * a.dh * 2, (cuuint64_t)a.page_stride * 2};
-  const cuuint32_t box[5] = {64, (cuuint32_t)a.box_rows, a.box_rows == 128 ? (cuuint32_t)a.dh / 64 : 1u, 1, 1};
+  const cuuint32_t box[5] = {64, (cuuint32_t)a.box_rows, a.box_rows == TREE_BK ? (cuuint32_t)a.dh / 64 : 1u, 1, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<__half*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -817,7 +848,9 @@ int attn_tree_tc_blocks() { const int n = device_attr(cudaDevAttrMultiProcessorC
 
 // rows of a page that one box can cover: a box never crosses a page (unless the sequence is one page,
 // where it ends at the map's bound), and starts at a multiple of 8 rows, the swizzle's period
-static int box_rows(const AttnTreeArgs& a) { return a.W == 1 ? 128 : (a.page & -a.page) > 128 ? 128 : a.page & -a.page; }
+static int box_rows(const AttnTreeArgs& a) {
+  return a.W == 1 || (a.page & -a.page) > TREE_BK ? TREE_BK : a.page & -a.page;
+}
 
 bool attn_tree_tc_ok(const AttnTreeArgs& a) {
   return (a.dh == 64 || a.dh == 128) && a.scale > 0.f && a.scale < 1e30f && box_rows(a) >= 8;
