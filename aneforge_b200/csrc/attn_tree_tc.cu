@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
 
   if (warp >= TMA_WARP) {
     // ------------------------------------------------------------- copies: a warp for K (and Q), one for V
-    const bool is_v = warp == TMA_WARP + 1;
+    const bool is_v = warp == TMA_WARP + 1, leader = elect_one();
     const int nbox = BK >> a.box_shift, per = 32 / nbox;     // boxes of a tile (at most 8), tiles of a page read
     bool waited = false, ok = true;
     int seq0[2] = {0, 0}, nseg = 0, nq = 0;                  // loads of each stream so far (two row tiles: of both)
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
           break;
         }
         if (seq >= HS && !tt_wait_warp(&sh->empty[st], (uint32_t)((seq / HS - 1) & 1), abort)) { ok = false; break; }
-        if (lane == 0) {
+        if (leader) {
           sh->vmask[st] = live;
           mbar_arrive_expect_tx(&sh->full[st], (uint32_t)(__popc(live) * a.box_rows * (DH * 2)));
         }
@@ -462,14 +462,24 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
         const int row = (sc.t0 + j) * BK;
         unsigned char* slot = smem + C::RING + st * TILE;
         const CUtensorMap* map = is_v ? &vmap : &kmap;
-        for (int k = 0; k < nbox; ++k) {
-          const int pk = __shfl_sync(0xffffffffu, pages, g * nbox + k);
-          if (pk >= 0 && lane == 0) {
-            const int y = row + k * a.box_rows, in = a.page_shift >= 0 ? y & (a.page - 1) : y % a.page;
-            tma_load_5d(slot + k * a.box_rows * 128, map, in, 0, sc.h, pk, &sh->full[st]);
-            if (DH == 128 && nbox > 1) tma_load_5d(slot + SLICE + k * a.box_rows * 128, map, in, 1, sc.h, pk, &sh->full[st]);
+        int pk[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) pk[k] = __shfl_sync(0xffffffffu, pages, (g * nbox + k) & 31);
+        if (leader) {
+          if (nbox == 1) {
+            if (pk[0] >= 0) tma_load_5d(slot, map, a.page_shift >= 0 ? row & (a.page - 1) : row % a.page, 0, sc.h, pk[0], &sh->full[st]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k < nbox && pk[k] >= 0) {
+                const int y = row + k * a.box_rows, in = a.page_shift >= 0 ? y & (a.page - 1) : y % a.page;
+#pragma unroll
+                for (int c = 0; c < DH / 64; ++c)
+                  tma_load_5d(slot + c * SLICE + k * a.box_rows * 128, map, in, c, sc.h, pk[k], &sh->full[st]);
+              }
           }
         }
+        __syncwarp();
         armed |= 1u << st;
         phase = (phase & ~(1u << st)) | (uint32_t)((seq / HS) & 1) << st;
       }
