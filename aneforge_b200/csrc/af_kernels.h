@@ -359,6 +359,7 @@ struct KvPagesArgs {
   int D = 0;
   int* lens_out = nullptr;             // compact: [S]
   int* scratch = nullptr;              // reserve: kv_reserve_scratch_bytes
+  int heads = 0;                       // set by the launcher: heads that a block copies
   int* err = nullptr;
 };
 cudaError_t kv_free_launch(const KvPagesArgs& a, cudaStream_t st);

@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(pages::THREADS) kv_fork_kernel(KvPagesArgs a) 
 // scratch: copies [n][4] = (old page, new page, rows, -), then the numbers of the free pages handed out
 __global__ void __launch_bounds__(pages::THREADS) kv_reserve_kernel(KvPagesArgs a) {
   __shared__ int list[pages::THREADS], warp_sums[32];
+  pdl_trigger();                                // the copies' blocks may take their places
   const int i = threadIdx.x;
   const int s = own_slot(a.slots, a.n, a.S, list, a.err);
   int c0 = 0, c1 = 0, fill = 0, tail = -1;
@@ -213,75 +214,98 @@ __global__ void __launch_bounds__(pages::THREADS) kv_reserve_kernel(KvPagesArgs 
   }
 }
 
-// grid (n, 2 * layers): the filled rows of one copied page, every head, one layer's K or V
+// grid (n, 2 * layers, head groups): the filled rows of one copied page, one layer's K or V, a.heads heads.
+// A head's rows are contiguous; four 16-byte pieces a thread are on their way together.
 __global__ void __launch_bounds__(256) kv_copy_kernel(KvPagesArgs a) {
-  const int4 c = reinterpret_cast<const int4*>(a.scratch)[blockIdx.x];
+  pdl_wait();                                   // the list comes from kv_reserve
+  const int4 c = __ldcg(reinterpret_cast<const int4*>(a.scratch) + blockIdx.x);
   if (c.x < 0) return;
   const size_t head = (size_t)a.page * a.row16, pg = head * a.KV;
+  const int h0 = blockIdx.z * a.heads, h1 = min(a.KV, h0 + a.heads);
   uint4* plane = static_cast<uint4*>(a.pool) + (size_t)blockIdx.y * a.P * pg;
-  const uint4* from = plane + (size_t)c.x * pg;
-  uint4* to = plane + (size_t)c.y * pg;
-  const int per = c.z * a.row16;                // 16-byte pieces of a head's filled rows
-  for (int e = threadIdx.x; e < per * a.KV; e += blockDim.x) {
-    const size_t o = (size_t)(e / per) * head + e % per;
-    to[o] = from[o];
+  const int per = c.z * a.row16;                // pieces of a head's filled rows
+  for (int h = h0; h < h1; ++h) {
+    const uint4* from = plane + (size_t)c.x * pg + h * head;
+    uint4* to = plane + (size_t)c.y * pg + h * head;
+    for (int e = threadIdx.x; e < per; e += 4 * 256) {
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + 256 * k < per) v[k] = __ldcs(from + e + 256 * k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + 256 * k < per) __stcs(to + e + 256 * k, v[k]);
+    }
   }
 }
 
-// a path is taken if its nodes rise (parents come before children) and its rows have pages
-AF_DEV bool path_ok(const KvPagesArgs& a, int b, int s, int n, int len, const int* table) {
+// whether rows j, j + step, ... of a path can be taken: its nodes rise (parents come before children) and
+// its rows have pages
+AF_DEV bool path_bad(const KvPagesArgs& a, int b, int s, int n, int len, int j, int step) {
   bool bad = s < 0 || s >= a.S || n < 0 || n > a.D;
-  if (!bad)
-    for (int j = threadIdx.x; j < n; j += blockDim.x) {
-      const int at = a.path[(size_t)b * a.D + j];
-      const long long from = (long long)len + at;
-      bad |= at < j || (j && at <= a.path[(size_t)b * a.D + j - 1]) || from >= (long long)a.W * a.page;
-      if (!bad) {
-        const int p = table[from / a.page], q = table[(len + j) / a.page];
-        bad |= p < 0 || p >= a.P || q < 0 || q >= a.P;
-      }
+  if (bad) return true;
+  const int* table = a.table + (size_t)s * a.W;
+  for (; j < n && !bad; j += step) {
+    const int at = a.path[(size_t)b * a.D + j];
+    const long long from = (long long)len + at;
+    bad = at < j || (j && at <= a.path[(size_t)b * a.D + j - 1]) || from >= (long long)a.W * a.page;
+    if (!bad) {
+      const int p = table[from / a.page], q = table[(len + j) / a.page];
+      bad = p < 0 || p >= a.P || q < 0 || q >= a.P;
     }
-  return !__syncthreads_or(bad);
+  }
+  return bad;
 }
 
-// grid (B, 2 * layers + 1): one layer's K or V of one sequence; the last blocks (y = 2 * layers) write
-// the new lengths. A thread moves one 16-byte column of one head through the rows of the path in order:
-// row j is written after row path[j] >= j is read and no later row is read from it, so that no other
-// thread's access meets it.
+// grid (B, 2 * layers + 1): one layer's K or V of one sequence; block (0, 2 * layers) writes the new
+// lengths. A thread moves one 16-byte column of one head through the rows of the path in order: row j is
+// written after row path[j] >= j is read and no later row is read from it, so that no other thread's
+// access meets it.
 __global__ void __launch_bounds__(256) kv_compact_kernel(KvPagesArgs a) {
-  const int b = blockIdx.x;
-  const int s = a.slots[b], n = a.rows[b];
-  const bool in = s >= 0 && s < a.S;
-  const int len = in ? a.lens[s] : 0;
-  const int* table = a.table + (size_t)(in ? s : 0) * a.W;
-  const bool ok = path_ok(a, b, s, n, len, table);
   if (blockIdx.y == 2 * a.layers) {
-    if (threadIdx.x == 0) {
-      if (in) a.lens_out[s] = len + (ok ? n : 0);
-      if (!ok) af_set_err(a.err, AF_DEV_BAD_SLOT);
+    if (blockIdx.x) return;
+    for (int s = threadIdx.x; s < a.S; s += blockDim.x) a.lens_out[s] = a.lens[s];
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    for (int b = threadIdx.x >> 5; b < a.n; b += blockDim.x >> 5) {
+      const int s = a.slots[b], n = a.rows[b], len = s >= 0 && s < a.S ? a.lens[s] : 0;
+      const bool bad = __any_sync(0xffffffffu, path_bad(a, b, s, n, len, lane, 32));
+      if (lane == 0) {
+        if (bad) af_set_err(a.err, AF_DEV_BAD_SLOT);
+        else a.lens_out[s] = len + n;
+      }
     }
     return;
   }
-  if (!ok) return;
+  const int b = blockIdx.x;
+  const int s = a.slots[b], n = a.rows[b];
+  const int len = s >= 0 && s < a.S ? a.lens[s] : 0;
+  __shared__ size_t from_s[256], to_s[256];     // places of the rows, 256 at a time
+  if (__syncthreads_or(path_bad(a, b, s, n, len, threadIdx.x, blockDim.x))) return;
+  const int* table = a.table + (size_t)s * a.W;
   const size_t head = (size_t)a.page * a.row16, pg = head * a.KV;
   uint4* plane = static_cast<uint4*>(a.pool) + (size_t)blockIdx.y * a.P * pg;
-  for (int e = threadIdx.x; e < a.KV * a.row16; e += blockDim.x) {
-    uint4* col = plane + (size_t)(e / a.row16) * head + e % a.row16;
-    constexpr int U = 8;
-    for (int j0 = 0; j0 < n; j0 += U) {
-      uint4 v[U];
+  for (int base = 0; base < n; base += 256) {
+    const int m = min(256, n - base);
+    __syncthreads();
+    if ((int)threadIdx.x < m) {
+      const int r = len + a.path[(size_t)b * a.D + base + threadIdx.x], w = len + base + threadIdx.x;
+      from_s[threadIdx.x] = (size_t)table[r / a.page] * pg + (size_t)(r % a.page) * a.row16;
+      to_s[threadIdx.x] = (size_t)table[w / a.page] * pg + (size_t)(w % a.page) * a.row16;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.KV * a.row16; e += blockDim.x) {
+      uint4* col = plane + (size_t)(e / a.row16) * head + e % a.row16;
+      constexpr int U = 8;
+      for (int j0 = 0; j0 < m; j0 += U) {
+        uint4 v[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (j0 + k < n) {
-          const int r = len + a.path[(size_t)b * a.D + j0 + k];
-          v[k] = col[(size_t)table[r / a.page] * pg + (size_t)(r % a.page) * a.row16];
-        }
+        for (int k = 0; k < U; ++k)
+          if (j0 + k < m) v[k] = col[from_s[j0 + k]];
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (j0 + k < n) {
-          const int r = len + j0 + k;
-          col[(size_t)table[r / a.page] * pg + (size_t)(r % a.page) * a.row16] = v[k];
-        }
+        for (int k = 0; k < U; ++k)
+          if (j0 + k < m) col[to_s[j0 + k]] = v[k];
+      }
     }
   }
 }
@@ -317,15 +341,26 @@ cudaError_t kv_reserve_launch(const KvPagesArgs& a, cudaStream_t st) {
     return cudaErrorInvalidValue;
   if (a.n == 0) return cudaSuccess;
   kv_reserve_kernel<<<1, pages::THREADS, 0, st>>>(a);
-  kv_copy_kernel<<<dim3(a.n, 2 * a.layers), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  // blocks of all heads where there are plenty, of fewer where the copies would not fill the GPU
+  KvPagesArgs c = a;
+  c.heads = a.KV;
+  while (c.heads > 1 && (long long)a.n * 2 * a.layers * ((a.KV + c.heads - 1) / c.heads) < 8 * 148) c.heads = (c.heads + 1) / 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(a.n, 2 * a.layers, (a.KV + c.heads - 1) / c.heads);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, kv_copy_kernel, c);
 }
 
 cudaError_t kv_compact_launch(const KvPagesArgs& a, cudaStream_t st) {
   if (!pages_ok(a) || ((!a.rows || !a.path) && a.n) || !pool_ok(a) || a.D < 1 || !a.lens_out || a.lens_out == a.lens)
     return cudaErrorInvalidValue;
-  const cudaError_t e = cudaMemcpyAsync(a.lens_out, a.lens, 4 * (size_t)a.S, cudaMemcpyDeviceToDevice, st);
-  if (e != cudaSuccess || a.n == 0) return e;
+  if (a.n == 0) return cudaMemcpyAsync(a.lens_out, a.lens, 4 * (size_t)a.S, cudaMemcpyDeviceToDevice, st);
   kv_compact_kernel<<<dim3(a.n, 2 * a.layers + 1), 256, 0, st>>>(a);
   return cudaGetLastError();
 }

@@ -335,65 +335,71 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   fp16 [B * T, H * dh], zeros for nodes that see nothing or are not live. err: int32 [1], zero: gets the device
   error code of a node without a page or rotary position."""
   import torch
-  _need(qkv.is_cuda and qkv.dtype == torch.float32 and qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be fp32 [B * T, cols] on the GPU")
-  _need(table.dim() == 2, "table must be int32 [B, W]")
-  B, W = table.shape
-  _need(KV >= 1 and H % KV == 0 and qkv.shape[1] >= (H + 2 * KV) * dh, "qkv needs (H + 2 KV) dh columns, H a multiple of KV")
-  _need(B >= 1 and qkv.shape[0] % B == 0 and qkv.shape[0] >= B, "qkv needs the same number of rows for each sequence of the table")
-  T = qkv.shape[0] // B
-  _need(T <= 256, "at most 256 nodes")
-  _need(dh in (16, 32, 64, 128), "head dims 16, 32, 64 and 128")
-  _need(kc.shape == vc.shape and kc.dim() == 4 and kc.dtype == vc.dtype == torch.float16 and kc.is_cuda and vc.is_cuda,
-        "kc / vc must be fp16 [P, KV, page, dh] on the GPU")
-  P, kvh, page, d = kc.shape
-  _need(kvh == KV and d == dh, "kc / vc must be fp16 [P, KV, page, dh] on the GPU")
-  ps = kc.stride(0) if P > 1 else KV * page * dh
-  _need(kc.stride()[1:] == (page * dh, dh, 1) and vc.stride() == kc.stride() and ps >= KV * page * dh and ps % 8 == 0,
-        "kc / vc pages must be contiguous, and alike")
-  pt, pl = _i32(table, (B, W), "table"), _i32(lens, (B,), "lens")
-  pn = 0 if nodes is None else _i32(nodes, (B,), "nodes")
-  pd = 0 if depth is None else _i32(depth, (B, T), "depth")
+  f16 = torch.float16
+  if not (qkv.is_cuda and qkv.dtype == torch.float32 and qkv.dim() == 2 and table.dim() == 2):
+    raise ValueError("qkv must be fp32 [B * T, cols] on the GPU and table int32 [B, W]")
+  (n, cols), (ld, one), (B, W) = qkv.shape, qkv.stride(), table.shape
+  if not (one == 1 and KV >= 1 and H % KV == 0 and cols >= (H + 2 * KV) * dh):
+    raise ValueError("qkv needs contiguous rows of (H + 2 KV) dh columns, H a multiple of KV")
+  if not (B >= 1 and n >= B and n % B == 0 and n <= 256 * B):
+    raise ValueError("qkv needs the same number of rows, 1 to 256, for each sequence of the table")
+  T = n // B
+  if dh not in (16, 32, 64, 128):
+    raise ValueError("head dims 16, 32, 64 and 128")
+  shape, strides = kc.shape, kc.stride()
+  if not (kc.dtype == f16 and vc.dtype == f16 and kc.is_cuda and vc.is_cuda and vc.shape == shape and len(shape) == 4
+          and shape[1] == KV and shape[3] == dh):
+    raise ValueError("kc / vc must be fp16 [P, KV, page, dh] on the GPU")
+  P, _, page, _ = shape
+  ps = strides[0] if P > 1 else KV * page * dh
+  if not (strides[1:] == (page * dh, dh, 1) and vc.stride() == strides and ps >= KV * page * dh and ps % 8 == 0):
+    raise ValueError("kc / vc pages must be contiguous, and alike")
   words = (T + 31) // 32
-  pm = 0 if mask is None else _i32(mask, (B, T, words), "mask")
   rows = 0
   if cos_t is not None:
     rows = cos_t.shape[0]
-    _need(cos_t.shape == sin_t.shape == (rows, dh) and cos_t.dtype == sin_t.dtype == torch.float16 and cos_t.is_contiguous()
-          and sin_t.is_contiguous() and cos_t.is_cuda and sin_t.is_cuda, "cos_t / sin_t must be fp16 [rows, dh] on the GPU")
+    if not (cos_t.shape == (rows, dh) and sin_t.shape == (rows, dh) and cos_t.dtype == f16 and sin_t.dtype == f16
+            and cos_t.is_contiguous() and sin_t.is_contiguous() and cos_t.is_cuda and sin_t.is_cuda):
+      raise ValueError("cos_t / sin_t must be fp16 [rows, dh] on the GPU")
   for g, name in ((qn, "qn"), (kn, "kn")):
-    _need(g is None or (g.is_cuda and g.dtype == torch.float16 and g.shape == (dh,) and g.is_contiguous()), f"{name} must be fp16 [dh] on the GPU")
+    if g is not None and not (g.is_cuda and g.dtype == f16 and g.shape == (dh,) and g.is_contiguous()):
+      raise ValueError(f"{name} must be fp16 [dh] on the GPU")
   if out is None:
-    out = torch.empty((B * T, H * dh), dtype=torch.float16, device=qkv.device)
+    out = qkv.new_empty((n, H * dh), dtype=f16)
+    ldo = H * dh
   else:
-    _need(out.is_cuda and out.dtype == torch.float16 and out.shape == (B * T, H * dh) and out.stride(1) == 1, "out must be fp16 [B * T, H * dh]")
+    if not (out.is_cuda and out.dtype == f16 and out.shape == (n, H * dh) and out.stride(1) == 1):
+      raise ValueError("out must be fp16 [B * T, H * dh]")
+    ldo = out.stride(0)
   if scratch is None:
     scratch = attn_tree_scratch(B, T, H, KV, dh, qkv.device)
-  R.check(R.lib().af_attn_tree(qkv.data_ptr(), qkv.stride(0), kc.data_ptr(), vc.data_ptr(), ps, P, page, pt, W, pl, pn, pd, pm,
-                               words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), float(qn_floor), float(kn_floor),
-                               out.data_ptr(), out.stride(0), B, T, H, KV, dh, float(scale), scratch.data_ptr(),
-                               scratch.numel(), _p(err), _stream(qkv)), "af_attn_tree")
+  rc = R.lib().af_attn_tree(
+    qkv.data_ptr(), ld, kc.data_ptr(), vc.data_ptr(), ps, P, page, _i32(table, (B, W), "table"), W, _i32(lens, (B,), "lens"),
+    0 if nodes is None else _i32(nodes, (B,), "nodes"), 0 if depth is None else _i32(depth, (B, T), "depth"),
+    0 if mask is None else _i32(mask, (B, T, words), "mask"), words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), qn_floor,
+    kn_floor, out.data_ptr(), ldo, B, T, H, KV, dh, scale, scratch.data_ptr(), scratch.numel(), _p(err), _stream(qkv))
+  if rc:
+    R.check(rc, "af_attn_tree")
   return out
 
 
 def _book(table, lens, refs, slots):
-  import torch
-  _need(table.dim() == 2 and lens.dim() == 1 and slots.dim() == 1, "table [S, W], lens [S] and slots [n] are wanted")
+  if not (table.dim() == 2 and lens.dim() == 1 and slots.dim() == 1 and (refs is None or refs.dim() == 1)):
+    raise ValueError("table [S, W], lens [S], refs [P] and slots [n] are wanted")
   S, W = table.shape
   n = slots.shape[0]
-  _need(n <= 1024, "at most 1024 slots a call")
-  pr = 0
-  if refs is not None:
-    _need(refs.dim() == 1, "refs must be int32 [P]")
-    pr = _i32(refs, refs.shape, "refs")
-  return _i32(table, (S, W), "table"), S, W, _i32(lens, (S,), "lens"), pr, _i32(slots, (n,), "slots"), n
+  if n > 1024:
+    raise ValueError("at most 1024 slots a call")
+  return (_i32(table, (S, W), "table"), S, W, _i32(lens, (S,), "lens"), 0 if refs is None else _i32(refs, refs.shape, "refs"),
+          _i32(slots, (n,), "slots"), n)
 
 
 def _pool(pool):
-  import torch
-  _need(pool.is_cuda and pool.dim() == 6 and pool.shape[1] == 2 and pool.is_contiguous() and pool.element_size() == 2,
-        "pool must be a contiguous 16-bit CUDA tensor [layers, 2, P, KV, page, dh]")
-  L, _, P, KV, page, dh = pool.shape
-  _need(2 * dh % 16 == 0, "dh must be a multiple of 8")
+  if not (pool.is_cuda and pool.dim() == 6 and pool.is_contiguous() and pool.element_size() == 2):
+    raise ValueError("pool must be a contiguous 16-bit CUDA tensor [layers, 2, P, KV, page, dh]")
+  L, two, P, KV, page, dh = pool.shape
+  if two != 2 or dh % 8:
+    raise ValueError("pool must be [layers, 2, P, KV, page, dh], dh a multiple of 8")
   return L, P, KV, page, 2 * dh
 
 
@@ -410,14 +416,15 @@ def kv_fork(table, lens, refs, src, dst, page, err=None):
 def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
   """Rows [lens, lens + rows[i]) of each slot get pages of the slot's own: free ones, lowest number first, and
   copies (in every layer of pool [layers, 2, P, KV, page, dh]) of a shared page that rows are appended to."""
-  import torch
   pt, S, W, pl, pr, ps, n = _book(table, lens, refs, slots)
   L, P, KV, page, rb = _pool(pool)
   _need(refs.shape[0] == P, "refs must have an entry for each page of the pool")
+  lib = R.lib()
+  need = lib.af_kv_reserve_scratch_bytes(n, P)
   if scratch is None:
-    scratch = torch.empty((R.lib().af_kv_reserve_scratch_bytes(n, P),), dtype=torch.uint8, device=pool.device)
-  R.check(R.lib().af_kv_reserve(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows"), n,
-                                scratch.data_ptr(), scratch.numel(), _p(err), _stream(pool)), "af_kv_reserve")
+    scratch = refs.new_empty((need // 4 + 1,))               # int32
+  R.check(lib.af_kv_reserve(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows"), n,
+                                scratch.data_ptr(), scratch.numel() * scratch.element_size(), _p(err), _stream(pool)), "af_kv_reserve")
 
 
 def kv_free(table, lens, refs, slots, page, keep=None, err=None):
@@ -432,13 +439,12 @@ def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
   """The rows lens + path[i, j], j < n_path[i], of each slot move to lens + j in every layer's K and V: the accepted
   path [n, D] through a drafted tree (node numbers, rising) becomes part of the prefix. Returns the new lengths:
   lens with n_path added to the listed slots (a new tensor, or lens_out)."""
-  import torch
   pt, S, W, pl, _, ps, n = _book(table, lens, None, slots)
   L, P, KV, page, rb = _pool(pool)
   _need(path.dim() == 2, "path must be int32 [n, D]")
   D = path.shape[1]
   if lens_out is None:
-    lens_out = torch.empty_like(lens)
+    lens_out = lens.new_empty(lens.shape)
   _need(lens_out.data_ptr() != lens.data_ptr(), "lens_out must be another buffer than lens")
   R.check(R.lib().af_kv_compact(pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path"), D,
                                 _i32(n_path, (n,), "n_path"), n, _i32(lens_out, (S,), "lens_out"), _p(err), _stream(pool)),
