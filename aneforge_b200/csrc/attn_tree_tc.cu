@@ -785,7 +785,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(AttnTreeArgs a, int b
   blocks = (int)min((long long)blocks, total);
   const long long u0 = first + (long long)(h * a.row_groups + rg) * (sc.nt + TREE_PAIR) + TREE_PAIR, u1 = u0 + sc.nt;
   const int c0 = tree_block_of(u0, total, blocks), c1 = tree_block_of(u1 - 1, total, blocks);
-  if (c0 == c1) return;                        // the pair is whole
+  if (c0 == c1) {                              // the pair is whole
+    pdl_wait();                                // a grid that ended sooner would let its dependents read early
+    return;
+  }
   const int lr = tid % ROWS, c4 = tid / ROWS, r = row0 + lr, pr = r - rg * 256;
   const int n = c1 - c0 + 1;
   for (int k = tid; k < n; k += 256) part_s[k] = (c0 + k) * 2 + (tree_unit(c0 + k, total, blocks) > u0 ? 0 : 1);

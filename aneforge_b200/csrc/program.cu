@@ -37,7 +37,7 @@ static void set_error(const std::string& msg) {
 
 void set_error_public(const std::string& msg) { set_error(msg); }
 
-enum Role { R_IN, R_OUT, R_STATE, R_TMP, R_WEIGHT, R_SCRATCH };
+enum Role { R_IN, R_OUT, R_STATE, R_TMP, R_WEIGHT, R_SCRATCH, R_EXT };   // R_EXT: always the caller's memory (bind)
 
 struct Buffer {
   std::string name;
@@ -80,6 +80,7 @@ static bool parse_role(const std::string& s, Role& r) {
   else if (s == "tmp") r = R_TMP;
   else if (s == "weight") r = R_WEIGHT;
   else if (s == "scratch") r = R_SCRATCH;
+  else if (s == "ext") r = R_EXT;
   else return false;
   return true;
 }
@@ -668,6 +669,58 @@ static cudaError_t run_op(Program& p, const Op& op, bool dry, std::string& why) 
       e = rope_kv_prefill_launch(a, qbuf, st);
       if (e == cudaSuccess) e = attn_prefill_with_q(a, qbuf, st);
     }
+  } else if (op.kind == "attn_tree") {
+    AttnTreeArgs a;
+    a.B = (int)c.i("b"); a.T = (int)c.i("t"); a.H = (int)c.i("h"); a.KV = (int)c.i("kv"); a.dh = (int)c.i("dh");
+    a.P = (int)c.i("p"); a.page = (int)c.i("page"); a.W = (int)c.i("w");
+    a.rope_rows = (int)c.i("rows", 0);
+    if (a.B < 1 || a.T < 1 || a.T > TREE_MAX_NODES || a.KV < 1 || a.H < 1 || a.H % a.KV || a.dh < 1 || a.P < 1 || a.page < 1 || a.W < 1)
+      c.err = "attn_tree: bad dimensions";
+    if (!c.err.empty()) { why = c.err; return cudaErrorInvalidValue; }
+    const size_t n = (size_t)a.B * a.T;
+    a.ld_qkv = (a.H + 2 * a.KV) * a.dh;
+    a.ld_out = a.H * a.dh;
+    a.page_stride = (long long)a.KV * a.page * a.dh;
+    a.qkv = (const float*)c.ptr("qkv", 4 * n * a.ld_qkv);
+    a.kc = (__half*)c.ptr("kc", 2 * (size_t)a.P * a.page_stride);
+    a.vc = (__half*)c.ptr("vc", 2 * (size_t)a.P * a.page_stride);
+    a.table = (const int*)c.ptr("table", 4 * (size_t)a.B * a.W);
+    a.lens = (const int*)c.ptr("lens", 4 * (size_t)a.B);
+    a.nodes = (const int*)c.ptr("nodes", 4 * (size_t)a.B, true);
+    a.depth = (const int*)c.ptr("depth", 4 * n, true);
+    a.mask_words = (a.T + 31) / 32;
+    a.mask = (const int*)c.ptr("mask", 4 * n * a.mask_words, true);
+    a.cos_t = (const __half*)c.ptr("cos", 2 * (size_t)a.rope_rows * a.dh, true);
+    a.sin_t = (const __half*)c.ptr("sin", 2 * (size_t)a.rope_rows * a.dh, true);
+    a.qn_g = (const __half*)c.ptr("qn", 2 * (size_t)a.dh, true);
+    a.kn_g = (const __half*)c.ptr("kn", 2 * (size_t)a.dh, true);
+    a.qn_floor = (float)c.f("qnf", 0.0);
+    a.kn_floor = (float)c.f("knf", 0.0);
+    a.out = (__half*)c.ptr("out", 2 * n * a.ld_out);
+    a.scale = (float)c.f("scale");
+    a.scratch_bytes = attn_tree_scratch_bytes(a.B, a.T, a.H, a.KV, a.dh);
+    a.scratch = c.ptr("scr", a.scratch_bytes);
+    a.err = p.d_err;
+    if ((a.cos_t == nullptr) != (a.sin_t == nullptr)) c.err = "cos/sin must both be given";
+    if (!c.err.empty()) { why = c.err; return cudaErrorInvalidValue; }
+    if (!dry) e = attn_tree_launch(a, st, pdl);
+  } else if (op.kind == "sample") {
+    SampleArgs a;
+    a.R = (int)c.i("nb"); a.V = (int)c.i("v");
+    a.ld = c.i("ld", a.V);
+    if (a.R < 1 || a.V < 1 || a.ld < a.V) c.err = "sample: bad dimensions";
+    if (!c.err.empty()) { why = c.err; return cudaErrorInvalidValue; }
+    const size_t row = 4 * (size_t)a.R;
+    a.logits = c.ptr("logits", 4 * ((size_t)(a.R - 1) * a.ld + a.V));
+    a.u = (const float*)c.ptr("u", row);
+    a.temperature = (const float*)c.ptr("temp", row);
+    a.top_k = (const int*)c.ptr("topk", row);
+    a.top_p = (const float*)c.ptr("topp", row);
+    a.min_p = (const float*)c.ptr("minp", row);
+    a.tok = (int*)c.ptr("tok", row);
+    a.logp = (float*)c.ptr("logp", row, true);
+    if (!c.err.empty()) { why = c.err; return cudaErrorInvalidValue; }
+    if (!dry) e = sample_launch(a, st, pdl);
   } else if (op.kind.compare(0, 2, "g_") == 0) {
     if (!graph_op(c, op, dry, st, e, why)) return cudaErrorInvalidValue;
   } else if (op.kind == "moe_gate") {
@@ -823,7 +876,7 @@ static bool parse_plan(Program& p, const std::string& text, std::string& err) {
 static bool alloc_buffers(Program& p, std::string& err) {
   for (auto& b : p.bufs) {
     const size_t bytes = ((b.bytes + 255) / 256) * 256;
-    if (bytes == 0) continue;
+    if (bytes == 0 || b.role == R_EXT) continue;
     cudaError_t e = cudaMalloc(&b.dev, bytes);
     if (e != cudaSuccess) { err = "cudaMalloc(" + b.name + ", " + std::to_string(bytes) + ") failed: " + cudaGetErrorString(e); return false; }
     b.owned = true;
@@ -931,7 +984,7 @@ static int launch_all(Program& p) {
 
 static int finalize(Program& p) {
   for (auto& b : p.bufs)
-    if (b.role == R_WEIGHT && !b.ready && b.alias_of < 0) {
+    if ((b.role == R_WEIGHT || b.role == R_EXT) && !b.ready && b.alias_of < 0) {
       set_error("weight buffer '" + b.name + "' was never uploaded or bound");
       return -1;
     }

@@ -218,6 +218,18 @@ def emit_attention_decode(pb, ctx, li, lw, cfg, ls):
   pre = f"L{li}"
   _emit_attn_norm(pb, cfg, pre, lw, NB)
   _emit_linear(pb, ctx, f"{pre}.qkv", lw["qkv"], "xn", "qkv", "f32")
+  if ctx.get("tree"):
+    # a tree of tokens per sequence over a paged cache: K / V of the nodes are appended, then each attends to
+    # the prefix and its ancestors (the GQA factor leaves every normal fp16 number as it is)
+    kv = dict(qkv="qkv", kc=f"{pre}.K", vc=f"{pre}.V", table="kv.table", lens="kv.lens", nodes="nodes", depth="depth",
+              mask="mask", out="att", scr="tree.scr", h=H, kv=KV, dh=dh, scale=ctx["scale"], **ctx["tree"])
+    if cfg.rope:
+      kv.update(cos="rope.cos", sin="rope.sin")
+    if ls.qk_norm:
+      kv.update(qn=f"{pre}.qn", kn=f"{pre}.kn", qnf=lw["qn_floor"], knf=lw["kn_floor"])
+    pb.op("attn_tree", **kv)
+    _emit_row_parallel(pb, ctx, f"{pre}.o", lw["o"], "att")
+    return
   # prefetch=1: the step's position is only advanced by its last kernel (the head), so attention may
   # stage its first cache rows before the qkv projection finishes
   kv = dict(qkv="qkv", kc=f"{pre}.K", vc=f"{pre}.V", pos="pos", out="att", nb=NB, h=H, kv=KV, dh=dh, m=M,

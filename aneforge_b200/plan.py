@@ -10,7 +10,7 @@ from dataclasses import dataclass, field
 class Buf:
   name: str
   nbytes: int
-  role: str               # in | out | state | tmp | weight | scratch
+  role: str               # in | out | state | tmp | weight | scratch | ext (the caller's memory, bound)
 
 
 @dataclass
@@ -20,7 +20,7 @@ class PlanBuilder:
   wfile: dict = field(default_factory=dict)
 
   def buf(self, name: str, nbytes: int, role: str) -> str:
-    if role not in ("in", "out", "state", "tmp", "weight", "scratch"):
+    if role not in ("in", "out", "state", "tmp", "weight", "scratch", "ext"):
       raise ValueError(role)
     nbytes = int(nbytes)
     if name in self.bufs:

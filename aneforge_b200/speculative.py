@@ -108,3 +108,118 @@ def spec_generate(target: LlamaPrefill, draft: LlamaPrefill, token_ids, max_new_
   if stats is not None:
     stats.update(verify_steps=n_verify, accepted=n_accept)
   return out[:max_new_tokens]
+
+
+def tree_parents(branches):
+  """Parents of a tree with a root and branches[d] children of every node of level d, level by level."""
+  parents, level = [-1], [0]
+  for b in branches:
+    if int(b) < 1:
+      raise ValueError("branches must be positive")
+    parents += [p for p in level for _ in range(int(b))]
+    level = list(range(len(parents) - len(level) * int(b), len(parents)))
+  return parents
+
+
+def tree_generate(target: LlamaPrefill, draft: LlamaPrefill, token_ids, max_new_tokens=40, eos_id=None, branches=(3, 2, 1),
+                  temperature=0.0, top_p=1.0, top_k=0, min_p=0.0, seed=None, page=64, on_token=None,
+                  stats: dict | None = None):
+  """Speculative decoding with a drafted tree: every round the draft proposes its branches[d] best tokens after
+  each node of level d, the target runs the last token and the whole tree in one step and draws its own token
+  after every node, the matching path is kept in both caches and its tokens and one more are emitted. The head's
+  logits are the device's. `stats` gets the number of target steps and of accepted draft tokens."""
+  from .paged import PagedKV, TreeStep, _stops
+  prompt = [int(t) for t in token_ids]
+  target._check_ids(prompt)
+  parents = tree_parents(branches)
+  T, depth = len(parents), len(branches)
+  if T > 256:
+    raise ValueError("a tree has at most 256 nodes")
+  if draft.device != target.device or draft.cfg.vocab != target.cfg.vocab:
+    raise ValueError("draft and target must share a vocabulary and a device")
+  if not prompt or max_new_tokens < 1:
+    return []
+  eos, P = _stops(eos_id), len(prompt)
+  children = [[] for _ in parents]
+  for t, p in enumerate(parents):
+    if p >= 0:
+      children[p].append(t)
+  rows = P + max_new_tokens + T
+  dev = torch.device("cuda", target.device)
+  rng = np.random.default_rng(seed)
+  kvt, kvd = (PagedKV(m.cfg, 1, rows, page=page, device=m.device) for m in (target, draft))
+  last = P + max_new_tokens + depth                          # positions of drafted nodes stay below
+  big = TreeStep(target, kvt, 1, parents, last, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+  small = None
+  try:
+    small = TreeStep(draft, kvd, 1, parents, last)
+    logits = None
+    for model, kv, step in ((draft, kvd, small), (target, kvt, big)):
+      pre, real, _ = model._prefill_hidden(prompt)
+      with torch.cuda.stream(step.stream):
+        kv.seed(0, pre, real)
+      if model is target:
+        logits = model._logits(pre["prog"].read_output("hid")[real - 1])
+      torch.cuda.synchronize(dev)
+    from . import kernels
+    first, _ = kernels.sample(torch.from_numpy(np.ascontiguousarray(logits, np.float32)).to(dev)[None],
+                              torch.from_numpy(rng.random(1, np.float32)).to(dev), temperature, top_k, top_p, min_p)
+    cur = int(first[0])
+    out, n_steps, n_accept = [cur], 0, 0
+    if on_token is not None and cur not in eos:
+      on_token(cur)
+    slot, grow = (torch.tensor([v], dtype=torch.int32, device=dev) for v in (0, T))
+    path_host = np.zeros((1, depth + 1), np.int32)
+    while len(out) < max_new_tokens and out[-1] not in eos:
+      with torch.cuda.stream(small.stream):
+        # level by level: the draft runs the nodes that it has, the best tokens after the last level's are the next
+        kvd.reserve(slot, grow)
+        small.tok[0, 0] = cur
+        lo, hi = 0, 1
+        for b in branches:
+          small.nodes.fill_(hi)
+          small.run()
+          best = small.logits[0, lo:hi].topk(int(b), dim=1).indices
+          lo, hi = hi, hi + best.numel()
+          small.tok[0, lo:hi] = best.reshape(-1).to(torch.int32)
+      with torch.cuda.stream(big.stream):
+        big.stream.wait_stream(small.stream)
+        kvt.reserve(slot, grow)
+        big.tok.copy_(small.tok)
+        big.u.copy_(torch.from_numpy(rng.random((1, T), np.float32)))
+        big.run()
+        toks, drawn = torch.stack((big.tok[0], big.out[0])).tolist()
+      n_steps += 1
+      path = [0]
+      while True:
+        nxt = next((c for c in children[path[-1]] if toks[c] == drawn[path[-1]]), None)
+        if nxt is None:
+          break
+        path.append(nxt)
+      n_accept += len(path) - 1
+      path_host[0, :len(path)] = path
+      with torch.cuda.stream(small.stream):
+        if len(path) == depth + 1:                           # a leaf: its row is not in the draft's cache yet
+          small.nodes.fill_(T)
+          small.run()
+        kvd.compact(slot, torch.from_numpy(path_host).to(dev), [len(path)])
+      with torch.cuda.stream(big.stream):
+        kvt.compact(slot, torch.from_numpy(path_host).to(dev), [len(path)])
+      for t in (drawn[p] for p in path):
+        out.append(t)
+        if t in eos:
+          break
+        if on_token is not None:
+          on_token(t)
+        if len(out) >= max_new_tokens:
+          break
+      cur = out[-1]
+    small.check()
+    big.check()
+  finally:
+    big.release()
+    if small is not None:
+      small.release()
+  if stats is not None:
+    stats.update(verify_steps=n_steps, accepted=n_accept)
+  return out
