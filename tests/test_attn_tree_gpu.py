@@ -298,3 +298,23 @@ def test_matches_the_decode_step():
     assert torch.equal(kc, k2) and torch.equal(vc, v2)
     # both within 2^-10 of the weighted |v| (at most 3 here) of the formula
     assert (got.float() - want.float()).abs().max() < 2 * 2.0 ** -10 * 3
+
+
+@pytest.mark.parametrize("B,T,H,KV,dh,lens,page", [(2, 1, 8, 2, 128, [700, 0], 64), (3, 33, 8, 2, 64, [129, 1000, 5], 16),
+                                                   (1, 70, 4, 1, 128, [3000], 64), (2, 5, 4, 2, 32, [40, 100], 8)])
+def test_workspace_may_hold_anything(B, T, H, KV, dh, lens, page):
+  """A workspace full of NaN, and one that another size has used before."""
+  from aneforge_b200 import kernels as K
+  outs = []
+  for fill in (0, 255, None):
+    scratch = K.attn_tree_scratch(B, T, H, KV, dh)
+    if fill is not None:
+      scratch.fill_(fill)
+    else:
+      scratch = K.attn_tree_scratch(4, 64, H, KV, dh) if T < 64 else K.attn_tree_scratch(B, 2 * T, H, KV, dh)
+      big = setup(4, 17, H, KV, dh, [900, 64, 0, 333], page, seed=9)
+      call(big, H, KV, dh, 0.1, scratch=scratch)
+    d = setup(B, T, H, KV, dh, lens, page, seed=3)
+    outs.append(call(d, H, KV, dh, 0.1, scratch=scratch))
+  assert torch.isfinite(outs[0]).all()
+  assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])

@@ -230,3 +230,9 @@ def test_agrees_with_the_host_sampler():
     np.random.seed(r)
     host = sample_token(l[r], **kw)
     assert run(torch.tensor(l[r:r + 1]).cuda(), [u], **kw)[0][0] == host
+
+
+@pytest.mark.parametrize("V,dtype", [(393217, torch.float32), (500001, torch.bfloat16)])
+def test_rows_longer_than_a_clusters_registers(V, dtype):
+  l = np.stack([rows(1, V, 40 + i, 3.0)[0] for i in range(4)])
+  check(l, [(1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (1.0, 0, 0.6, 0.0), (0.9, 1000, 0.8, 0.02)], seed=4, dtype=dtype)
