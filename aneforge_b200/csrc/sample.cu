@@ -18,11 +18,7 @@ namespace af {
 
 typedef unsigned long long u64;
 
-namespace smp {
-constexpr int THREADS = 1024;
-}
-
-AF_DEV float as_logit(float l) { return l != l ? -INFINITY : l + 0.f; }
+AF_DEV float as_logit(float l) { return fmaxf(l, -INFINITY) + 0.f; }       // the number, of a NaN and a number
 
 template <class T> AF_DEV float load_logit(const void* row, int i);
 template <> AF_DEV float load_logit<float>(const void* row, int i) { return as_logit(static_cast<const float*>(row)[i]); }
@@ -46,156 +42,6 @@ struct RowScale {
   AF_DEV float e(float l) const { return expf(below(l)); }
   AF_DEV u64 w(float l) const { return (u64)(e(l) * 1099511627776.f); }
 };
-
-template <class T>
-AF_DEV T block_sum(T v, T* buf) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T s = 0;
-  for (int k = 0; k < smp::THREADS / 32; ++k) s += buf[k];
-  return s;
-}
-
-// ---- rows too long for a cluster's registers: one block per row, the row read again for each step
-template <class T>
-__global__ void __launch_bounds__(smp::THREADS) sample_long_kernel(SampleArgs a) {
-  __shared__ u64 sum_s[32];
-  __shared__ u64 hist[256];
-  __shared__ u64 best_s;
-  __shared__ u64 pick_s[4];
-  const int r = blockIdx.x, V = a.V, tid = threadIdx.x;
-  const char* row = static_cast<const char*>(a.logits) + (size_t)r * a.ld * sizeof(T);
-  const float temp = a.temperature ? a.temperature[r] : a.temperature_s;
-  const int top_k = a.top_k ? a.top_k[r] : a.top_k_s;
-  const float top_p = a.top_p ? a.top_p[r] : a.top_p_s;
-  const float min_p = fminf(a.min_p ? a.min_p[r] : a.min_p_s, 1.f);
-  // the first largest logit: the greatest (key, ~index)
-  u64 best = 0;
-  for (int i = tid; i < V; i += smp::THREADS) {
-    const u64 k = (u64)key_of(load_logit<T>(row, i)) << 32 | (uint32_t)~i;
-    best = k > best ? k : best;
-  }
-  if (tid == 0) best_s = 0;
-  __syncthreads();
-  atomicMax(&best_s, best);
-  __syncthreads();
-  best = best_s;
-  const int first = (int)~(uint32_t)best;
-  RowScale sc;
-  sc.lmax = load_logit<T>(row, first);
-  sc.temp = temp > 0.f ? temp : 1.f;
-  sc.zmax = __fdiv_rn(sc.lmax, sc.temp);
-  if (sc.lmax == -INFINITY || !(temp > 0.f)) {
-    if (tid == 0) {
-      const bool none = sc.lmax == -INFINITY;
-      a.tok[r] = none ? -1 : first;
-      if (a.logp) a.logp[r] = none ? -INFINITY : 0.f;
-    }
-    return;
-  }
-  // top-k: the k-th largest key, byte by byte
-  uint32_t kth = 0;
-  if (top_k > 0 && top_k < V) {
-    u64 left = top_k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += smp::THREADS) {
-        const uint32_t k = key_of(load_logit<T>(row, i));
-        if (shift == 24 || (k >> (shift + 8)) == (kth >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1ull);
-      }
-      __syncthreads();
-      int d = 255;
-      for (; d > 0 && left > hist[d]; --d) left -= hist[d];
-      kth |= (uint32_t)d << shift;
-    }
-  }
-  // top-p: the key that the limit falls into, and how much of it is left for the ties
-  uint32_t pth = 0;
-  int pidx = V;
-  if (top_p > 0.f && top_p < 1.f) {
-    u64 total = 0;
-    for (int i = tid; i < V; i += smp::THREADS) {
-      const float l = load_logit<T>(row, i);
-      if (key_of(l) >= kth) total += sc.w(l);
-    }
-    total = block_sum(total, sum_s);
-    u64 left = (u64)ceil((double)top_p * (double)total);
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += smp::THREADS) {
-        const float l = load_logit<T>(row, i);
-        const uint32_t k = key_of(l);
-        if (k >= kth && (shift == 24 || (k >> (shift + 8)) == (pth >> (shift + 8))))
-          atomicAdd(&hist[(k >> shift) & 255], sc.w(l));
-      }
-      __syncthreads();
-      int d = 255;
-      for (; d > 0 && left > hist[d]; --d) left -= hist[d];
-      pth |= (uint32_t)d << shift;
-    }
-    // of the tokens with exactly this key, the first ceil(left / weight) in index order
-    const u64 w1 = sc.w(__uint_as_float(pth & 0x80000000u ? pth & 0x7fffffffu : ~pth));
-    const u64 ties = w1 ? (left + w1 - 1) / w1 : 0;
-    u64 seen = 0;
-    for (int base = 0; base < V; base += smp::THREADS) {
-      const int i = base + tid;
-      const bool tie = i < V && key_of(load_logit<T>(row, i)) == pth;
-      const unsigned ball = __ballot_sync(0xffffffffu, tie);
-      __syncthreads();
-      if ((tid & 31) == 0) sum_s[tid >> 5] = __popc(ball);
-      __syncthreads();
-      u64 before = seen + __popc(ball & ((1u << (tid & 31)) - 1));
-      for (int k = 0; k < 32; ++k) {
-        if (k < (tid >> 5)) before += sum_s[k];
-        seen += sum_s[k];
-      }
-      if (tie && before + 1 == ties) pick_s[0] = i;
-      if (seen >= ties) break;
-    }
-    __syncthreads();
-    pidx = (int)pick_s[0];
-  }
-  // kept weights in index order: every thread a run of consecutive tokens
-  const int per = (V + smp::THREADS - 1) / smp::THREADS, i0 = tid * per, i1 = min(V, i0 + per);
-  auto kept = [&](int i) -> u64 {
-    const float l = load_logit<T>(row, i);
-    const uint32_t k = key_of(l);
-    if (k < kth || k < pth || (k == pth && i > pidx) || !(sc.e(l) >= min_p)) return 0;
-    return sc.w(l);
-  };
-  u64 mine = 0;
-  for (int i = i0; i < i1; ++i) mine += kept(i);
-  const u64 total = block_sum(mine, sum_s);
-  u64 target = (u64)fmax(floor((double)a.u[r] * (double)total), 0.0);
-  target = target < total ? target : total - 1;
-  u64 x = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, x, o);
-    if ((tid & 31) >= o) x += y;
-  }
-  u64 before = x - mine;
-  for (int k = 0; k < (tid >> 5); ++k) before += sum_s[k];
-  if (before <= target && target < before + mine) {
-    int i = i0;
-    for (; i < i1; ++i) {
-      before += kept(i);
-      if (before > target) break;
-    }
-    a.tok[r] = i;
-    if (a.logp) {
-      const float l = load_logit<T>(row, i);
-      a.logp[r] = sc.below(l) - logf((float)total / 1099511627776.f);
-    }
-  }
-}
 
 // ---- rows held in registers: a cluster of blocks per row
 //
@@ -226,7 +72,7 @@ struct SampleShared {
   uint32_t count[smr::MAXC];                   // listed tokens,
   u64 total[smr::MAXC];                        // weight
   u64 kept[smr::MAXC];                         // and kept weight
-  uint32_t hist[smr::BINS];
+  alignas(16) uint32_t hist[smr::BINS];
   uint32_t ecnt[smr::EBINS], elow[smr::EBINS]; // tokens, and the sum of their weights' lower bits
   u64 radix[2][256];
   u64 sums[smr::WARPS * 12];                   // kept weight (or ties) of a (vector, warp)
@@ -239,8 +85,22 @@ struct SampleShared {
   u64 total_w;
   u64 need;                                    // weight that the nucleus takes from its last bin
   int where, bin;
+  alignas(16) float edge[3][8];                // one block per row: the first and last vector if not whole; none
 };
 
+// 16 bytes where `yes`; no branch, on which the loads after it would wait
+AF_DEV uint4 ldg_if(bool yes, const void* p) {
+  uint4 r;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+               "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "r"((uint32_t)yes));
+  return r;
+}
+AF_DEV float ex2(float x) {                    // for estimates
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 AF_DEV float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 template <class P> AF_DEV P* peer(P* p, int rank) {
@@ -506,6 +366,10 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   };
   load_row();
   auto index_of = [&](int j) { return (rank * per + (j / VE) * THREADS + tid) * VE - skip + j % VE; };
+  auto in_row = [&](int j) {
+    const int idx = index_of(j);
+    return idx >= 0 && idx < V && (j / VE) * THREADS + tid < per;
+  };
   const bool use_k = top_k > 0 && top_k < V, use_p = top_p > 0.f && top_p < 1.f, use_m = min_p > 0.f;
   if (use_p && !use_k)                         // while the row is on its way
     for (int k = tid; k < EBINS; k += THREADS) sh.ecnt[k] = sh.elow[k] = 0;
@@ -584,7 +448,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
       for (int j = 0; j < E; ++j) add(v[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) add(sc.e(v[j]));
+      for (int j = 0; j < E; ++j) add(in_row(j) ? sc.e(v[j]) : 0.f);       // -inf may be the largest z
     }
     hi = __reduce_add_sync(0xffffffffu, hi);
     lo = __reduce_add_sync(0xffffffffu, lo);
@@ -689,10 +553,8 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int idx = index_of(j);
-        if (idx >= 0 && idx < V && (j / VE) * THREADS + tid < per) f(v[j], idx);
-      }
+      for (int j = 0; j < E; ++j)
+        if (in_row(j)) f(v[j], index_of(j));
     }
   };
   // the largest key such that the weights (or counts) of the keys over it stay under `want`; `left` gets
@@ -754,7 +616,8 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
         for (int k = 0; k < VE; ++k) {
           const int idx = index_of(i * VE + k);
           uint32_t h, l;
-          weight_parts(f(v[i * VE + k], idx), h, l);      // past the row's end: -inf, or e = 0
+          const float e = f(v[i * VE + k], idx);          // past the row's end: of -inf
+          weight_parts(far && !in_row(i * VE + k) ? 0.f : e, h, l);
           hi += h;
           lo += l;
         }
@@ -1010,6 +873,600 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   finish(at, sum);
 }
 
+// ---- many rows, and rows too long for a cluster's registers: one block per row, which reads the row again
+// for each step (from L2, mostly). A step has no barrier between its loads, so the loads of a row flow without
+// a pause, where a cluster waits for its peers several times a row. Steps: the maximum, with an estimate of
+// the total weight; top-k: the k-th largest of the threads' maxima bounds the k-th largest logit from below, so
+// that few more than k tokens are listed; nucleus: the bins of e as in a cluster; then the kept weight of each
+// run ("cell") of the row, and the one cell that the target falls into. What does not fit its list or bin goes
+// the general way: a radix search, a pass over the row for each 8 bits.
+namespace smw {
+constexpr int CELLS = 1024;                    // runs of 32 * K vectors
+}
+
+template <class T>
+__global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs a) {
+  using namespace smr;
+  constexpr int VE = 16 / (int)sizeof(T), U = 4, U1 = 32 / VE;         // U, U1: vectors of a thread on their way
+  extern __shared__ __align__(16) unsigned char sample_raw[];
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
+  u64* cells = reinterpret_cast<u64*>(sh.ecnt);              // after the bins
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = blockIdx.x, V = a.V;
+  const float temp = a.temperature ? __ldg(a.temperature + r) : a.temperature_s;
+  const int top_k = a.top_k ? __ldg(a.top_k + r) : a.top_k_s;
+  const float top_p = a.top_p ? __ldg(a.top_p + r) : a.top_p_s;
+  const float min_p = fminf(a.min_p ? __ldg(a.min_p + r) : a.min_p_s, 1.f);
+  const bool use_k = top_k > 0 && top_k < V, use_p = top_p > 0.f && top_p < 1.f;
+  const float u = __ldg(a.u + r);
+  if (tid == 0) { sh.nlocal = 0; sh.kloc = 0; sh.floc = 0xffffffffu; sh.in_bin = 0; sh.bin = -1; sh.first[0] = 0xffffffffu; }
+  const T* row = static_cast<const T*>(a.logits) + (size_t)r * a.ld;
+  const int skip = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  const int nvec = (skip + V + VE - 1) / VE;
+  // vector vi as logits (-inf outside the row)
+  const int full0 = skip ? 1 : 0, nfull = max((skip + V) / VE - full0, 0);
+  auto is_full = [&](int vi) { return (unsigned)(vi - full0) < (unsigned)nfull; };
+  auto unpack = [&](bool full, const uint4& x, int vi, float (&l)[VE]) {
+    if (full) {
+      const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+      for (int k = 0; k < VE; ++k) l[k] = load_logit<T>(e, k);
+    } else {
+      const float* e = sh.edge[vi == 0 ? 0 : vi == nvec - 1 ? 1 : 2];
+#pragma unroll
+      for (int k = 0; k < VE; ++k) l[k] = e[k];
+    }
+  };
+  if (tid < 3 * 8) {
+    const int i = (tid < 8 ? 0 : nvec - 1) * VE - skip + tid % 8;
+    sh.edge[tid / 8][tid % 8] = tid < 16 && tid % 8 < VE && i >= 0 && i < V ? load_logit<T>(row, i) : -INFINITY;
+  }
+  __syncthreads();
+  auto fetch = [&](int vi) { return ldg_if(is_full(vi), row + vi * VE - skip); };
+  // f(logits, vector) for the n vectors from v0 in steps of `step`, U loads on their way together. The loop is not
+  // unrolled: with U bodies a step the warps waited for instructions (96 rows of 50257, min-p: 25.7 us, 18.3 us so)
+  auto run = [&](int v0, int n, int step, auto f) {
+    uint4 x[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) x[j] = fetch(j < n ? v0 + j * step : nvec);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const uint4 y = x[0];
+#pragma unroll
+      for (int j = 0; j + 1 < U; ++j) x[j] = x[j + 1];
+      const int vi = v0 + i * step;
+      x[U - 1] = fetch(i + U < n ? vi + U * step : nvec);
+      float l[VE];
+      unpack(is_full(vi), y, vi, l);
+      f(l, vi);
+    }
+  };
+  auto walk = [&](auto f) { run(tid, (nvec - tid + THREADS - 1) / THREADS, THREADS, f); };
+  // ---- the maximum, and about how much all tokens weigh
+  float m = -INFINITY, s = 0.f;
+  int at = 0;                                  // the first vector that holds m
+  const bool estimate = use_p && !use_k && temp > 0.f;
+  const float c2 = 1.4426950408889634f / temp;
+  auto first_pass = [&](const float (&l)[VE], int vi) {
+    float x = l[0];
+#pragma unroll
+    for (int k = 1; k < VE; ++k) x = fmaxf(x, l[k]);
+    if (x > m) {
+      if (estimate) s = m == -INFINITY ? 0.f : s * exp2f((m - x) * c2);
+      m = x;
+      at = vi;
+    }
+    if (estimate && m != -INFINITY)
+#pragma unroll
+      for (int k = 0; k < VE; ++k) s += ex2((l[k] - m) * c2);
+  };
+  for (int base = tid; base < nvec; base += U1 * THREADS) {       // the row comes from memory: more loads on their way
+    uint4 x[U1];
+#pragma unroll
+    for (int j = 0; j < U1; ++j) x[j] = fetch(base + j * THREADS);
+#pragma unroll
+    for (int j = 0; j < U1; ++j) {
+      const int vi = base + j * THREADS;
+      float l[VE];
+      unpack(is_full(vi), x[j], vi, l);
+      first_pass(l, vi);
+    }
+  }
+  const uint32_t mine_key = key_of(m);
+  uint32_t kmax = __reduce_max_sync(0xffffffffu, mine_key);
+  __syncthreads();
+  if (lane == 0) atomicMax(&sh.kloc, kmax);
+  __syncthreads();
+  kmax = sh.kloc;
+  RowScale sc;
+  sc.lmax = logit_of(kmax);
+  sc.temp = temp > 0.f ? temp : 1.f;
+  sc.zmax = __fdiv_rn(sc.lmax, sc.temp);
+  if (sc.lmax == -INFINITY) {
+    if (tid == 0) {
+      a.tok[r] = -1;
+      if (a.logp) a.logp[r] = -INFINITY;
+    }
+    return;
+  }
+  if (!(temp > 0.f)) {
+    if (mine_key == kmax) atomicMin(&sh.first[0], (uint32_t)at);
+    __syncthreads();
+    if (tid == 0) {
+      const int vi = (int)sh.first[0];
+      int i = max(vi * VE - skip, 0);
+      while (load_logit<T>(row, i) != sc.lmax) ++i;          // it is in this vector
+      a.tok[r] = i;
+      if (a.logp) a.logp[r] = 0.f;
+    }
+    return;
+  }
+  const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
+  auto e_of = [&](float l) {
+    if (far) return sc.e(l);
+    return expf((sc.temp == 1.f ? l : __fdiv_rn(l, sc.temp)) - sc.zmax);
+  };
+  // of a vector: the branches once, the exponentials side by side
+  auto es_of = [&](const float (&l)[VE], float (&e)[VE]) {
+    if (far) {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) e[k] = sc.e(l[k]);
+      return;
+    }
+    if (sc.temp == 1.f) {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) e[k] = l[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) e[k] = __fdiv_rn(l[k], sc.temp);
+    }
+#pragma unroll
+    for (int k = 0; k < VE; ++k) e[k] = expf(e[k] - sc.zmax);
+  };
+  auto parts_of = [&](const float (&e)[VE], uint32_t& hi, uint32_t& lo) {
+    hi = 0u - VE * 0x41000000u;
+    lo = 0u - VE * 0x37000000u;
+#pragma unroll
+    for (int k = 0; k < VE; ++k) {
+      const float t = __fadd_rd(e[k], 8.f);
+      hi += __float_as_uint(t);
+      lo += __float_as_uint(__fadd_rd(e[k] - (t - 8.f), 7.62939453125e-06f));
+    }
+  };
+  auto w_of = [&](float e) { return (u64)(e * 1099511627776.f); };
+  auto order = [&](float l, int idx) { return (u64)key_of(l) << 32 | (uint32_t)~idx; };
+  // ---- sums of f(logit, index) over the cells, and the token of a cell that passes a target
+  const int K = max(8, (nvec + 32 * smw::CELLS - 1) / (32 * smw::CELLS)), ncell = (nvec + 32 * K - 1) / (32 * K);
+  auto warp_sum64 = [&](u64 w) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    return w;
+  };
+  // (f(logits, e, vector) gives e, or 0 for a token that is not kept)
+  auto group = [&](auto f, int v0) -> u64 {                  // one lane's part of 32 vectors from v0
+    const int vi = v0 + lane;
+    uint32_t hi = 0, lo = 0;
+    if (vi < nvec) {
+      const bool full = is_full(vi);
+      const uint4 x = fetch(vi);
+      float l[VE], e[VE];
+      unpack(full, x, vi, l);
+      f(l, e, vi);
+      parts_of(e, hi, lo);
+    }
+    return ((u64)hi << 20) + lo;
+  };
+  auto cell_rows = [&](int c) { return min(K, (nvec - c * K * 32 + 31) / 32); };      // runs of 32 vectors
+  auto sum_cells = [&](auto f) {
+    __syncthreads();
+    for (int c = warp; c < ncell; c += WARPS) {
+      u64 w = 0;
+      run(c * K * 32 + lane, cell_rows(c), 32, [&](const float (&l)[VE], int vi) {
+        float e[VE];
+        uint32_t hi, lo;
+        f(l, e, vi);
+        parts_of(e, hi, lo);
+        w += ((u64)hi << 20) + lo;
+      });
+      w = warp_sum64(w);
+      if (lane == 0) cells[c] = w;
+    }
+    __syncthreads();
+  };
+  // the same where only tokens from l_lo on count: those of 32 vectors are queued, and a full warp of them is
+  // looked at together. f(logit, index, e) gives e or 0
+  auto sum_above = [&](float l_lo, auto f) {
+    static_assert(LIST + 64 * WARPS <= LOCAL, "the warps' queues lie after the list");
+    u64* queue = sh.local + LIST + 64 * warp;
+    __syncthreads();
+    for (int c = warp; c < ncell; c += WARPS) {
+      u64 w = 0;
+      int n = 0;
+      auto flush = [&](bool mine) {
+        __syncwarp();
+        uint32_t h = 0, g = 0;
+        if (mine) {
+          const u64 x = queue[lane];
+          const float l = logit_of((uint32_t)(x >> 32));
+          weight_parts(f(l, (int)~(uint32_t)x, e_of(l)), h, g);
+        }
+        w += ((u64)h << 20) + g;
+      };
+      run(c * K * 32 + lane, cell_rows(c), 32, [&](const float (&l)[VE], int vi) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          const bool yes = l[k] >= l_lo;
+          const unsigned who = __ballot_sync(0xffffffffu, yes);
+          if (!who) continue;
+          if (yes) queue[n + __popc(who & ((1u << lane) - 1))] = order(l[k], vi * VE - skip + k);
+          n += __popc(who);
+          if (n >= 32) {
+            flush(true);
+            n -= 32;
+            const u64 x = queue[32 + lane];
+            __syncwarp();
+            queue[lane] = x;
+          }
+        }
+      });
+      flush(lane < n);
+      w = warp_sum64(w);
+      if (lane == 0) cells[c] = w;
+    }
+    __syncthreads();
+  };
+  auto total_cells = [&](u64& before) {        // all cells' sum; this thread's two cells begin after `before`
+    u64 all;
+    const u64 w = (2 * tid < ncell ? cells[2 * tid] : 0) + (2 * tid + 1 < ncell ? cells[2 * tid + 1] : 0);
+    before = scan_excl(w, sh.scan, all);
+    return all;
+  };
+  auto locate = [&](auto f, u64 before, u64 target) -> int {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c = 2 * tid + j;
+      const u64 w = c < ncell ? cells[c] : 0;
+      if (before <= target && target < before + w) {
+        sh.where = c;
+        sh.pick = target - before;
+      }
+      before += w;
+    }
+    __syncthreads();
+    const int c = sh.where;
+    for (int k = warp; k < K; k += WARPS) {
+      const u64 w = warp_sum64(group(f, (c * K + k) * 32));
+      if (lane == 0) sh.radix[0][k] = w;       // K <= 128: V <= 2^24
+    }
+    __syncthreads();
+    if (warp == 0) {
+      u64 in = sh.pick;
+      int k = 0;
+      while (k + 1 < K && in >= sh.radix[0][k]) in -= sh.radix[0][k++];
+      const int v0 = (c * K + k) * 32;
+      const u64 w = group(f, v0);
+      u64 x = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      u64 b = x - w;
+      if (b <= in && in < x) {
+        const int vi = v0 + lane;
+        float l[VE], e[VE];
+        unpack(is_full(vi), fetch(vi), vi, l);
+        f(l, e, vi);
+        int i = 0;
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          b += w_of(e[k]);
+          if (b <= in) i = k + 1;
+        }
+        sh.where = vi * VE - skip + i;
+      }
+    }
+    __syncthreads();
+    return sh.where;
+  };
+  // kept: l over l_last, or l_last itself up to index i_last, and e >= min_p
+  float l_last = -INFINITY;
+  int i_last = V;
+  auto inside = [&](int idx) { return idx >= 0 && idx < V; };
+  bool narrow = far || use_k || use_p || min_p > 0.f;        // else every token is kept
+  auto kept = [&](const float (&l)[VE], float (&e)[VE], int vi) {
+    es_of(l, e);
+    if (!narrow) return;
+#pragma unroll
+    for (int k = 0; k < VE; ++k) {
+      const int idx = vi * VE - skip + k;
+      const bool yes = (l[k] > l_last || (l[k] == l_last && idx <= i_last)) && e[k] >= min_p && (!far || inside(idx));
+      e[k] = yes ? e[k] : 0.f;
+    }
+  };
+  auto finish = [&](u64 before, u64 sum) {
+    const int i = locate(kept, before, draw_target(u, sum));
+    if (tid == 0) {
+      a.tok[r] = i;
+      if (a.logp) a.logp[r] = logp_of(sc, load_logit<T>(row, i), sum);
+    }
+  };
+  u64 before;
+  bool listed = false;                         // every token that may be kept is in `local`
+  uint32_t n_list = 0;
+  if (use_k && (top_k <= THREADS * 3 / 4 || !far)) {
+    float least = -INFINITY, cut = INFINITY;
+    const float scale = 8.f / sc.temp;
+    if (top_k <= THREADS * 3 / 4) {
+      // at least k tokens are as large as the k-th largest of the threads' maxima
+      uint32_t* keys = sh.hist;
+      static_assert(THREADS <= BINS + EBINS, "the threads' maxima lie over the histogram and the bins");
+      keys[tid] = mine_key;
+      __syncthreads();
+      int over = 0;
+      for (int k = 0; k < THREADS; k += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(keys + k);
+        over += (x.x > mine_key) + (x.y > mine_key) + (x.z > mine_key) + (x.w > mine_key);
+      }
+      if (over < top_k) atomicMin(&sh.floc, mine_key);
+      __syncthreads();
+      least = logit_of(sh.floc);
+    } else {
+      // the eighth of a nat that the k-th lies in
+      if (tid < BINS) sh.hist[tid] = 0;
+      if (tid == 0) sh.where = BINS - 1;
+      __syncthreads();
+      walk([&](const float (&l)[VE], int) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          const float d = (sc.lmax - l[k]) * scale;
+          if (d < (float)BINS) atomicAdd(&sh.hist[(int)d], 1u);
+        }
+      });
+      u64 all;
+      __syncthreads();
+      const u64 n = tid < BINS ? sh.hist[tid] : 0;
+      before = scan_excl(n, sh.scan, all);
+      if (before < (u64)top_k && (u64)top_k <= before + n) sh.where = tid;
+      __syncthreads();
+      cut = (float)(sh.where + 1);             // fewer than k weigh anything: all of those
+    }
+    walk([&](const float (&l)[VE], int vi) {
+      float most = l[0];
+#pragma unroll
+      for (int k = 1; k < VE; ++k) most = fmaxf(most, l[k]);
+      if (most < least) return;
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        const int i = vi * VE - skip + k;
+        if (l[k] >= least && (cut == INFINITY || (sc.lmax - l[k]) * scale < cut) && inside(i)) {
+          const uint32_t n = atomicAdd(&sh.nlocal, 1u);
+          if (n < (uint32_t)LOCAL) sh.local[n] = order(l[k], i);
+        }
+      }
+    });
+    __syncthreads();
+    n_list = sh.nlocal;
+    if (n_list <= (uint32_t)LIST) {
+      few_tokens(a, sh, sc, r, (int)n_list, top_k, use_p, top_p, min_p, u, 0);
+      return;
+    }
+    listed = n_list <= (uint32_t)LOCAL;
+  }
+  // a logit under this one has a smaller e (logf, product and quotient are off by far less than the margin)
+  auto under = [&](float e) { return sc.lmax + sc.temp * (logf(e) - 1e-3f) - 1e-5f * fabsf(sc.lmax); };
+  u64 total = 0, limit = 0;
+  if (estimate && !far) {
+    // ---- nucleus: the weights by the upper bits of e
+    s = m == -INFINITY ? 0.f : s * exp2f((m - sc.lmax) * c2);
+    s = warp_sum(s);
+    __syncthreads();
+    if (lane == 0) sh.scan[warp] = __float_as_uint(s);
+    __syncthreads();
+    s = 0.f;
+    for (int k = 0; k < WARPS; ++k) s += __uint_as_float((uint32_t)sh.scan[k]);
+    __syncthreads();
+    // tokens so light that all V of them together would not reach past the nucleus need no bin
+    const float sure = fmaxf((1.f - top_p) * 0.99f * s / (float)V, 6.0e-8f);
+    // most likely all under `light` do not either: of every 16th vector (one of 16 in turn) the weights, by
+    // eighths of a nat, say under which the tail weighs 0.7 of what the nucleus leaves (a few heavy tokens, which
+    // the choice may have missed, are not taken for a tail: 64 of those chosen have to be over `light`)
+    float light = sure;
+    {
+      const float scale = 8.f / sc.temp;
+      if (tid < BINS) sh.hist[tid] = 0;
+      if (tid == 0) sh.where = BINS;
+      __syncthreads();
+      for (int j = tid; j < nvec / 16; j += THREADS) {
+        const int vi = 16 * j + (int)((uint32_t)j * 0x9e3779b1u >> 28);
+        float l[VE];
+        unpack(is_full(vi), fetch(vi), vi, l);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          const float d = (sc.lmax - l[k]) * scale;
+          if (d < (float)BINS) atomicAdd(&sh.hist[(int)d], 1u);
+        }
+      }
+      __syncthreads();
+      const float unit = 16.f * 1073741824.f;
+      const u64 n = tid < BINS ? (u64)((float)sh.hist[tid] * expf(-0.125f * (float)tid - 0.0625f) * unit) : 0;
+      u64 all, many;
+      const u64 over = scan_excl(tid < BINS ? sh.hist[tid] : 0u, sh.scan, many);
+      before = scan_excl(n, sh.scan, all);
+      if (tid < BINS && over >= 64 && (float)(all - before) <= 0.7f * (1.f - top_p) * s * 1073741824.f) atomicMin(&sh.where, tid);
+      __syncthreads();
+      light = fmaxf(sure, expf(-0.125f * (float)sh.where));
+    }
+    u64 w;
+    while (true) {
+      for (int k = tid; k < EBINS; k += THREADS) sh.ecnt[k] = sh.elow[k] = 0;
+      __syncthreads();
+      w = 0;
+      walk([&](const float (&l)[VE], int) {
+        float e[VE];
+        uint32_t hi, lo;
+        es_of(l, e);
+        parts_of(e, hi, lo);
+        w += ((u64)hi << 20) + lo;
+        float most = e[0];
+#pragma unroll
+        for (int k = 1; k < VE; ++k) most = fmaxf(most, e[k]);
+        if (most >= light)
+#pragma unroll
+          for (int k = 0; k < VE; ++k)
+            if (e[k] >= light) {
+              const uint32_t b = __float_as_uint(e[k]);
+              const int bin = (int)((0x3f800000u >> EBITS) - (b >> EBITS)), drop = 110 - (int)(b >> 23);
+              atomicAdd(&sh.ecnt[bin], 1u);
+              atomicAdd(&sh.elow[bin], (b & ((1u << EBITS) - 1)) >> max(drop, 0));
+            }
+      });
+      u64 none;
+      scan_excl(w, sh.scan, total);
+      limit = (u64)ceil((double)top_p * (double)total);
+      const int run = (EBINS + THREADS - 1) / THREADS, b0 = tid * run, b1 = min(b0 + run, EBINS);
+      // (the sum of 2^16 lower bits fits 32; past so many tokens in a bin: the general way)
+      auto weight = [&](int b) -> u64 {
+        const uint32_t bits = 0x3f800000u - ((uint32_t)b << EBITS);
+        const int up = 17 + (int)(bits >> 23) - 127;
+        const u64 mant = (bits & 0x7fffffu) | 0x800000u, cnt = sh.ecnt[b], low = sh.elow[b];
+        return up >= 0 ? (cnt * mant + low) << up : cnt * (mant >> -up) + low;
+      };
+      w = 0;
+      bool full = false;
+      for (int b = b0; b < b1; ++b) {
+        w += weight(b);
+        full |= sh.ecnt[b] > 65536u;
+      }
+      full = __syncthreads_or(full);
+      before = scan_excl(w, sh.scan, none);
+      if (!full && before < limit && limit <= before + w)
+        for (int b = b0; b < b1; ++b) {
+          const u64 x = weight(b);
+          if (before < limit && limit <= before + x) {
+            sh.bin = b;
+            sh.need = limit - before;
+          }
+          before += x;
+        }
+      __syncthreads();
+      if (sh.bin >= 0 || light == sure) break;               // the same answer in all threads
+      light = sure;
+      __syncthreads();
+    }
+    if (sh.bin >= 0) {
+      const uint32_t q = (0x3f800000u >> EBITS) - (uint32_t)sh.bin;
+      const float lo_e = __uint_as_float(q << EBITS);
+      sum_above(under(lo_e), [&](float l, int idx, float e) {
+        const uint32_t b = __float_as_uint(e) >> EBITS;
+        if (b == q) {
+          const uint32_t n = atomicAdd(&sh.in_bin, 1u);
+          if (n < (uint32_t)LIST) sh.local[n] = order(l, idx);
+        }
+        return b > q && e >= min_p ? e : 0.f;
+      });
+      const int n = (int)min(sh.in_bin, (uint32_t)LIST + 1);
+      if (n <= LIST) {
+        const u64 last = last_of(sh, sc, n, sh.need);
+        l_last = logit_of((uint32_t)(last >> 32));
+        i_last = (int)~(uint32_t)last;
+        for (int k = tid; k < n; k += THREADS) {
+          const u64 x = sh.local[k];
+          const float e = e_of(logit_of((uint32_t)(x >> 32)));
+          if (x >= last && e >= min_p) atomicAdd(&cells[((int)~(uint32_t)x + skip) / VE / (32 * K)], w_of(e));
+        }
+        __syncthreads();
+        const u64 sum = total_cells(before);
+        finish(before, sum);
+        return;
+      }
+      __syncthreads();
+    }
+  }
+  // ---- the general way, over the list or the row
+  auto each = [&](auto f) {
+    if (listed) {
+      for (uint32_t i = tid; i < n_list; i += THREADS) {
+        const u64 x = sh.local[i];
+        f(logit_of((uint32_t)(x >> 32)));
+      }
+    } else {
+      walk([&](const float (&l)[VE], int vi) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+          if (inside(vi * VE - skip + k)) f(l[k]);
+      });
+    }
+  };
+  // the largest key such that the weights (or counts) of the keys over it stay under `want`; `left` gets what
+  // is wanted of that key itself
+  uint32_t kth = 0;
+  auto search = [&](bool counts, u64 want, u64& left) -> uint32_t {
+    uint32_t key = 0;
+    left = want;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      __syncthreads();
+      if (tid < 256) sh.radix[0][tid] = 0;
+      if (tid == 0) { sh.where = 0; sh.pick = 0; }
+      __syncthreads();
+      each([&](float l) {
+        const uint32_t x = key_of(l);
+        if (x >= kth && (shift == 24 || (x >> (shift + 8)) == (key >> (shift + 8))))
+          atomicAdd(&sh.radix[0][(x >> shift) & 255], counts ? 1ull : w_of(e_of(l)));
+      });
+      __syncthreads();
+      const u64 n = tid < 256 ? sh.radix[0][255 - tid] : 0;
+      u64 all;
+      const u64 over = scan_excl(n, sh.scan, all);
+      if (over < left && left <= over + n) {
+        sh.where = 255 - tid;
+        sh.pick = over;
+      }
+      __syncthreads();
+      left -= sh.pick;
+      key |= (uint32_t)sh.where << shift;
+    }
+    return key;
+  };
+  u64 left;
+  if (use_k && (!listed || (uint32_t)top_k <= n_list)) {
+    kth = search(true, (u64)top_k, left);
+    l_last = logit_of(kth);
+  }
+  if (use_p) {
+    u64 w = 0;
+    each([&](float l) { if (key_of(l) >= kth) w += w_of(e_of(l)); });
+    scan_excl(w, sh.scan, total);
+    const uint32_t pth = search(false, (u64)ceil((double)top_p * (double)total), left);
+    // of the tokens with exactly this key the first ceil(left / weight) in index order are kept
+    const u64 w1 = w_of(e_of(logit_of(pth)));
+    const u64 ties = w1 ? (left + w1 - 1) / w1 : 1;
+    l_last = logit_of(pth);
+    auto tie = [&](const float (&l)[VE], float (&e)[VE], int vi) {       // 2^-40 each
+#pragma unroll
+      for (int k = 0; k < VE; ++k) e[k] = l[k] == l_last && inside(vi * VE - skip + k) ? 9.094947017729282e-13f : 0.f;
+    };
+    sum_cells(tie);
+    const u64 n = total_cells(before);
+    i_last = locate(tie, before, min(ties, n) - 1);
+  }
+  if (use_k || use_p || far || !(min_p > 0.f)) sum_cells(kept);
+  else sum_above(under(min_p), [&](float, int, float e) { return e >= min_p ? e : 0.f; });
+  const u64 sum = total_cells(before);
+  finish(before, sum);
+}
+
+template <class T>
+static cudaError_t launch_wide(const SampleArgs& a, cudaStream_t st) {
+  static PerDeviceOnce attrs;
+  const cudaError_t ae = attrs.run([] {
+    return cudaFuncSetAttribute(sample_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared));
+  });
+  if (ae != cudaSuccess) return ae;
+  sample_wide_kernel<T><<<a.R, smr::THREADS, sizeof(SampleShared), st>>>(a);
+  return cudaGetLastError();
+}
+
 template <class T, int NV>
 static cudaError_t launch_rows(const SampleArgs& a, int C, cudaStream_t st) {
   static PerDeviceOnce attrs;
@@ -1045,10 +1502,10 @@ static cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
                            ((long long)a.R * C * 2 <= sms && (nvec + C - 1) / C > smr::THREADS)))
     C <<= 1;
   const int NV = ((nvec + C - 1) / C + smr::THREADS - 1) / smr::THREADS;
-  if (NV > 48 / VE) {
-    sample_long_kernel<T><<<a.R, smp::THREADS, 0, st>>>(a);
-    return cudaGetLastError();
-  }
+  // one block per row from five rows for eight SMs on (B200, us, clusters / single blocks; 128256 fp32: 64 rows
+  // top-k 42 / 33, nucleus 66 / 101, min-p 31 / 34; 96 rows 61 / 33, 98 / 101, 45 / 34; 256 rows 168 / 71,
+  // 271 / 159, 125 / 66; 50257 fp16: 64 rows 21 / 18, 33 / 42, 16 / 18; 96 rows 34 / 18, 58 / 39, 25 / 18)
+  if (NV > 48 / VE || 8ll * a.R >= 5ll * sms) return launch_wide<T>(a, st);
   if (NV <= 8 / VE) return launch_rows<T, 8 / VE>(a, C, st);
   if (NV <= 16 / VE) return launch_rows<T, 16 / VE>(a, C, st);
   if (NV <= 32 / VE) return launch_rows<T, 32 / VE>(a, C, st);

@@ -236,3 +236,41 @@ def test_agrees_with_the_host_sampler():
 def test_rows_longer_than_a_clusters_registers(V, dtype):
   l = np.stack([rows(1, V, 40 + i, 3.0)[0] for i in range(4)])
   check(l, [(1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (1.0, 0, 0.6, 0.0), (0.9, 1000, 0.8, 0.02)], seed=4, dtype=dtype)
+
+
+@pytest.mark.parametrize("V,dtype", [(3, torch.float32), (700, torch.bfloat16), (5001, torch.float32), (50257, torch.float16),
+                                     (128256, torch.float32)])
+def test_many_rows_agree_with_few(V, dtype):
+  """Rows and settings of every kind alone and many times over: another split of the work, the same tokens."""
+  inf, nan = float("inf"), float("nan")
+  rng = np.random.default_rng(V)
+  l = np.stack([rows(1, V, 60 + i, 2.0 + i % 3)[0] for i in range(24)])
+  l[1] = -inf
+  l[2] = nan
+  l[3, V // 2:] = -inf
+  l[4, ::2] = nan
+  l[5, V // 3] = inf
+  l[6] = 0.25
+  l[7] = np.round(l[7])
+  l[8] = np.where(rng.random(V) < 0.5, -3.0, 1.0)
+  l[9] = -3.0e38
+  l[10, :] = -60.0
+  l[10, V - 1] = 10.0
+  l[11, [0, V - 1]] = inf
+  sets = [(1.0, 0, 1.0, 0.0), (0.7, 40, 0.9, 0.0), (1.0, 0, 0.95, 0.0), (0.0, 0, 1.0, 0.0), (1.3, 0, 1.0, 0.02),
+          (0.9, 1000, 0.99, 0.01), (1.0, 0, 0.3, 0.1), (1e-3, 0, 0.5, 0.0), (5.0, 400, 1.0, 0.0), (2.0, 0, 0.999999, 0.0),
+          (1.0, 3000, 0.5, 0.0), (1.0, 20, 1.0, 1.0)]
+  x = torch.tensor(l).to(dtype).cuda()
+  for shift in range(3):
+    pick = [sets[(r + 5 * shift) % len(sets)] for r in range(24)]
+    u = rng.random(24).astype(np.float32)
+
+    def go(reps):
+      col = lambda i, dt: torch.tensor([s[i] for s in pick], dtype=dt).cuda().repeat(reps)
+      return run(x.repeat(reps, 1), np.tile(u, reps), temperature=col(0, torch.float32), top_k=col(1, torch.int32),
+                 top_p=col(2, torch.float32), min_p=col(3, torch.float32))
+
+    tok, logp = go(1)
+    toks, logps = go(8)
+    assert toks.reshape(8, 24).tolist() == [tok.tolist()] * 8
+    np.testing.assert_allclose(logps.reshape(8, 24), np.tile(logp, (8, 1)), rtol=2.0 ** -20, atol=2.0 ** -20)
