@@ -54,6 +54,10 @@ struct RowScale {
 // A nucleus without top-k can hold a quarter of the vocabulary: the weights are summed by the upper bits
 // of e (exactly: a bin's tokens share an octave, so a count and the sum of the lower bits give their
 // weight), only the bin that the limit falls into is sorted, and the kept sums come from the registers.
+// Bound by latency: a row of 0.5 MB takes 0.1 us to read, the cluster's barriers, scans and the sort take the rest.
+// B200, one row of 128256 fp32: greedy 4.7 us, plain 7.6, min-p 9.0, top-k 50 with top-p 12.6, nucleus 17.8;
+// 16 rows of 152064 with mixed settings 53 (the row with top-k 1000 and top-p is the slowest). Up to 16 blocks a
+// row, each down to a vector a thread: a single block (below) takes 33 us for the row of top-k, 101 us for the nucleus.
 namespace smr {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 256;                      // 32 nats: what lies further below weighs nothing
@@ -880,6 +884,10 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
 // that few more than k tokens are listed; nucleus: the bins of e as in a cluster; then the kept weight of each
 // run ("cell") of the row, and the one cell that the target falls into. What does not fit its list or bin goes
 // the general way: a radix search, a pass over the row for each 8 bits.
+// B200, 256 rows of 128256 fp32 (131 MB, 20 us at the rate of a copy): greedy 25 us, min-p 65, top-k 50 with top-p
+// 70, plain 74, nucleus 159. The first pass comes from memory at 5.3 TB/s; the passes that need every token's exact
+// e are bound by their instructions (16 warps a row, about 40 a token) and not by L2: a nucleus has one such pass
+// and one over the tokens that reach the limit's bin, which are queued so that a warp works on 32 of them.
 namespace smw {
 constexpr int CELLS = 1024;                    // runs of 32 * K vectors
 }
