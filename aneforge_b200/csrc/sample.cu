@@ -61,7 +61,7 @@ struct RowScale {
 namespace smr {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 256;                      // 32 nats: what lies further below weighs nothing
-constexpr int LIST = 1024;                     // tokens that one block puts in order: LIST / C from each
+constexpr int LIST = 2048, PER = LIST / THREADS;             // tokens that one block puts in order: LIST / C from each
 constexpr int PAIRS = 256;                     // up to so many by comparing all pairs
 constexpr int LOCAL = 3200;                    // listed tokens of one block
 constexpr int MAXC = 16;
@@ -123,24 +123,57 @@ AF_DEV void weight_parts(float e, uint32_t& hi, uint32_t& lo) {
   lo = __float_as_uint(t2) - 0x37000000u;
 }
 
-// descending bitonic sort of N (a power of two) 64-bit values in shared memory by the whole block (one
-// warp where that is enough)
+// Descending bitonic sort of N values (a power of two, 128 to LIST) in shared memory by the whole block: a
+// thread holds PER neighbours, a step inside them or inside a warp needs no barrier.
 AF_DEV void sort_desc(u64* x, int N) {
-  const int tid = threadIdx.x;
-  const bool small = N <= 64;
-  if (small && tid >= 32) N = 0;
-  for (int k = 2; k <= N; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = tid; i < N / 2; i += smr::THREADS) {
-        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-        const u64 a = x[lo], b = x[hi];
-        const bool up = lo & k;                // this run ascends
-        if ((a < b) != up) { x[lo] = b; x[hi] = a; }
-        if (small) continue;
+  using namespace smr;
+  static_assert(PER == 4, "the steps inside a thread are written out");
+  const int p0 = PER * threadIdx.x;
+  const bool on = p0 < N;                      // whole warps
+  u64 v[PER];
+#pragma unroll
+  for (int q = 0; q < PER; ++q) v[q] = on ? x[p0 + q] : 0;
+  auto pair = [](u64& a, u64& b, bool desc) {
+    const u64 lo = a < b ? a : b, hi = a < b ? b : a;
+    a = desc ? hi : lo;
+    b = desc ? lo : hi;
+  };
+#pragma unroll 1
+  for (int k = 2; k <= N; k <<= 1) {
+    const bool desc = !(p0 & k);
+#pragma unroll 1
+    for (int j = k >> 1; j >= PER; j >>= 1) {
+      const bool top = desc == !(p0 & j);      // this thread's places get the larger ones
+      u64 o[PER];
+      if (j >= 32 * PER) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < PER; ++q)
+          if (on) x[p0 + q] = v[q];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < PER; ++q) o[q] = on ? x[(p0 ^ j) + q] : 0;
+      } else {
+#pragma unroll
+        for (int q = 0; q < PER; ++q) o[q] = __shfl_xor_sync(0xffffffffu, v[q], j / PER);
       }
-      if (small) __syncwarp();
-      else __syncthreads();
+#pragma unroll
+      for (int q = 0; q < PER; ++q) v[q] = (v[q] < o[q]) == top ? o[q] : v[q];
     }
+    if (k == 2) {
+      pair(v[0], v[1], true);
+      pair(v[2], v[3], false);
+      continue;
+    }
+    pair(v[0], v[2], desc);
+    pair(v[1], v[3], desc);
+    pair(v[0], v[1], desc);
+    pair(v[2], v[3], desc);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < PER; ++q)
+    if (on) x[p0 + q] = v[q];
   __syncthreads();
 }
 
@@ -187,8 +220,10 @@ AF_DEV void gather(SampleShared& sh, int C, int share) {
 
 // The last token in order (falling key, rising index) with less than `need` of the weight before it, of
 // the n <= LIST in `local`; by comparing all pairs, or by sorting where those are many.
-AF_DEV u64 last_of(SampleShared& sh, const RowScale& sc, int n, u64 need) {
+__device__ __noinline__ u64 last_of(RowScale sc, int n, u64 need) {
   using namespace smr;
+  extern __shared__ __align__(16) unsigned char sample_raw[];
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
   const int tid = threadIdx.x;
   if (n <= PAIRS) {
     int pad = 16;
@@ -205,18 +240,22 @@ AF_DEV u64 last_of(SampleShared& sh, const RowScale& sc, int n, u64 need) {
     __syncthreads();
     return sh.pick;
   }
-  int N = 2;
+  int N = 32 * PER;
   while (N < n) N <<= 1;
   for (int k = tid; k < N; k += THREADS) sh.list[k] = k < n ? sh.local[k] : 0;
   __syncthreads();
   sort_desc(sh.list, N);
-  u64 w[2], all;
+  u64 w[PER], all, mine = 0;
+  const int p0 = PER * tid;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) w[k] = 2 * tid + k < n ? sc.w(logit_of((uint32_t)(sh.list[2 * tid + k] >> 32))) : 0;
-  u64 b = scan_excl(w[0] + w[1], sh.scan, all);
+  for (int k = 0; k < PER; ++k) {
+    w[k] = p0 + k < n ? sc.w(logit_of((uint32_t)(sh.list[p0 + k] >> 32))) : 0;
+    mine += w[k];
+  }
+  u64 b = scan_excl(mine, sh.scan, all);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (2 * tid + k < n && b < need && need <= b + w[k]) sh.pick = sh.list[2 * tid + k];
+  for (int k = 0; k < PER; ++k) {
+    if (p0 + k < n && b < need && need <= b + w[k]) sh.pick = sh.list[p0 + k];
     b += w[k];
   }
   __syncthreads();
@@ -225,9 +264,11 @@ AF_DEV u64 last_of(SampleShared& sh, const RowScale& sc, int n, u64 need) {
 
 // The whole choice among the n <= LIST tokens in `local`, which hold every token that may be kept (k 0: no
 // top-k; without it `limit` is the nucleus' weight).
-AF_DEV void few_tokens(const SampleArgs& a, SampleShared& sh, const RowScale& sc, int r, int n, int k, bool use_p, float top_p,
-                       float min_p, float u, u64 limit) {
+__device__ __noinline__ void few_tokens(int* tok, float* logp, RowScale sc, int V, int n, int k, bool use_p, float top_p, float min_p,
+                                        float u, u64 limit) {
   using namespace smr;
+  extern __shared__ __align__(16) unsigned char sample_raw[];
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
   const int tid = threadIdx.x;
   u64 sum;
   if (n <= PAIRS) {
@@ -266,22 +307,22 @@ AF_DEV void few_tokens(const SampleArgs& a, SampleShared& sh, const RowScale& sc
       if ((uint32_t)sh.local[j] > (uint32_t)x) before += sh.list[j];       // a lower index: the complement is larger
     for (int o = L >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     if (mine && before <= target && target < before + kept) {
-      a.tok[r] = (int)~(uint32_t)x;
-      if (a.logp) a.logp[r] = logp_of(sc, logit_of(key), sum);
+      *tok = (int)~(uint32_t)x;
+      if (logp) *logp = logp_of(sc, logit_of(key), sum);
     }
     return;
   }
-  int N = 2;
+  int N = 32 * PER;
   while (N < n) N <<= 1;
   for (int q = tid; q < N; q += THREADS) sh.list[q] = q < n ? sh.local[q] : 0;
   __syncthreads();
   sort_desc(sh.list, N);
   const uint32_t kth = k && k <= n ? (uint32_t)(sh.list[k - 1] >> 32) : 0u;
-  const int p0 = 2 * tid;
-  u64 w[2], mine = 0;
-  float e[2];
+  const int p0 = PER * tid;
+  u64 w[PER], mine = 0;
+  float e[PER];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
+  for (int q = 0; q < PER; ++q) {
     const uint32_t key = p0 + q < n ? (uint32_t)(sh.list[p0 + q] >> 32) : 0u;
     const bool ok = p0 + q < n && key >= kth;
     e[q] = ok ? sc.e(logit_of(key)) : -1.f;
@@ -292,40 +333,54 @@ AF_DEV void few_tokens(const SampleArgs& a, SampleShared& sh, const RowScale& sc
   if (use_p && k) limit = (u64)ceil((double)top_p * (double)sum);
   u64 kept = 0;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
+  for (int q = 0; q < PER; ++q) {
     const bool ok = e[q] >= 0.f && (!use_p || before < limit) && e[q] >= min_p;
     before += w[q];
     if (!ok) w[q] = 0;
     kept += w[q];
   }
   scan_excl(kept, sh.scan, sum);
-  // the kept ones in index order: ~index << 32 | key, descending
-#pragma unroll
-  for (int q = 0; q < 2; ++q)
-    if (p0 + q < N) {
-      const u64 x = sh.list[p0 + q];
-      sh.list[p0 + q] = w[q] ? (x << 32 | x >> 32) : 0;
-    }
+  // index order: the kept weights of 512 equal runs of the vocabulary, then the tokens of the target's run
+  u64* cells = sh.radix[0];
+  static_assert(THREADS == 512 && sizeof(sh.radix) == 512 * sizeof(u64), "a run for each thread");
+  int shift = 0;
+  while ((V - 1) >> shift >= THREADS) ++shift;
+  cells[tid] = 0;
+  if (tid == 0) sh.nlocal = 0;
   __syncthreads();
-  sort_desc(sh.list, N);
-  mine = 0;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const u64 x = p0 + q < N ? sh.list[p0 + q] : 0;
-    w[q] = x ? sc.w(logit_of((uint32_t)x)) : 0;
-    mine += w[q];
-  }
+  for (int q = 0; q < PER; ++q)
+    if (w[q]) atomicAdd(&cells[(int)~(uint32_t)sh.list[p0 + q] >> shift], w[q]);
+  __syncthreads();
   const u64 target = draw_target(u, sum);
+  mine = cells[tid];
   u64 all;
   before = scan_excl(mine, sh.scan, all);
+  if (before <= target && target < before + mine) {
+    sh.where = tid;
+    sh.pick = target - before;
+  }
+  __syncthreads();
+  const int cell = sh.where;
+  const u64 in = sh.pick;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    if (before <= target && target < before + w[q]) {
-      const u64 x = sh.list[p0 + q];
-      a.tok[r] = (int)~(uint32_t)(x >> 32);
-      if (a.logp) a.logp[r] = logp_of(sc, logit_of((uint32_t)x), sum);
+  for (int q = 0; q < PER; ++q)
+    if (w[q] && (int)~(uint32_t)sh.list[p0 + q] >> shift == cell) {
+      const uint32_t at = atomicAdd(&sh.nlocal, 1u);
+      sh.mine[at] = sh.list[p0 + q];
+      sh.local[at] = w[q];
     }
-    before += w[q];
+  __syncthreads();
+  const int c = (int)sh.nlocal;
+  for (int i = tid; i < c; i += THREADS) {
+    const u64 x = sh.mine[i];
+    before = 0;
+    for (int j = 0; j < c; ++j)
+      if ((uint32_t)sh.mine[j] > (uint32_t)x) before += sh.local[j];       // a lower index: the complement is larger
+    if (before <= in && in < before + sh.local[i]) {
+      *tok = (int)~(uint32_t)x;
+      if (logp) *logp = logp_of(sc, logit_of((uint32_t)(x >> 32)), sum);
+    }
   }
 }
 
@@ -543,7 +598,8 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     if (small) {
       if (rank) return;                        // nobody reads the other blocks' memory any more
       gather(sh, C, share);
-      few_tokens(a, sh, sc, r, (int)n_all, use_k ? top_k : 0, use_p, top_p, min_p, u, use_k ? 0 : limit);
+      few_tokens(a.tok + r, a.logp ? a.logp + r : nullptr, sc, V, (int)n_all, use_k ? top_k : 0, use_p, top_p, min_p, u,
+                 use_k ? 0 : limit);
       return;
     }
   }
@@ -829,7 +885,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     }
     if (fit) {                                 // the same in every block
       gather(sh, C, share);
-      const u64 last = last_of(sh, sc, n_bin, need);
+      const u64 last = last_of(sc, n_bin, need);
       draw_e(max((q + 1) << EBITS, __float_as_uint(fmaxf(min_p, 0.f))), (int)sh.in_bin, last);
       return;
     }
@@ -1256,7 +1312,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
     __syncthreads();
     n_list = sh.nlocal;
     if (n_list <= (uint32_t)LIST) {
-      few_tokens(a, sh, sc, r, (int)n_list, top_k, use_p, top_p, min_p, u, 0);
+      few_tokens(a.tok + r, a.logp ? a.logp + r : nullptr, sc, V, (int)n_list, top_k, use_p, top_p, min_p, u, 0);
       return;
     }
     listed = n_list <= (uint32_t)LOCAL;
@@ -1375,7 +1431,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
       });
       const int n = (int)min(sh.in_bin, (uint32_t)LIST + 1);
       if (n <= LIST) {
-        const u64 last = last_of(sh, sc, n, sh.need);
+        const u64 last = last_of(sc, n, sh.need);
         l_last = logit_of((uint32_t)(last >> 32));
         i_last = (int)~(uint32_t)last;
         for (int k = tid; k < n; k += THREADS) {
