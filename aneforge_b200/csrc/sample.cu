@@ -55,9 +55,9 @@ struct RowScale {
 // of e (exactly: a bin's tokens share an octave, so a count and the sum of the lower bits give their
 // weight), only the bin that the limit falls into is sorted, and the kept sums come from the registers.
 // Bound by latency: a row of 0.5 MB takes 0.1 us to read, the cluster's barriers, scans and the sort take the rest.
-// B200, one row of 128256 fp32: greedy 4.7 us, plain 7.6, min-p 9.0, top-k 50 with top-p 12.6, nucleus 17.8;
-// 16 rows of 152064 with mixed settings 53 (the row with top-k 1000 and top-p is the slowest). Up to 16 blocks a
-// row, each down to a vector a thread: a single block (below) takes 33 us for the row of top-k, 101 us for the nucleus.
+// B200, one row of 128256 fp32: greedy 4.2 us, plain 7.0, min-p 8.9, top-k 50 with top-p 11.9, top-k 1000 26,
+// nucleus 18.0; 16 rows of 152064 with mixed settings 35 (two blocks share an SM; top-k 1000 and the nuclei are the
+// slowest). Up to 16 blocks a row, each down to a vector a thread: a single block (below) takes 33 us for the row of top-k, 101 us for the nucleus.
 namespace smr {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 256;                      // 32 nats: what lies further below weighs nothing
@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
 // run ("cell") of the row, and the one cell that the target falls into. What does not fit its list or bin goes
 // the general way: a radix search, a pass over the row for each 8 bits.
 // B200, 256 rows of 128256 fp32 (131 MB, 20 us at the rate of a copy): greedy 25 us, min-p 65, top-k 50 with top-p
-// 70, plain 74, nucleus 159. The first pass comes from memory at 5.3 TB/s; the passes that need every token's exact
+// 71, top-k 1000 128, plain 75, nucleus 160. The first pass comes from memory at 5.3 TB/s; the passes that need every token's exact
 // e are bound by their instructions (16 warps a row, about 40 a token) and not by L2: a nucleus has one such pass
 // and one over the tokens that reach the limit's bin, which are queued so that a warp works on 32 of them.
 namespace smw {
@@ -1566,9 +1566,9 @@ static cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
                            ((long long)a.R * C * 2 <= sms && (nvec + C - 1) / C > smr::THREADS)))
     C <<= 1;
   const int NV = ((nvec + C - 1) / C + smr::THREADS - 1) / smr::THREADS;
-  // one block per row from five rows for eight SMs on (B200, us, clusters / single blocks; 128256 fp32: 64 rows
-  // top-k 42 / 33, nucleus 66 / 101, min-p 31 / 34; 96 rows 61 / 33, 98 / 101, 45 / 34; 256 rows 168 / 71,
-  // 271 / 159, 125 / 66; 50257 fp16: 64 rows 21 / 18, 33 / 42, 16 / 18; 96 rows 34 / 18, 58 / 39, 25 / 18)
+  // one block per row from five rows for eight SMs on (B200, us, clusters / single blocks: 128256 fp32, 64 rows:
+  // top-k 46 / 33, nucleus 71 / 101, min-p 34 / 34, plain 26 / 37; 96 rows 64 / 33, 105 / 101, 47 / 34, 37 / 37; 256
+  // rows 171 / 71, 288 / 161, 129 / 66, 106 / 75; 50257 fp16, 96 rows: 39 / 18, 65 / 40, 28 / 19, 21 / 18)
   if (NV > 48 / VE || 8ll * a.R >= 5ll * sms) return launch_wide<T>(a, st);
   if (NV <= 8 / VE) return launch_rows<T, 8 / VE>(a, C, st);
   if (NV <= 16 / VE) return launch_rows<T, 16 / VE>(a, C, st);
