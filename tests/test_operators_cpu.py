@@ -76,3 +76,32 @@ def test_native_entries_refuse_before_they_launch():
   assert L.af_kv_compact(p, 1, 1, 128, 8, 8, p, 4, 4, p, p, p, 0, p, 1, p + 64, None, None) == -1
   assert L.af_attn_tree_scratch_bytes(1, 0, 1, 1, 64) == 0 and L.af_attn_tree_scratch_bytes(1, 1, 3, 2, 64) == 0
   assert L.af_kv_reserve_scratch_bytes(-1, 4) == 0
+
+
+def test_plan_ops_are_checked(tmp_path):
+  """The plan ops `sample` and `attn_tree`: a whole plan is taken, one with a buffer missing or too small is not."""
+  from aneforge_b200 import _runtime as R
+  from aneforge_b200.plan import PlanBuilder
+  lib = R.load_library()
+
+  def plan(**change):
+    pb = PlanBuilder()
+    size = dict(qkv=4 * 8 * 192, K=2 * 4 * 16 * 64, V=2 * 4 * 16 * 64, table=4 * 2 * 4, lens=8, mask=32, att=2 * 8 * 64,
+                scr=lib.af_attn_tree_scratch_bytes(2, 4, 1, 1, 64), logits=4 * 2 * 100, u=8, temp=8, topk=8, topp=8, minp=8, tok=8)
+    size.update({k: v for k, v in change.items() if k in size})
+    for k, v in size.items():
+      pb.buf(k, v, "ext" if k in ("K", "V", "table", "lens") else "state")
+    kv = dict(qkv="qkv", kc="K", vc="V", table="table", lens="lens", mask="mask", out="att", scr="scr", b=2, t=4, h=1, kv=1, dh=64,
+              p=4, page=16, w=4, scale=0.125)
+    kv.update({k: v for k, v in change.items() if k in kv and k not in size})
+    pb.op("attn_tree", **kv)
+    pb.op("sample", logits="logits", nb=2, v=100, u="u", temp="temp", topk="topk", topp="topp", minp="minp", tok="tok")
+    d = tmp_path / f"p{len(list(tmp_path.iterdir()))}"
+    d.mkdir()
+    (d / "plan.txt").write_text(pb.text())
+    return lib.af_compile_check(str(d).encode(), b"", 1, None)
+
+  assert plan() == 0
+  for bad in (dict(K=2), dict(table=4), dict(scr=64), dict(mask=16), dict(logits=400), dict(tok=4), dict(b=0), dict(t=257),
+              dict(kv=2), dict(vc="none"), dict(u=4)):
+    assert plan(**bad) == -1, bad
