@@ -12,7 +12,10 @@ from . import _runtime as R
 
 def _stream(t) -> int:
   import torch
-  return torch._C._cuda_getCurrentRawStream(t.get_device())       # a twentieth of current_stream(...).cuda_stream
+  dev = t.get_device()
+  if dev < 0:                                              # the raw call would take -1 for the current device
+    raise ValueError(f"a CUDA tensor is wanted, not one on {t.device}")
+  return torch._C._cuda_getCurrentRawStream(dev)                  # a twentieth of current_stream(...).cuda_stream
 
 
 def _p(t) -> int:

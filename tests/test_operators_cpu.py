@@ -105,3 +105,9 @@ def test_plan_ops_are_checked(tmp_path):
   for bad in (dict(K=2), dict(table=4), dict(scr=64), dict(mask=16), dict(logits=400), dict(tok=4), dict(b=0), dict(t=257),
               dict(kv=2), dict(vc="none"), dict(u=4)):
     assert plan(**bad) == -1, bad
+
+
+def test_no_stream_for_a_host_tensor():
+  """Wrappers without checks of their own (rmsnorm, attn_decode, gemv_tc, ...) launch nothing on host memory."""
+  with pytest.raises(ValueError, match="CUDA tensor"):
+    K._stream(torch.zeros(2))
