@@ -242,11 +242,28 @@ def gemm_tc(x, tiles, scales, N, K, wf=R.W_I8, bias=None, epi=R.EPI_F32, y=None)
   return y
 
 
-def _i32(t, shape, name):
+def _i32(t, shape, name, dev):
   import torch
-  if not (t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.shape == shape):
-    raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of shape {tuple(shape)}")
+  if not (t.dtype == torch.int32 and t.get_device() == dev and dev >= 0 and t.is_contiguous() and t.shape == shape):
+    raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on the call's CUDA device")
   return t.data_ptr()
+
+
+def _err(t, dev):
+  """The caller's error word, or none."""
+  import torch
+  if t is None:
+    return 0
+  if not (t.get_device() == dev and t.dtype == torch.int32 and t.numel() >= 1):
+    raise ValueError("err must be int32 [1] on the call's CUDA device")
+  return t.data_ptr()
+
+
+def _scratch(t, dev):
+  """Pointer and bytes of a workspace."""
+  if not (t.get_device() == dev and t.is_contiguous()):
+    raise ValueError("scratch must be a contiguous tensor on the call's CUDA device")
+  return t.data_ptr(), t.numel() * t.element_size()
 
 
 _SAMPLE_DT = {}
@@ -259,11 +276,11 @@ def _sample_types():
   return _SAMPLE_DT
 
 
-def _per_row(x, name, dtype, rows):
+def _per_row(x, name, dtype, rows, dev):
   """A setting as (pointer of its row values, 0) or (0, the number for all rows)."""
   if hasattr(x, "data_ptr"):
-    if not (x.is_cuda and x.dtype == dtype and x.shape == rows and x.is_contiguous()):
-      raise ValueError(f"{name} must be a number or a contiguous {dtype} CUDA tensor [R]")
+    if not (x.get_device() == dev and x.dtype == dtype and x.shape == rows and x.is_contiguous()):
+      raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [R] on the logits' device")
     return x.data_ptr(), 0
   _need(x == x and abs(x) != float("inf"), f"{name} must be finite")
   return 0, (max(-1, min(int(x), 0x7fffffff)) if name == "top_k" else x)
@@ -278,7 +295,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
   (tokens int32 [R], log-probabilities among the kept tokens fp32 [R]); -1 and -inf for a row that is all -inf
   or NaN. `out` = the two outputs, preallocated."""
   import torch
-  if not (logits.is_cuda and logits.dim() == 2 and logits.dtype in _sample_types()):
+  dev = logits.get_device()
+  if not (dev >= 0 and logits.dim() == 2 and logits.dtype in _sample_types()):
     raise ValueError("logits must be a 2-D CUDA tensor of fp32, fp16 or bf16")
   n, V = logits.shape
   ld, col = logits.stride()
@@ -287,17 +305,19 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     ld = V
   _need(ld >= V, "rows of logits must not overlap")
   rows = (n,)
-  _need(u.is_cuda and u.dtype == torch.float32 and u.shape == rows and u.is_contiguous(), "u must be fp32 [R] on the GPU")
-  pt, st = _per_row(temperature, "temperature", torch.float32, rows)
-  pk, sk = _per_row(top_k, "top_k", torch.int32, rows)
-  pp, sp = _per_row(top_p, "top_p", torch.float32, rows)
-  pm, sm = _per_row(min_p, "min_p", torch.float32, rows)
+  _need(u.get_device() == dev and u.dtype == torch.float32 and u.shape == rows and u.is_contiguous(),
+        "u must be fp32 [R] on the logits' device")
+  pt, st = _per_row(temperature, "temperature", torch.float32, rows, dev)
+  pk, sk = _per_row(top_k, "top_k", torch.int32, rows, dev)
+  pp, sp = _per_row(top_p, "top_p", torch.float32, rows, dev)
+  pm, sm = _per_row(min_p, "min_p", torch.float32, rows, dev)
   if out is None:
     tok, logp = torch.empty_like(u, dtype=torch.int32), torch.empty_like(u)
   else:
     tok, logp = out
-    _need(tok.dtype == torch.int32 and logp.dtype == torch.float32 and all(o.is_cuda and o.shape == rows and o.is_contiguous() for o in out),
-          "out must be (int32 [R], fp32 [R]) on the GPU")
+    _need(tok.dtype == torch.int32 and logp.dtype == torch.float32
+          and all(o.get_device() == dev and o.shape == rows and o.is_contiguous() for o in out),
+          "out must be (int32 [R], fp32 [R]) on the logits' device")
   rc = R.lib().af_sample(logits.data_ptr(), _SAMPLE_DT[logits.dtype], ld, n, V, u.data_ptr(), pt, pk, pp, pm, st, sk, sp, sm,
                          tok.data_ptr(), logp.data_ptr(), _stream(logits))
   if rc:
@@ -339,7 +359,8 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   error code of a node without a page or rotary position."""
   import torch
   f16 = torch.float16
-  if not (qkv.is_cuda and qkv.dtype == torch.float32 and qkv.dim() == 2 and table.dim() == 2):
+  dev = qkv.get_device()
+  if not (dev >= 0 and qkv.dtype == torch.float32 and qkv.dim() == 2 and table.dim() == 2):
     raise ValueError("qkv must be fp32 [B * T, cols] on the GPU and table int32 [B, W]")
   (n, cols), (ld, one), (B, W) = qkv.shape, qkv.stride(), table.shape
   if not (one == 1 and KV >= 1 and H % KV == 0 and cols >= (H + 2 * KV) * dh):
@@ -350,9 +371,9 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   if dh not in (16, 32, 64, 128):
     raise ValueError("head dims 16, 32, 64 and 128")
   shape, strides = kc.shape, kc.stride()
-  if not (kc.dtype == f16 and vc.dtype == f16 and kc.is_cuda and vc.is_cuda and vc.shape == shape and len(shape) == 4
-          and shape[1] == KV and shape[3] == dh):
-    raise ValueError("kc / vc must be fp16 [P, KV, page, dh] on the GPU")
+  if not (kc.dtype == f16 and vc.dtype == f16 and kc.get_device() == dev and vc.get_device() == dev and vc.shape == shape
+          and len(shape) == 4 and shape[1] == KV and shape[3] == dh):
+    raise ValueError("kc / vc must be fp16 [P, KV, page, dh] on qkv's device")
   P, _, page, _ = shape
   ps = strides[0] if P > 1 else KV * page * dh
   if not (strides[1:] == (page * dh, dh, 1) and vc.stride() == strides and ps >= KV * page * dh and ps % 8 == 0):
@@ -362,25 +383,26 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   if cos_t is not None:
     rows = cos_t.shape[0]
     if not (cos_t.shape == (rows, dh) and sin_t.shape == (rows, dh) and cos_t.dtype == f16 and sin_t.dtype == f16
-            and cos_t.is_contiguous() and sin_t.is_contiguous() and cos_t.is_cuda and sin_t.is_cuda):
-      raise ValueError("cos_t / sin_t must be fp16 [rows, dh] on the GPU")
+            and cos_t.is_contiguous() and sin_t.is_contiguous() and cos_t.get_device() == dev and sin_t.get_device() == dev):
+      raise ValueError("cos_t / sin_t must be fp16 [rows, dh] on qkv's device")
   for g, name in ((qn, "qn"), (kn, "kn")):
-    if g is not None and not (g.is_cuda and g.dtype == f16 and g.shape == (dh,) and g.is_contiguous()):
-      raise ValueError(f"{name} must be fp16 [dh] on the GPU")
+    if g is not None and not (g.get_device() == dev and g.dtype == f16 and g.shape == (dh,) and g.is_contiguous()):
+      raise ValueError(f"{name} must be fp16 [dh] on qkv's device")
   if out is None:
     out = qkv.new_empty((n, H * dh), dtype=f16)
     ldo = H * dh
   else:
-    if not (out.is_cuda and out.dtype == f16 and out.shape == (n, H * dh) and out.stride(1) == 1):
-      raise ValueError("out must be fp16 [B * T, H * dh]")
+    if not (out.get_device() == dev and out.dtype == f16 and out.shape == (n, H * dh) and out.stride(1) == 1):
+      raise ValueError("out must be fp16 [B * T, H * dh] on qkv's device")
     ldo = out.stride(0)
   if scratch is None:
     scratch = attn_tree_scratch(B, T, H, KV, dh, qkv.device)
+  scr, scr_bytes = _scratch(scratch, dev)
   rc = R.lib().af_attn_tree(
-    qkv.data_ptr(), ld, kc.data_ptr(), vc.data_ptr(), ps, P, page, _i32(table, (B, W), "table"), W, _i32(lens, (B,), "lens"),
-    0 if nodes is None else _i32(nodes, (B,), "nodes"), 0 if depth is None else _i32(depth, (B, T), "depth"),
-    0 if mask is None else _i32(mask, (B, T, words), "mask"), words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), qn_floor,
-    kn_floor, out.data_ptr(), ldo, B, T, H, KV, dh, scale, scratch.data_ptr(), scratch.numel(), _p(err), _stream(qkv))
+    qkv.data_ptr(), ld, kc.data_ptr(), vc.data_ptr(), ps, P, page, _i32(table, (B, W), "table", dev), W,
+    _i32(lens, (B,), "lens", dev), 0 if nodes is None else _i32(nodes, (B,), "nodes", dev),
+    0 if depth is None else _i32(depth, (B, T), "depth", dev), 0 if mask is None else _i32(mask, (B, T, words), "mask", dev), words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), qn_floor,
+    kn_floor, out.data_ptr(), ldo, B, T, H, KV, dh, scale, scr, scr_bytes, _err(err, dev), _stream(qkv))
   if rc:
     R.check(rc, "af_attn_tree")
   return out
@@ -393,13 +415,14 @@ def _book(table, lens, refs, slots):
   n = slots.shape[0]
   if n > 1024:
     raise ValueError("at most 1024 slots a call")
-  return (_i32(table, (S, W), "table"), S, W, _i32(lens, (S,), "lens"), 0 if refs is None else _i32(refs, refs.shape, "refs"),
-          _i32(slots, (n,), "slots"), n)
+  dev = table.get_device()
+  return (_i32(table, (S, W), "table", dev), S, W, _i32(lens, (S,), "lens", dev),
+          0 if refs is None else _i32(refs, refs.shape, "refs", dev), _i32(slots, (n,), "slots", dev), n, dev)
 
 
-def _pool(pool):
-  if not (pool.is_cuda and pool.dim() == 6 and pool.is_contiguous() and pool.element_size() == 2):
-    raise ValueError("pool must be a contiguous 16-bit CUDA tensor [layers, 2, P, KV, page, dh]")
+def _pool(pool, dev):
+  if not (pool.get_device() == dev and pool.dim() == 6 and pool.is_contiguous() and pool.element_size() == 2):
+    raise ValueError("pool must be a contiguous 16-bit tensor [layers, 2, P, KV, page, dh] on the table's device")
   L, two, P, KV, page, dh = pool.shape
   if two != 2 or dh % 8:
     raise ValueError("pool must be [layers, 2, P, KV, page, dh], dh a multiple of 8")
@@ -410,46 +433,48 @@ def kv_fork(table, lens, refs, src, dst, page, err=None):
   """Slots dst[i] become copies of slots src[i]: they give back the pages they hold and share the ones that src
   fills (counted in refs [P]); no row moves until `kv_reserve` makes a shared page writable. All int32 on the GPU;
   table [S, W], lens [S]. The dst are distinct and none is a src."""
-  pt, S, W, pl, pr, pd, n = _book(table, lens, refs, dst)
+  pt, S, W, pl, pr, pd, n, dev = _book(table, lens, refs, dst)
   _need(page >= 1, "page must be positive")
-  R.check(R.lib().af_kv_fork(pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src"), pd, n, _p(err), _stream(table)),
+  R.check(R.lib().af_kv_fork(pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src", dev), pd, n, _err(err, dev),
+                             _stream(table)),
           "af_kv_fork")
 
 
 def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
   """Rows [lens, lens + rows[i]) of each slot get pages of the slot's own: free ones, lowest number first, and
   copies (in every layer of pool [layers, 2, P, KV, page, dh]) of a shared page that rows are appended to."""
-  pt, S, W, pl, pr, ps, n = _book(table, lens, refs, slots)
-  L, P, KV, page, rb = _pool(pool)
+  pt, S, W, pl, pr, ps, n, dev = _book(table, lens, refs, slots)
+  L, P, KV, page, rb = _pool(pool, dev)
   _need(refs.shape[0] == P, "refs must have an entry for each page of the pool")
   lib = R.lib()
   need = lib.af_kv_reserve_scratch_bytes(n, P)
   if scratch is None:
     scratch = refs.new_empty((need // 4 + 1,))               # int32
-  R.check(lib.af_kv_reserve(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows"), n,
-                                scratch.data_ptr(), scratch.numel() * scratch.element_size(), _p(err), _stream(pool)), "af_kv_reserve")
+  scr, scr_bytes = _scratch(scratch, dev)
+  R.check(lib.af_kv_reserve(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows", dev), n,
+                            scr, scr_bytes, _err(err, dev), _stream(pool)), "af_kv_reserve")
 
 
 def kv_free(table, lens, refs, slots, page, keep=None, err=None):
   """Gives back what the slots hold past keep[i] rows (default: everything)."""
-  pt, S, W, pl, pr, ps, n = _book(table, lens, refs, slots)
+  pt, S, W, pl, pr, ps, n, dev = _book(table, lens, refs, slots)
   _need(page >= 1, "page must be positive")
-  R.check(R.lib().af_kv_free(pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep"), n,
-                             _p(err), _stream(table)), "af_kv_free")
+  R.check(R.lib().af_kv_free(pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep", dev), n,
+                             _err(err, dev), _stream(table)), "af_kv_free")
 
 
 def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
   """The rows lens + path[i, j], j < n_path[i], of each slot move to lens + j in every layer's K and V: the accepted
   path [n, D] through a drafted tree (node numbers, rising) becomes part of the prefix. Returns the new lengths:
   lens with n_path added to the listed slots (a new tensor, or lens_out)."""
-  pt, S, W, pl, _, ps, n = _book(table, lens, None, slots)
-  L, P, KV, page, rb = _pool(pool)
+  pt, S, W, pl, _, ps, n, dev = _book(table, lens, None, slots)
+  L, P, KV, page, rb = _pool(pool, dev)
   _need(path.dim() == 2, "path must be int32 [n, D]")
   D = path.shape[1]
   if lens_out is None:
     lens_out = lens.new_empty(lens.shape)
   _need(lens_out.data_ptr() != lens.data_ptr(), "lens_out must be another buffer than lens")
-  R.check(R.lib().af_kv_compact(pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path"), D,
-                                _i32(n_path, (n,), "n_path"), n, _i32(lens_out, (S,), "lens_out"), _p(err), _stream(pool)),
-          "af_kv_compact")
+  R.check(R.lib().af_kv_compact(pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path", dev), D,
+                                _i32(n_path, (n,), "n_path", dev), n, _i32(lens_out, (S,), "lens_out", dev), _err(err, dev),
+                                _stream(pool)), "af_kv_compact")
   return lens_out

@@ -111,3 +111,89 @@ def test_no_stream_for_a_host_tensor():
   """Wrappers without checks of their own (rmsnorm, attn_decode, gemv_tc, ...) launch nothing on host memory."""
   with pytest.raises(ValueError, match="CUDA tensor"):
     K._stream(torch.zeros(2))
+
+
+class On(torch.Tensor):
+  """A host tensor that says it lies on GPU `dev`."""
+  dev = 0
+  is_cuda = property(lambda self: self.dev >= 0)
+
+  def get_device(self):
+    return self.dev
+
+
+def on(dev, t):
+  t = t.as_subclass(On)
+  t.dev = dev
+  return t
+
+
+class Calls:
+  """A library that takes every call down, with the device it was made on."""
+
+  def __init__(self):
+    self.made = []
+
+  def __getattr__(self, name):
+    if name.endswith("_bytes"):
+      return lambda *a: 64
+    return lambda *a: self.made.append((name, torch._C._cuda_getDevice(), a[-1])) or 0
+
+
+@pytest.fixture
+def calls(monkeypatch):
+  c, now = Calls(), [0]
+
+  class Device:
+    def __init__(self, d):
+      self.d = d
+
+    def __enter__(self):
+      self.was, now[0] = now[0], self.d
+
+    def __exit__(self, *a):
+      now[0] = self.was
+
+  monkeypatch.setattr(K.R, "lib", lambda: c)
+  monkeypatch.setattr(K.R, "load_library", lambda: c)
+  monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+  monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
+  monkeypatch.setattr(torch.cuda, "device", Device)
+  return c
+
+
+def operands(dev):
+  """For each entry point: the call, and its tensors by name."""
+  i = lambda *s: on(dev, torch.zeros(s, dtype=torch.int32))
+  f = lambda *s: on(dev, torch.zeros(s))
+  h = lambda *s: on(dev, torch.zeros(s).half())
+  books = dict(table=i(3, 2), lens=i(3), refs=i(4), err=i(1))
+  return {
+    "af_sample": (lambda **k: K.sample(**k), dict(
+      logits=f(2, 8), u=f(2), temperature=f(2), top_k=i(2), top_p=f(2), min_p=f(2), out=(i(2), f(2)))),
+    "af_attn_tree": (lambda **k: K.attn_tree(H=1, KV=1, dh=64, scale=1.0, **k), dict(
+      qkv=f(2, 192), kc=h(4, 1, 8, 64), vc=h(4, 1, 8, 64), table=i(2, 1), lens=i(2), cos_t=h(8, 64), sin_t=h(8, 64), mask=i(2, 1, 1),
+      depth=i(2, 1), nodes=i(2), qn=h(64), kn=h(64), scratch=on(dev, torch.zeros(64, dtype=torch.uint8)), err=i(1), out=h(2, 64))),
+    "af_kv_fork": (lambda **k: K.kv_fork(page=8, **k), dict(books, src=i(1), dst=i(1))),
+    "af_kv_reserve": (lambda **k: K.kv_reserve(**k), dict(books, pool=h(1, 2, 4, 1, 8, 8), slots=i(1), rows=i(1), scratch=i(64))),
+    "af_kv_free": (lambda **k: K.kv_free(page=8, **k), dict(books, slots=i(1), keep=i(1))),
+    "af_kv_compact": (lambda **k: K.kv_compact(**k), dict(
+      pool=h(1, 2, 4, 1, 8, 8), table=i(3, 2), lens=i(3), slots=i(1), path=i(1, 2), n_path=i(1), lens_out=i(3), err=i(1))),
+  }
+
+
+@pytest.mark.parametrize("entry", ["af_sample", "af_attn_tree", "af_kv_fork", "af_kv_reserve", "af_kv_free", "af_kv_compact"])
+def test_every_operand_lies_on_the_calls_device(entry, calls):
+  """A tensor of the host or of another GPU, the workspace and the error word among them, is refused before a launch."""
+  call, good = operands(0)[entry]
+  call(**good)
+  assert [c[0] for c in calls.made] == [entry]
+  for name, t in good.items():
+    for dev in (-1, 1):
+      bad = tuple(on(dev, x.clone()) for x in t) if isinstance(t, tuple) else on(dev, t.clone())
+      with pytest.raises(ValueError):
+        call(**dict(good, **{name: bad}))
+  if "err" in good:
+    with pytest.raises(ValueError):
+      call(**dict(good, err=on(0, torch.zeros(1))))
+  assert len(calls.made) == 1
