@@ -249,6 +249,19 @@ def _i32(t, shape, name, dev):
   return t.data_ptr()
 
 
+def _on(dev, name, *args):
+  """Calls the C entry `name` on GPU `dev` and its current stream, whichever GPU is the current one."""
+  import torch
+  fn, stream = getattr(R.lib(), name), torch._C._cuda_getCurrentRawStream(dev)
+  if dev == torch._C._cuda_getDevice():
+    rc = fn(*args, stream)
+  else:
+    with torch.cuda.device(dev):
+      rc = fn(*args, stream)
+  if rc:
+    R.check(rc, name)
+
+
 def _err(t, dev):
   """The caller's error word, or none."""
   import torch
@@ -318,10 +331,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     _need(tok.dtype == torch.int32 and logp.dtype == torch.float32
           and all(o.get_device() == dev and o.shape == rows and o.is_contiguous() for o in out),
           "out must be (int32 [R], fp32 [R]) on the logits' device")
-  rc = R.lib().af_sample(logits.data_ptr(), _SAMPLE_DT[logits.dtype], ld, n, V, u.data_ptr(), pt, pk, pp, pm, st, sk, sp, sm,
-                         tok.data_ptr(), logp.data_ptr(), _stream(logits))
-  if rc:
-    R.check(rc, "af_sample")
+  _on(dev, "af_sample", logits.data_ptr(), _SAMPLE_DT[logits.dtype], ld, n, V, u.data_ptr(), pt, pk, pp, pm, st, sk, sp, sm,
+      tok.data_ptr(), logp.data_ptr())
   return tok, logp
 
 
@@ -398,13 +409,12 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   if scratch is None:
     scratch = attn_tree_scratch(B, T, H, KV, dh, qkv.device)
   scr, scr_bytes = _scratch(scratch, dev)
-  rc = R.lib().af_attn_tree(
-    qkv.data_ptr(), ld, kc.data_ptr(), vc.data_ptr(), ps, P, page, _i32(table, (B, W), "table", dev), W,
-    _i32(lens, (B,), "lens", dev), 0 if nodes is None else _i32(nodes, (B,), "nodes", dev),
-    0 if depth is None else _i32(depth, (B, T), "depth", dev), 0 if mask is None else _i32(mask, (B, T, words), "mask", dev), words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), qn_floor,
-    kn_floor, out.data_ptr(), ldo, B, T, H, KV, dh, scale, scr, scr_bytes, _err(err, dev), _stream(qkv))
-  if rc:
-    R.check(rc, "af_attn_tree")
+  _on(dev, "af_attn_tree",
+      qkv.data_ptr(), ld, kc.data_ptr(), vc.data_ptr(), ps, P, page, _i32(table, (B, W), "table", dev), W,
+      _i32(lens, (B,), "lens", dev), 0 if nodes is None else _i32(nodes, (B,), "nodes", dev),
+      0 if depth is None else _i32(depth, (B, T), "depth", dev), 0 if mask is None else _i32(mask, (B, T, words), "mask", dev),
+      words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), qn_floor, kn_floor, out.data_ptr(), ldo, B, T, H, KV, dh, scale, scr,
+      scr_bytes, _err(err, dev))
   return out
 
 
@@ -435,9 +445,7 @@ def kv_fork(table, lens, refs, src, dst, page, err=None):
   table [S, W], lens [S]. The dst are distinct and none is a src."""
   pt, S, W, pl, pr, pd, n, dev = _book(table, lens, refs, dst)
   _need(page >= 1, "page must be positive")
-  R.check(R.lib().af_kv_fork(pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src", dev), pd, n, _err(err, dev),
-                             _stream(table)),
-          "af_kv_fork")
+  _on(dev, "af_kv_fork", pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src", dev), pd, n, _err(err, dev))
 
 
 def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
@@ -446,21 +454,19 @@ def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
   pt, S, W, pl, pr, ps, n, dev = _book(table, lens, refs, slots)
   L, P, KV, page, rb = _pool(pool, dev)
   _need(refs.shape[0] == P, "refs must have an entry for each page of the pool")
-  lib = R.lib()
-  need = lib.af_kv_reserve_scratch_bytes(n, P)
   if scratch is None:
-    scratch = refs.new_empty((need // 4 + 1,))               # int32
+    scratch = refs.new_empty((R.lib().af_kv_reserve_scratch_bytes(n, P) // 4 + 1,))               # int32
   scr, scr_bytes = _scratch(scratch, dev)
-  R.check(lib.af_kv_reserve(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows", dev), n,
-                            scr, scr_bytes, _err(err, dev), _stream(pool)), "af_kv_reserve")
+  _on(dev, "af_kv_reserve", pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows", dev), n, scr,
+      scr_bytes, _err(err, dev))
 
 
 def kv_free(table, lens, refs, slots, page, keep=None, err=None):
   """Gives back what the slots hold past keep[i] rows (default: everything)."""
   pt, S, W, pl, pr, ps, n, dev = _book(table, lens, refs, slots)
   _need(page >= 1, "page must be positive")
-  R.check(R.lib().af_kv_free(pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep", dev), n,
-                             _err(err, dev), _stream(table)), "af_kv_free")
+  _on(dev, "af_kv_free", pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep", dev), n,
+      _err(err, dev))
 
 
 def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
@@ -474,7 +480,6 @@ def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
   if lens_out is None:
     lens_out = lens.new_empty(lens.shape)
   _need(lens_out.data_ptr() != lens.data_ptr(), "lens_out must be another buffer than lens")
-  R.check(R.lib().af_kv_compact(pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path", dev), D,
-                                _i32(n_path, (n,), "n_path", dev), n, _i32(lens_out, (S,), "lens_out", dev), _err(err, dev),
-                                _stream(pool)), "af_kv_compact")
+  _on(dev, "af_kv_compact", pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path", dev), D,
+      _i32(n_path, (n,), "n_path", dev), n, _i32(lens_out, (S,), "lens_out", dev), _err(err, dev))
   return lens_out

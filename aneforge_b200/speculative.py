@@ -162,9 +162,10 @@ def tree_generate(target: LlamaPrefill, draft: LlamaPrefill, token_ids, max_new_
         logits = model._logits(pre["prog"].read_output("hid")[real - 1])
       torch.cuda.synchronize(dev)
     from . import kernels
-    first, _ = kernels.sample(torch.from_numpy(np.ascontiguousarray(logits, np.float32)).to(dev)[None],
-                              torch.from_numpy(rng.random(1, np.float32)).to(dev), temperature, top_k, top_p, min_p)
-    cur = int(first[0])
+    with torch.cuda.stream(big.stream):
+      first, _ = kernels.sample(torch.from_numpy(np.ascontiguousarray(logits, np.float32)).to(dev)[None],
+                                torch.from_numpy(rng.random(1, np.float32)).to(dev), temperature, top_k, top_p, min_p)
+      cur = int(first[0])
     out, n_steps, n_accept = [cur], 0, 0
     if on_token is not None and cur not in eos:
       on_token(cur)

@@ -197,3 +197,13 @@ def test_every_operand_lies_on_the_calls_device(entry, calls):
     with pytest.raises(ValueError):
       call(**dict(good, err=on(0, torch.zeros(1))))
   assert len(calls.made) == 1
+
+
+@pytest.mark.parametrize("entry", ["af_sample", "af_attn_tree", "af_kv_fork", "af_kv_reserve", "af_kv_free", "af_kv_compact"])
+def test_a_call_runs_on_its_operands_gpu(entry, calls):
+  """With GPU 0 current and the operands on GPU 1, the launch is made on GPU 1, on its stream."""
+  call, good = operands(1)[entry]
+  call(**good)
+  call, good = operands(0)[entry]
+  call(**good)
+  assert calls.made == [(entry, 1, 101), (entry, 0, 100)] and torch._C._cuda_getDevice() == 0
