@@ -246,11 +246,12 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvPagesArgs a) {
   }
 }
 
-// whether rows j, j + step, ... of a path can be taken: its nodes rise (parents come before children) and
-// its rows have pages
+// whether rows j, j + step, ... of a path can be taken: its nodes rise (parents come before children), its rows
+// have pages, and none of slots j, j + step, ... before it is the same one (whose block moves rows meanwhile)
 AF_DEV bool path_bad(const KvPagesArgs& a, int b, int s, int n, int len, int j, int step) {
   bool bad = s < 0 || s >= a.S || n < 0 || n > a.D;
   if (bad) return true;
+  for (int k = j; k < b; k += step) bad |= a.slots[k] == s;
   const int* table = a.table + (size_t)s * a.W;
   for (; j < n && !bad; j += step) {
     const int at = a.path[(size_t)b * a.D + j];
@@ -365,7 +366,8 @@ cudaError_t kv_reserve_launch(const KvPagesArgs& a, cudaStream_t st) {
 }
 
 cudaError_t kv_compact_launch(const KvPagesArgs& a, cudaStream_t st) {
-  if (!pages_ok(a) || ((!a.rows || !a.path) && a.n) || !pool_ok(a) || a.D < 1 || !a.lens_out || a.lens_out == a.lens)
+  if (!pages_ok(a) || ((!a.rows || !a.path) && a.n) || !pool_ok(a) || a.D < 1 || !a.lens_out || a.lens_out == a.lens ||
+      a.n > pages::THREADS)
     return cudaErrorInvalidValue;
   if (a.n == 0) return cudaMemcpyAsync(a.lens_out, a.lens, 4 * (size_t)a.S, cudaMemcpyDeviceToDevice, st);
   kv_compact_kernel<<<dim3(a.n, 2 * a.layers + 1), 256, 0, st>>>(a);

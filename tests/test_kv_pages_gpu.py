@@ -255,3 +255,32 @@ def test_rows_past_32_bits():
   pool[:, :, P - 1, :, 47] = 3.0
   out = K.kv_compact(pool, table, lens, i(1), i(7).view(1, 1), i(1))
   assert out.tolist() == [40, 41] and bool((pool[:, :, P - 1, :, 40] == 3.0).all())
+
+
+@pytest.mark.parametrize("KV,dh", [(1, 8), (8, 128)])
+def test_compact_of_a_slot_listed_twice(KV, dh):
+  """Only the first mention moves rows and counts, as for the other calls; the second one is recorded."""
+  S, T = 300, 12
+  m = Model(2, S * 2, KV, 16, dh, S, 2)
+  d = Device(m)
+  for x in (m, d):
+    x.reserve(list(range(S)), [30] * S)
+  m.lens[:] = 15
+  d.lens = torch.tensor(m.lens).cuda()
+  slots = list(range(S))
+  path = [[1, 4, 7, 11]] * S
+  for where in (1, 40, S - 1):                             # the same warp's, another's, another pass of the block's
+    slots[where] = slots[0]
+  n = [1 + i % 4 for i in range(S)]
+  d.compact(slots, path, n)
+  assert int(d.err) == 5
+  d.err.zero_()
+  ok = [i for i in range(S) if slots.index(slots[i]) == i]
+  assert len(ok) == S - 3
+  m.compact([slots[i] for i in ok], [path[i] for i in ok], [n[i] for i in ok])
+  d.same(m)
+  d.compact([2, 2], [[0, 3], [1, 2]], [2, 2])
+  assert int(d.err) == 5
+  d.err.zero_()
+  m.compact([2], [[0, 3]], [2])
+  d.same(m)

@@ -207,3 +207,14 @@ def test_a_call_runs_on_its_operands_gpu(entry, calls):
   call, good = operands(0)[entry]
   call(**good)
   assert calls.made == [(entry, 1, 101), (entry, 0, 100)] and torch._C._cuda_getDevice() == 0
+
+
+def test_compact_refuses_more_slots_than_the_other_page_calls():
+  from aneforge_b200 import build, _runtime as R
+  L = ctypes.CDLL(str(build.build()))
+  for name, res, args in R.SIGNATURES:
+    getattr(L, name).restype, getattr(L, name).argtypes = res, args
+  p = 1 << 20                                              # never read
+  for n in (-1, 1025):
+    assert L.af_kv_compact(p, 1, 1, 128, 8, 8, p, 4, 4, p, p, p, 1, p, n, p + 64, None, None) == -1
+    assert b"invalid argument" in L.af_last_error()
