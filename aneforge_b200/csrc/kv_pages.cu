@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(pages::THREADS) kv_free_kernel(KvPagesArgs a) 
   __syncthreads();
   list[i] = s;
   if (s >= 0) {
-    const int len = a.lens[s];
+    const int len = max(a.lens[s], 0);
     const int keep = a.rows ? min(max(a.rows[i], 0), len) : 0;
     from[i] = (keep + a.page - 1) / a.page;
     a.lens[s] = keep;
@@ -152,14 +152,14 @@ __global__ void __launch_bounds__(pages::THREADS) kv_reserve_kernel(KvPagesArgs 
   if (s >= 0) {
     const int len = a.lens[s], need = max(a.rows[i], 0);
     t = a.table + (size_t)s * a.W;
-    c0 = len / a.page;
-    fill = len - c0 * a.page;
-    c1 = (int)(((long long)len + need + a.page - 1) / a.page);
-    if (c1 > a.W || need == 0) {
+    const long long end = ((long long)len + need + a.page - 1) / a.page;
+    if (len < 0 || end > a.W || need == 0) {    // nothing for this slot
       if (need) af_set_err(a.err, AF_DEV_BAD_POS);
-      c1 = c0 = 0;                              // nothing for this slot
-    } else if (fill) {
-      tail = t[c0];
+    } else {
+      c0 = len / a.page;
+      c1 = (int)end;
+      fill = len - c0 * a.page;
+      if (fill) tail = t[c0];
       if (tail >= a.P) tail = -1;
     }
   }
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvPagesArgs a) {
 // whether rows j, j + step, ... of a path can be taken: its nodes rise (parents come before children), its rows
 // have pages, and none of slots j, j + step, ... before it is the same one (whose block moves rows meanwhile)
 AF_DEV bool path_bad(const KvPagesArgs& a, int b, int s, int n, int len, int j, int step) {
-  bool bad = s < 0 || s >= a.S || n < 0 || n > a.D;
+  bool bad = s < 0 || s >= a.S || len < 0 || n < 0 || n > a.D;
   if (bad) return true;
   for (int k = j; k < b; k += step) bad |= a.slots[k] == s;
   const int* table = a.table + (size_t)s * a.W;

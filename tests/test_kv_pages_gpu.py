@@ -284,3 +284,38 @@ def test_compact_of_a_slot_listed_twice(KV, dh):
   d.err.zero_()
   m.compact([2], [[0, 3]], [2])
   d.same(m)
+
+
+@pytest.mark.parametrize("page", [1, 8])
+def test_lengths_and_reservations_outside_the_table(page):
+  """A length under 0, and rows whose count passes 32 bits: refused like any that the table cannot hold."""
+  most = (1 << 31) - 1
+  m = Model(1, 64, 1, page, 8, 4, 64 // page)
+  d = Device(m)
+  for x in (m, d):
+    x.reserve([0, 1], [20, 20])
+
+  def at(*lens):
+    m.lens[:] = lens
+    d.lens = torch.tensor(m.lens).cuda()
+
+  def refused(code):
+    assert int(d.err) == code
+    d.err.zero_()
+    d.same(m)
+
+  for n in (-1, -20, -most - 1):
+    at(n, 10, 0, 0)
+    d.reserve([0], [5]); refused(2)
+    d.reserve([0], [most]); refused(2)
+    d.reserve([0], [0]); d.same(m)
+    d.compact([0], [[1, 2]], [2]); refused(5)
+    d.reserve([0, 1], [5, 2])                              # the others get theirs
+    m.reserve([1], [2]); refused(2)
+  at(10, 10, most, 0)
+  d.reserve([1], [most]); refused(2)
+  d.reserve([2], [1]); refused(2)
+  d.reserve([2], [most]); refused(2)
+  at(-3, 10, 0, 0)
+  d.free([0])
+  m.lens[0] = 0; m.free([0]); d.same(m)
