@@ -33,6 +33,13 @@ AF_DEV uint32_t key_of(float l) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// a row's temperature. An infinite one would make NaN of the logits that are -inf (masked, or past the row's end): it
+// counts as the largest finite one, by which every logit under 1e30 in size still weighs as much as the largest
+AF_DEV float row_temperature(const SampleArgs& a, int r) {
+  const float t = a.temperature ? __ldg(a.temperature + r) : a.temperature_s;
+  return t == INFINITY ? 3.402823466e38f : t;
+}
+
 struct RowScale {
   float lmax, zmax, temp;
   AF_DEV float below(float l) const {           // z - max z, 0 for the largest (also where both are infinite)
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / C, rank = blockIdx.x % C, V = a.V;
-  const float temp = a.temperature ? __ldg(a.temperature + r) : a.temperature_s;
+  const float temp = row_temperature(a, r);
   const int top_k = a.top_k ? __ldg(a.top_k + r) : a.top_k_s;
   const float top_p = a.top_p ? __ldg(a.top_p + r) : a.top_p_s;
   const float min_p = fminf(a.min_p ? __ldg(a.min_p + r) : a.min_p_s, 1.f);
@@ -957,7 +964,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
   u64* cells = reinterpret_cast<u64*>(sh.ecnt);              // after the bins
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x, V = a.V;
-  const float temp = a.temperature ? __ldg(a.temperature + r) : a.temperature_s;
+  const float temp = row_temperature(a, r);
   const int top_k = a.top_k ? __ldg(a.top_k + r) : a.top_k_s;
   const float top_p = a.top_p ? __ldg(a.top_p + r) : a.top_p_s;
   const float min_p = fminf(a.min_p ? __ldg(a.min_p + r) : a.min_p_s, 1.f);

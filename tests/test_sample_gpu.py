@@ -274,3 +274,26 @@ def test_many_rows_agree_with_few(V, dtype):
     toks, logps = go(8)
     assert toks.reshape(8, 24).tolist() == [tok.tolist()] * 8
     np.testing.assert_allclose(logps.reshape(8, 24), np.tile(logp, (8, 1)), rtol=2.0 ** -20, atol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("reps", [1, 24])                  # clusters; one block a row
+@pytest.mark.parametrize("V,dtype", [(31, torch.float32), (3001, torch.bfloat16), (50257, torch.float32)])
+def test_an_infinite_temperature_draws_evenly(V, dtype, reps):
+  """Every token that is not masked weighs the same; a token past the row, or a masked one, is never drawn."""
+  rng = np.random.default_rng(V)
+  l = rows(5, V, 81)
+  l[1, ::3] = NEG
+  l[2, V // 2:] = NEG
+  l[3, 1::2] = np.nan
+  l[4, :] = NEG
+  l[4, V - 1] = 3.0
+  x = torch.tensor(l).to(dtype)
+  lf = x.float().numpy()
+  for k, p, mp in ((0, 1.0, 0.0), (7, 1.0, 0.0), (600, 1.0, 0.0), (0, 0.75, 0.0), (0, 1.0, 0.5), (20, 0.5, 0.25)):
+    for scalar in (False, True):
+      want = [pick(distribution(lf[r], 1e300, k, p, mp), rng) for r in range(5)]
+      temp = 1e39 if scalar else torch.full((5 * reps,), float("inf")).cuda()        # 1e39 is infinite in 32 bits
+      tok, logp = run(x.repeat(reps, 1).cuda(), [w[1] for w in want] * reps, temperature=temp, top_k=k, top_p=p, min_p=mp)
+      assert tok.tolist() == [w[0] for w in want] * reps, (k, p, mp)
+      ref = [np.log(distribution(lf[r], 1e300, k, p, mp)[want[r][0]]) for r in range(5)]
+      np.testing.assert_allclose(logp, ref * reps, atol=2.0 ** -18)
