@@ -42,9 +42,15 @@ AF_DEV float row_temperature(const SampleArgs& a, int r) {
 
 struct RowScale {
   float lmax, zmax, temp;
-  AF_DEV float below(float l) const {           // z - max z, 0 for the largest (also where both are infinite)
+  AF_DEV float below(float l) const {           // z - max z, 0 for the largest
+    if (l == lmax) return 0.f;
+    if (isinf(zmax)) return __fdiv_rn(l - lmax, temp);       // the quotients overflow, of unequal logits as well
     const float z = __fdiv_rn(l, temp);
-    return l == lmax || z == zmax ? 0.f : z - zmax;
+    return z == zmax ? 0.f : z - zmax;
+  }
+  // whether distances to the largest logit, in units of `scale` a logit, mean nothing
+  AF_DEV bool far(float scale) const {
+    return !(zmax < 1e30f && zmax > -1e30f && lmax < 1e30f && lmax > -1e30f && scale < INFINITY);
   }
   AF_DEV float e(float l) const { return expf(below(l)); }
   AF_DEV u64 w(float l) const { return (u64)(e(l) * 1099511627776.f); }
@@ -484,8 +490,8 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     return;
   }
   // ---- how far below the maximum the logits lie; total weight
-  const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
   const float scale = 8.f / sc.temp;
+  const bool far = sc.far(scale);
   float cut = -INFINITY;                       // no token under `cut` can be kept
   u64 total_w = 0, limit = 0;
   // e in the logits' place (past the row's end: 0)
@@ -1072,7 +1078,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
     }
     return;
   }
-  const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
+  const bool far = sc.far(8.f / sc.temp);
   auto e_of = [&](float l) {
     if (far) return sc.e(l);
     return expf((sc.temp == 1.f ? l : __fdiv_rn(l, sc.temp)) - sc.zmax);

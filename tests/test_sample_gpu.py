@@ -297,3 +297,29 @@ def test_an_infinite_temperature_draws_evenly(V, dtype, reps):
       assert tok.tolist() == [w[0] for w in want] * reps, (k, p, mp)
       ref = [np.log(distribution(lf[r], 1e300, k, p, mp)[want[r][0]]) for r in range(5)]
       np.testing.assert_allclose(logp, ref * reps, atol=2.0 ** -18)
+
+
+@pytest.mark.parametrize("reps", [1, 24])                  # clusters; one block a row
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_temperatures_near_zero(dtype, reps):
+  """Logits whose quotient or difference overflows: the largest takes all the weight, however it is chosen."""
+  l = rows(5, 3001, 71)
+  l[0] -= l[0].max() + 1.0                                 # the largest will be 0: 0 times an infinite scale is no distance
+  l[1] -= l[1].max() + 1.0                                 # all quotients -inf
+  l[2] += 8.0 - l[2].max()                                 # many quotients +inf
+  l[3, 100:] = NEG
+  l[4, ::2] = np.nan
+  x = torch.tensor(l).to(dtype)
+  x[0, 17], x[1, 3000], x[2, 0], x[3, 50], x[4, 7] = 0.0, -0.5, 20.0, 30.0, 25.0
+  want = [17, 3000, 0, 50, 7]
+  if dtype == torch.float32:
+    x[0, 0], want[0] = 0.0, 0
+    x[0, 17] = -1e-30
+  x = x.repeat(reps, 1).cuda()
+  n = 5 * reps
+  for temp in (1e-45, 1e-39, 2e-38, 1e-36):
+    for kw in (dict(), dict(top_k=40), dict(top_k=600), dict(min_p=0.25), dict(top_p=0.5), dict(top_k=40, top_p=0.5, min_p=0.1)):
+      out = torch.full((n,), -7, dtype=torch.int32).cuda(), torch.full((n,), 5.0).cuda()
+      tok, logp = run(x, np.tile(np.float32([0.0, 0.5, 0.9, 0.99, 0.2]), reps), temperature=torch.full((n,), temp).cuda(), out=out, **kw)
+      assert tok.tolist() == want * reps, (temp, kw)
+      assert (logp == 0).all(), (temp, kw)
