@@ -7,11 +7,12 @@ import ctypes
 
 import numpy as np
 
+import torch
+
 from . import _runtime as R
 
 
 def _stream(t) -> int:
-  import torch
   dev = t.get_device()
   if dev < 0:                                              # the raw call would take -1 for the current device
     raise ValueError(f"a CUDA tensor is wanted, not one on {t.device}")
@@ -243,28 +244,26 @@ def gemm_tc(x, tiles, scales, N, K, wf=R.W_I8, bias=None, epi=R.EPI_F32, y=None)
 
 
 def _i32(t, shape, name, dev):
-  import torch
   if not (t.dtype == torch.int32 and t.get_device() == dev and dev >= 0 and t.is_contiguous() and t.shape == shape):
     raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on the call's CUDA device")
   return t.data_ptr()
 
 
-def _on(dev, name, *args):
-  """Calls the C entry `name` on GPU `dev` and its current stream, whichever GPU is the current one."""
-  import torch
-  fn, stream = getattr(R.lib(), name), torch._C._cuda_getCurrentRawStream(dev)
+def _entry(name, dev):
+  """The C entry `name`, which runs on GPU `dev` whichever one is current; its last argument is dev's stream."""
+  fn = getattr(R.lib(), name)
   if dev == torch._C._cuda_getDevice():
-    rc = fn(*args, stream)
-  else:
+    return fn
+
+  def there(*args):
     with torch.cuda.device(dev):
-      rc = fn(*args, stream)
-  if rc:
-    R.check(rc, name)
+      return fn(*args)
+
+  return there
 
 
 def _err(t, dev):
   """The caller's error word, or none."""
-  import torch
   if t is None:
     return 0
   if not (t.get_device() == dev and t.dtype == torch.int32 and t.numel() >= 1):
@@ -279,14 +278,7 @@ def _scratch(t, dev):
   return t.data_ptr(), t.numel() * t.element_size()
 
 
-_SAMPLE_DT = {}
-
-
-def _sample_types():
-  if not _SAMPLE_DT:
-    import torch
-    _SAMPLE_DT.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-  return _SAMPLE_DT
+_SAMPLE_DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _per_row(x, name, dtype, rows, dev):
@@ -307,9 +299,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
   (fp32; top_k int32); 0 (or top_p 1) turns it off, temperature 0 takes the first largest logit. Returns
   (tokens int32 [R], log-probabilities among the kept tokens fp32 [R]); -1 and -inf for a row that is all -inf
   or NaN. `out` = the two outputs, preallocated."""
-  import torch
   dev = logits.get_device()
-  if not (dev >= 0 and logits.dim() == 2 and logits.dtype in _sample_types()):
+  if not (dev >= 0 and logits.dim() == 2 and logits.dtype in _SAMPLE_DT):
     raise ValueError("logits must be a 2-D CUDA tensor of fp32, fp16 or bf16")
   n, V = logits.shape
   ld, col = logits.stride()
@@ -331,8 +322,10 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     _need(tok.dtype == torch.int32 and logp.dtype == torch.float32
           and all(o.get_device() == dev and o.shape == rows and o.is_contiguous() for o in out),
           "out must be (int32 [R], fp32 [R]) on the logits' device")
-  _on(dev, "af_sample", logits.data_ptr(), _SAMPLE_DT[logits.dtype], ld, n, V, u.data_ptr(), pt, pk, pp, pm, st, sk, sp, sm,
-      tok.data_ptr(), logp.data_ptr())
+  rc = _entry("af_sample", dev)(logits.data_ptr(), _SAMPLE_DT[logits.dtype], ld, n, V, u.data_ptr(), pt, pk, pp, pm, st, sk, sp, sm,
+                                tok.data_ptr(), logp.data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
+  if rc:
+    R.check(rc, "af_sample")
   return tok, logp
 
 
@@ -353,7 +346,6 @@ def tree_layout(parents):
 
 def attn_tree_scratch(B, T, H, KV, dh, device=None):
   """Workspace of `attn_tree` for these sizes; it may serve any number of calls of one stream."""
-  import torch
   return torch.zeros((max(1, R.load_library().af_attn_tree_scratch_bytes(B, T, H, KV, dh)),), dtype=torch.uint8,
                      device=device or "cuda")
 
@@ -368,7 +360,6 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   decode step. nodes [B]: live nodes of each sequence. lens is left as it is (`kv_compact` advances it). Returns
   fp16 [B * T, H * dh], zeros for nodes that see nothing or are not live. err: int32 [1], zero: gets the device
   error code of a node without a page or rotary position."""
-  import torch
   f16 = torch.float16
   dev = qkv.get_device()
   if not (dev >= 0 and qkv.dtype == torch.float32 and qkv.dim() == 2 and table.dim() == 2):
@@ -409,12 +400,14 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   if scratch is None:
     scratch = attn_tree_scratch(B, T, H, KV, dh, qkv.device)
   scr, scr_bytes = _scratch(scratch, dev)
-  _on(dev, "af_attn_tree",
+  rc = _entry("af_attn_tree", dev)(
       qkv.data_ptr(), ld, kc.data_ptr(), vc.data_ptr(), ps, P, page, _i32(table, (B, W), "table", dev), W,
       _i32(lens, (B,), "lens", dev), 0 if nodes is None else _i32(nodes, (B,), "nodes", dev),
       0 if depth is None else _i32(depth, (B, T), "depth", dev), 0 if mask is None else _i32(mask, (B, T, words), "mask", dev),
       words, _p(cos_t), _p(sin_t), rows, _p(qn), _p(kn), qn_floor, kn_floor, out.data_ptr(), ldo, B, T, H, KV, dh, scale, scr,
-      scr_bytes, _err(err, dev))
+      scr_bytes, _err(err, dev), torch._C._cuda_getCurrentRawStream(dev))
+  if rc:
+    R.check(rc, "af_attn_tree")
   return out
 
 
@@ -445,7 +438,8 @@ def kv_fork(table, lens, refs, src, dst, page, err=None):
   table [S, W], lens [S]. The dst are distinct and none is a src."""
   pt, S, W, pl, pr, pd, n, dev = _book(table, lens, refs, dst)
   _need(page >= 1, "page must be positive")
-  _on(dev, "af_kv_fork", pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src", dev), pd, n, _err(err, dev))
+  R.check(_entry("af_kv_fork", dev)(pt, S, W, pl, pr, refs.shape[0], page, _i32(src, (n,), "src", dev), pd, n, _err(err, dev),
+                                    _stream(table)), "af_kv_fork")
 
 
 def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
@@ -457,16 +451,16 @@ def kv_reserve(pool, table, lens, refs, slots, rows, err=None, scratch=None):
   if scratch is None:
     scratch = refs.new_empty((R.lib().af_kv_reserve_scratch_bytes(n, P) // 4 + 1,))               # int32
   scr, scr_bytes = _scratch(scratch, dev)
-  _on(dev, "af_kv_reserve", pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows", dev), n, scr,
-      scr_bytes, _err(err, dev))
+  R.check(_entry("af_kv_reserve", dev)(pool.data_ptr(), L, KV, rb, pt, S, W, pl, pr, P, page, ps, _i32(rows, (n,), "rows", dev), n,
+                                       scr, scr_bytes, _err(err, dev), _stream(table)), "af_kv_reserve")
 
 
 def kv_free(table, lens, refs, slots, page, keep=None, err=None):
   """Gives back what the slots hold past keep[i] rows (default: everything)."""
   pt, S, W, pl, pr, ps, n, dev = _book(table, lens, refs, slots)
   _need(page >= 1, "page must be positive")
-  _on(dev, "af_kv_free", pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep", dev), n,
-      _err(err, dev))
+  R.check(_entry("af_kv_free", dev)(pt, S, W, pl, pr, refs.shape[0], page, ps, 0 if keep is None else _i32(keep, (n,), "keep", dev),
+                                    n, _err(err, dev), _stream(table)), "af_kv_free")
 
 
 def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
@@ -480,6 +474,7 @@ def kv_compact(pool, table, lens, slots, path, n_path, lens_out=None, err=None):
   if lens_out is None:
     lens_out = lens.new_empty(lens.shape)
   _need(lens_out.data_ptr() != lens.data_ptr(), "lens_out must be another buffer than lens")
-  _on(dev, "af_kv_compact", pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path", dev), D,
-      _i32(n_path, (n,), "n_path", dev), n, _i32(lens_out, (S,), "lens_out", dev), _err(err, dev))
+  R.check(_entry("af_kv_compact", dev)(pool.data_ptr(), L, KV, rb, P, page, pt, S, W, pl, ps, _i32(path, (n, D), "path", dev), D,
+                                       _i32(n_path, (n,), "n_path", dev), n, _i32(lens_out, (S,), "lens_out", dev), _err(err, dev),
+                                       _stream(table)), "af_kv_compact")
   return lens_out
