@@ -43,10 +43,9 @@ AF_DEV float row_temperature(const SampleArgs& a, int r) {
 struct RowScale {
   float lmax, zmax, temp;
   AF_DEV float below(float l) const {           // z - max z, 0 for the largest
-    if (l == lmax) return 0.f;
-    if (isinf(zmax)) return __fdiv_rn(l - lmax, temp);       // the quotients overflow, of unequal logits as well
-    const float z = __fdiv_rn(l, temp);
-    return z == zmax ? 0.f : z - zmax;
+    const bool over = isinf(zmax);              // the quotients overflow, of unequal logits as well
+    const float z = __fdiv_rn(over ? l - lmax : l, temp);
+    return l == lmax ? 0.f : over ? z : z - zmax;
   }
   // whether distances to the largest logit, in units of `scale` a logit, mean nothing
   AF_DEV bool far(float scale) const {
