@@ -1,7 +1,7 @@
 // One token per row of logits: temperature, top-k, top-p and min-p, drawn with a given uniform number.
 //
 // With l the row in fp32 (NaN as -inf, -0 as +0), z = l / temperature and e = exp(z - max z), a token's
-// weight is the integer w = floor(e * 2^40): sums of weights are exact (2^40 * 2^24 tokens fit 64 bits),
+// weight is the integer w = floor(e * 2^40): sums of weights are exact (those of less than 2^24 tokens fit 64 bits),
 // so the token does not depend on how a row is split or summed. Kept are
 //   top-k   l >= the k-th largest l (ties stay);
 //   top-p   of those, in the order of falling l (ties: lowest index first), the tokens with less than
@@ -1212,7 +1212,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
     const int c = sh.where;
     for (int k = warp; k < K; k += WARPS) {
       const u64 w = warp_sum64(group(f, (c * K + k) * 32));
-      if (lane == 0) sh.radix[0][k] = w;       // K <= 128: V <= 2^24
+      if (lane == 0) sh.radix[0][k] = w;       // K <= 129 (V < 2^24) of 256 places
     }
     __syncthreads();
     if (warp == 0) {
@@ -1590,7 +1590,7 @@ static cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
 
 cudaError_t sample_launch(const SampleArgs& a, cudaStream_t st, bool pdl) {
   (void)pdl;
-  if (a.R < 0 || a.V < 1 || a.ld < a.V || a.V > (1 << 24) || a.dtype < 0 || a.dtype > 2) return cudaErrorInvalidValue;
+  if (a.R < 0 || a.V < 1 || a.ld < a.V || a.V >= (1 << 24) || a.dtype < 0 || a.dtype > 2) return cudaErrorInvalidValue;
   if (a.R == 0) return cudaSuccess;
   if (!a.logits || !a.u || !a.tok) return cudaErrorInvalidValue;
   switch (a.dtype) {

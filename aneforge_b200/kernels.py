@@ -304,7 +304,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     raise ValueError("logits must be a 2-D CUDA tensor of fp32, fp16 or bf16")
   n, V = logits.shape
   ld, col = logits.stride()
-  _need(1 <= V <= 1 << 24 and (col == 1 or V == 1), "logits must have contiguous rows of 1 to 2^24 values")
+  _need(1 <= V < 1 << 24 and (col == 1 or V == 1), "logits must have contiguous rows of 1 to 2^24 - 1 values")
   if n <= 1:
     ld = V
   _need(ld >= V, "rows of logits must not overlap")

@@ -238,7 +238,7 @@ int af_attn_decode_noalloc(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t*
                            int kv, int dh, int m, int n_split, float scale, float kv_c, int expand, int* err,
                            void* stream);
 
-/* One token per row of logits [rows][ld] (dtype 0 fp32, 1 fp16, 2 bf16; ld >= vocab, vocab <= 2^24),
+/* One token per row of logits [rows][ld] (dtype 0 fp32, 1 fp16, 2 bf16; ld >= vocab, vocab < 2^24),
  * drawn with the given uniform numbers u [rows] in [0, 1): the device form of LlamaPrefill._sample
  * (aneforge/llm.py:407-419) with min-p added. The settings are per row where their pointer is given,
  * else the scalar: temperature (<= 0: the first largest logit), top_k (<= 0 or >= vocab: off; ties with

@@ -218,3 +218,20 @@ def test_compact_refuses_more_slots_than_the_other_page_calls():
   for n in (-1, 1025):
     assert L.af_kv_compact(p, 1, 1, 128, 8, 8, p, 4, 4, p, p, p, 1, p, n, p + 64, None, None) == -1
     assert b"invalid argument" in L.af_last_error()
+
+
+def test_a_vocabulary_whose_weights_pass_64_bits_is_refused(calls):
+  """2^24 equal logits weigh 2^40 each: their sum would be 0."""
+  from aneforge_b200 import build, _runtime as R
+  u = on(0, torch.zeros(1))
+  K.sample(on(0, torch.empty(1, (1 << 24) - 1)), u)
+  with pytest.raises(ValueError):
+    K.sample(on(0, torch.empty(1, 1 << 24)), u)
+  assert len(calls.made) == 1
+  L = ctypes.CDLL(str(build.build()))
+  for name, res, args in R.SIGNATURES:
+    getattr(L, name).restype, getattr(L, name).argtypes = res, args
+  p = 1 << 20                                              # never read
+  for dtype in (0, 1, 2):
+    assert L.af_sample(p, dtype, 1 << 24, 1, 1 << 24, p, None, None, None, None, 1.0, 0, 1.0, 0.0, p, None, None) == -1
+    assert b"invalid argument" in L.af_last_error()

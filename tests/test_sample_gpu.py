@@ -323,3 +323,16 @@ def test_temperatures_near_zero(dtype, reps):
       tok, logp = run(x, np.tile(np.float32([0.0, 0.5, 0.9, 0.99, 0.2]), reps), temperature=torch.full((n,), temp).cuda(), out=out, **kw)
       assert tok.tolist() == want * reps, (temp, kw)
       assert (logp == 0).all(), (temp, kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_longest_rows(dtype):
+  """2^24 - 1 tokens that tie: sums just under 2^64."""
+  V, one = (1 << 24) - 1, 1 - 2.0 ** -24
+  x = torch.full((1, V + 3), 7.0, dtype=dtype, device="cuda")
+  for l in (x[:, :V], x[:, 3:]):                           # on a 16-byte boundary, and off one
+    for kw, n in ((dict(), V), (dict(top_p=0.5), 1 << 23), (dict(top_k=5), V), (dict(min_p=0.5), V)):
+      for u, at in ((0.0, 0), (one, n - 1)):
+        tok, logp = run(l, [u], **kw)
+        assert tok.tolist() == [at], (kw, u)
+        np.testing.assert_allclose(logp, -np.log(n), rtol=2.0 ** -18)
