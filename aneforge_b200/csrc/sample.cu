@@ -34,22 +34,29 @@ AF_DEV uint32_t key_of(float l) {
 }
 
 // a row's temperature. An infinite one would make NaN of the logits that are -inf (masked, or past the row's end): it
-// counts as the largest finite one, by which every logit under 1e30 in size still weighs as much as the largest
+// counts as the largest finite one, by which every logit under 1e30 in size still weighs as much as the largest. One
+// under 2^-124 counts as that, so that 8 / temperature is finite.
 AF_DEV float row_temperature(const SampleArgs& a, int r) {
   const float t = a.temperature ? __ldg(a.temperature + r) : a.temperature_s;
-  return t == INFINITY ? 3.402823466e38f : t;
+  return t > 0.f ? fminf(fmaxf(t, 0x1p-124f), 0x1.fffffep127f) : t;
 }
 
 struct RowScale {
   float lmax, zmax, temp;
-  AF_DEV float below(float l) const {           // z - max z, 0 for the largest
-    const bool over = isinf(zmax);              // the quotients overflow, of unequal logits as well
-    const float z = __fdiv_rn(over ? l - lmax : l, temp);
-    return l == lmax ? 0.f : over ? z : z - zmax;
+  AF_DEV void set(float largest, float t) {
+    lmax = largest;
+    temp = t > 0.f ? t : 1.f;
+    zmax = __fdiv_rn(lmax, temp);
+    // Where a finite largest logit's quotient overflows, so do those of lower ones. The nearest one is 2^-25 of it below:
+    // any power of two under 2^-32 of it, by which quotients are exact, leaves the largest all the weight as well
+    if (isinf(zmax) && !isinf(lmax)) {
+      temp = __uint_as_float((__float_as_uint(lmax) & 0x7f800000u) - (100u << 23));      // |lmax| >= 16
+      zmax = __fdiv_rn(lmax, temp);
+    }
   }
-  // whether distances to the largest logit, in units of `scale` a logit, mean nothing
-  AF_DEV bool far(float scale) const {
-    return !(zmax < 1e30f && zmax > -1e30f && lmax < 1e30f && lmax > -1e30f && scale < INFINITY);
+  AF_DEV float below(float l) const {           // z - max z, 0 for the largest (also where both are infinite)
+    const float z = __fdiv_rn(l, temp);
+    return l == lmax || z == zmax ? 0.f : z - zmax;
   }
   AF_DEV float e(float l) const { return expf(below(l)); }
   AF_DEV u64 w(float l) const { return (u64)(e(l) * 1099511627776.f); }
@@ -459,9 +466,7 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
   kmax = sh.kmax[0];
   for (int k = 1; k < C; ++k) kmax = max(kmax, sh.kmax[k]);
   RowScale sc;
-  sc.lmax = logit_of(kmax);
-  sc.temp = temp > 0.f ? temp : 1.f;
-  sc.zmax = __fdiv_rn(sc.lmax, sc.temp);
+  sc.set(logit_of(kmax), temp);
   if (sc.lmax == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.tok[r] = -1;
@@ -489,8 +494,8 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     return;
   }
   // ---- how far below the maximum the logits lie; total weight
+  const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
   const float scale = 8.f / sc.temp;
-  const bool far = sc.far(scale);
   float cut = -INFINITY;                       // no token under `cut` can be kept
   u64 total_w = 0, limit = 0;
   // e in the logits' place (past the row's end: 0)
@@ -1055,9 +1060,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
   __syncthreads();
   kmax = sh.kloc;
   RowScale sc;
-  sc.lmax = logit_of(kmax);
-  sc.temp = temp > 0.f ? temp : 1.f;
-  sc.zmax = __fdiv_rn(sc.lmax, sc.temp);
+  sc.set(logit_of(kmax), temp);
   if (sc.lmax == -INFINITY) {
     if (tid == 0) {
       a.tok[r] = -1;
@@ -1077,7 +1080,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
     }
     return;
   }
-  const bool far = sc.far(8.f / sc.temp);
+  const bool far = !(sc.zmax < 1e30f && sc.zmax > -1e30f && sc.lmax < 1e30f && sc.lmax > -1e30f);   // no distances then
   auto e_of = [&](float l) {
     if (far) return sc.e(l);
     return expf((sc.temp == 1.f ? l : __fdiv_rn(l, sc.temp)) - sc.zmax);

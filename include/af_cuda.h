@@ -241,8 +241,8 @@ int af_attn_decode_noalloc(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t*
 /* One token per row of logits [rows][ld] (dtype 0 fp32, 1 fp16, 2 bf16; ld >= vocab, vocab < 2^24),
  * drawn with the given uniform numbers u [rows] in [0, 1): the device form of LlamaPrefill._sample
  * (aneforge/llm.py:407-419) with min-p added. The settings are per row where their pointer is given,
- * else the scalar: temperature (<= 0: the first largest logit), top_k (<= 0 or >= vocab: off; ties with
- * the k-th stay), top_p (outside (0, 1): off; the token that crosses it stays), min_p (<= 0: off).
+ * else the scalar: temperature (<= 0: the first largest logit; counted as 2^-124 at least and as the
+ * largest finite number at most), top_k (<= 0 or >= vocab: off; ties with the k-th stay), top_p (outside (0, 1): off; the token that crosses it stays), min_p (<= 0: off).
  * Weights are whole numbers, so equal inputs give equal tokens however the work is split. tok [rows]:
  * -1 for a row whose logits are all -inf or NaN; logp [rows] (may be NULL): the token's log-probability
  * among the kept ones. */
