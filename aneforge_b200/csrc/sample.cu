@@ -575,8 +575,9 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
     if (before < (u64)top_k && (u64)top_k <= before + n) sh.where = tid;
     __syncthreads();
     cut = -(float)(min(sh.where, BINS - 1) + 1);             // a distance, see below; fewer than k weigh anything: all of those
+    if (sh.where == BINS && !(fabsf(sc.zmax) < 16777216.f)) cut = -INFINITY;     // z may round by nats: any may weigh something
   } else if (use_m && !use_p && !use_k && !far) {
-    cut = -(-8.f * logf(min_p) * 1.0001f + 1.f);
+    cut = -(-8.f * logf(min_p) * 1.0001f + 1.f + fabsf(sc.zmax) * 0x1p-19f);     // z rounds to 2^-24 of its size
   }
   // a token may be kept if its distance is under -cut: the same product as in the histogram
   auto may = [&](float l) { return cut == -INFINITY || (sc.lmax - l) * scale < -cut; };
@@ -1309,6 +1310,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
       if (before < (u64)top_k && (u64)top_k <= before + n) sh.where = tid;
       __syncthreads();
       cut = (float)(sh.where + 1);             // fewer than k weigh anything: all of those
+      if (all < (u64)top_k && !(fabsf(sc.zmax) < 16777216.f)) cut = INFINITY;    // z may round by nats: any may
     }
     walk([&](const float (&l)[VE], int vi) {
       float most = l[0];

@@ -336,3 +336,38 @@ def test_the_longest_rows(dtype):
         tok, logp = run(l, [u], **kw)
         assert tok.tolist() == [at], (kw, u)
         np.testing.assert_allclose(logp, -np.log(n), rtol=2.0 ** -18)
+
+
+@pytest.mark.parametrize("reps", [1, 120])
+def test_min_p_of_large_logits(reps):
+  """z = l / temperature rounds to steps of 0.5 here, so tokens of other logits have the same z as the largest: they
+  are as probable, and min-p keeps them however the row is split."""
+  lmax, temp = np.float32(3000000.25), np.float32(0.7)
+  near = lmax - np.float32(0.25) * np.arange(12, dtype=np.float32)
+  z = near / temp
+  as_good = int((z == z[0]).sum())
+  assert as_good > 1 and z.dtype == np.float32
+  l = np.full((1, 2000), 2.9e6, np.float32)
+  l[0, 500:512] = near[::-1]
+  first = 512 - as_good
+  x = torch.tensor(l).cuda().repeat(reps, 1)
+  tok, logp = run(x, [0.0] * reps, temperature=float(temp), min_p=1.0)
+  assert tok.tolist() == [first] * reps
+  np.testing.assert_allclose(logp, -np.log(as_good), atol=2.0 ** -18)
+
+
+@pytest.mark.parametrize("reps", [1, 120])
+@pytest.mark.parametrize("k", [40, 600])
+def test_top_k_of_large_quotients(k, reps):
+  """z in steps of 128: two logits whose quotients lie 68 apart round to one z, and are as probable."""
+  temp = np.float32(1.752e-9)
+  l = np.full((1, 2000), -5.0, np.float32)
+  l[0, 901] = np.float32(1.9) + np.float32(2.0 ** -22)
+  l[0, 900] = l[0, 901] - np.float32(2.0 ** -23)
+  z = l[0, 900:902] / temp
+  assert z[0] == z[1] and l[0, 900] < l[0, 901]
+  x = torch.tensor(l).cuda().repeat(reps, 1)
+  for u, at in ((0.0, 900), (0.75, 901)):
+    tok, logp = run(x, [u] * reps, temperature=float(temp), top_k=k)
+    assert tok.tolist() == [at] * reps
+    np.testing.assert_allclose(logp, -np.log(2.0), rtol=2.0 ** -18)
