@@ -1171,6 +1171,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
           weight_parts(f(l, (int)~(uint32_t)x, e_of(l)), h, g);
         }
         w += ((u64)h << 20) + g;
+        __syncwarp();                          // the places may be written again
       };
       run(c * K * 32 + lane, cell_rows(c), 32, [&](const float (&l)[VE], int vi) {
 #pragma unroll
@@ -1186,6 +1187,7 @@ __global__ void __launch_bounds__(smr::THREADS, 2) sample_wide_kernel(SampleArgs
             const u64 x = queue[32 + lane];
             __syncwarp();
             queue[lane] = x;
+            __syncwarp();                      // before another lane's next token takes a place among them
           }
         }
       });

@@ -371,3 +371,18 @@ def test_top_k_of_large_quotients(k, reps):
     tok, logp = run(x, [u] * reps, temperature=float(temp), top_k=k)
     assert tok.tolist() == [at] * reps
     np.testing.assert_allclose(logp, -np.log(2.0), rtol=2.0 ** -18)
+
+
+@pytest.mark.parametrize("V", [4099, 50257])
+def test_runs_of_heavy_tokens_among_light_ones(V):
+  """Many rows: a warp queues the tokens that can be kept, 0 to 32 of each 32 places in every order of counts."""
+  rng = np.random.default_rng(V)
+  l = np.full((100, V), -30.0, np.float32)
+  for r in range(100):
+    i = 0
+    while i < V:
+      n = int(rng.integers(0, 33))
+      at = i + rng.permutation(32)[:n]
+      l[r, at[at < V]] = rng.random((at < V).sum()).astype(np.float32)
+      i += 32
+  check(l, [[(1.0, 0, 1.0, 0.25), (1.0, 0, 0.75, 0.0), (0.75, 0, 0.5, 0.5)][r % 3] for r in range(100)], V)
