@@ -154,15 +154,16 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(AttnTreeArgs a) {
         }
         s = dot * a.scale;
       }
+      const unsigned live = __ballot_sync(0xffffffffu, p >= 0);
+      if (!live) continue;
       const float mn = fmaxf(m, warp_max(s));
-      if (mn == -INFINITY) continue;
-      const float corr = expf(m - mn);
-      const float pe = p >= 0 ? expf(s - mn) : 0.f;
+      const float mb = mn == -INFINITY ? 0.f : mn;           // only scores of -inf so far, or NaN, which stays
+      const float corr = m == -INFINITY ? 0.f : expf(m - mn);
+      const float pe = p >= 0 ? expf(s - mb) : 0.f;
       l = l * corr + warp_sum(pe);
       m = mn;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) acc[e] *= corr;
-      const unsigned live = __ballot_sync(0xffffffffu, p >= 0);
       for (int k = 0; k < 32; ++k) {
         if (!(live >> k & 1)) continue;
         const float pk = __shfl_sync(0xffffffffu, pe, k);
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(AttnTreeArgs a) {
       }
     }
   }
-  const float il = l > 0.f ? 1.f / l : 0.f;
+  const float il = l == 0.f ? 0.f : 1.f / l;   // NaN stays
   if (active)
 #pragma unroll
     for (int e = 0; e < EPL; ++e) out[lane * EPL + e] = f2h(acc[e] * il);

@@ -318,3 +318,21 @@ def test_workspace_may_hold_anything(B, T, H, KV, dh, lens, page):
     outs.append(call(d, H, KV, dh, 0.1, scratch=scratch))
   assert torch.isfinite(outs[0]).all()
   assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("dh,page", [(16, 16), (32, 5), (64, 5), (64, 16), (128, 7), (128, 64)])
+def test_nan_stays_where_nothing_finite_is_seen(dh, page):
+  """A softmax over NaN scores alone, or over a first tile of them, is NaN in every form, not zeros."""
+  d = setup(2, 3, 4, 2, dh, [0, 50], page, seed=17)
+  x = d["qkv"].view(2, 3, 8, dh)
+  x[0, 0, 4:6] = float("nan")                              # sequence 0: node 0's k, the only key that it sees
+  d["mask"][0, :, 0] = torch.tensor([1, 2, 4], dtype=torch.int32)
+  x[1, 1, 0] = float("nan")                                # sequence 1: one query head of node 1
+  out = call(d, 4, 2, dh, 0.1).view(2, 3, 4, dh)
+  assert torch.isnan(out[0, 0]).all() and torch.isfinite(out[0, 1:]).all()
+  assert torch.isnan(out[1, 1, 0]).all() and torch.isfinite(out[1, 1, 1:]).all() and torch.isfinite(out[1, ::2]).all()
+  e = setup(1, 1, 4, 2, dh, [70], page, seed=18)
+  p = int(e["table"][0, 0])
+  for r in range(32):                                      # the first 32 keys are NaN, the others are not
+    e["kc"][int(e["table"][0, r // page]), :, r % page] = float("nan")
+  assert torch.isnan(call(e, 4, 2, dh, 0.1)).all()
