@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvPagesArgs a) {
 // whether rows j, j + step, ... of a path can be taken: its nodes rise (parents come before children), its rows
 // have pages, and none of slots j, j + step, ... before it is the same one (whose block moves rows meanwhile)
 AF_DEV bool path_bad(const KvPagesArgs& a, int b, int s, int n, int len, int j, int step) {
-  bool bad = s < 0 || s >= a.S || len < 0 || n < 0 || n > a.D;
+  bool bad = s < 0 || s >= a.S || n < 0 || n > a.D;
   if (bad) return true;
   for (int k = j; k < b; k += step) bad |= a.slots[k] == s;
   const int* table = a.table + (size_t)s * a.W;
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(KvPagesArgs a) {
     const int lane = threadIdx.x & 31;
     for (int b = threadIdx.x >> 5; b < a.n; b += blockDim.x >> 5) {
       const int s = a.slots[b], n = a.rows[b], len = s >= 0 && s < a.S ? a.lens[s] : 0;
-      const bool bad = __any_sync(0xffffffffu, path_bad(a, b, s, n, len, lane, 32));
+      const bool bad = __any_sync(0xffffffffu, path_bad(a, b, s, n, max(len, 0), lane, 32)) || len < 0;
       if (lane == 0) {
         if (bad) af_set_err(a.err, AF_DEV_BAD_SLOT);
         else a.lens_out[s] = len + n;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(KvPagesArgs a) {
   const int s = a.slots[b], n = a.rows[b];
   const int len = s >= 0 && s < a.S ? a.lens[s] : 0;
   __shared__ size_t from_s[256], to_s[256];     // places of the rows, 256 at a time
-  if (__syncthreads_or(path_bad(a, b, s, n, len, threadIdx.x, blockDim.x))) return;
+  if (__syncthreads_or(path_bad(a, b, s, n, max(len, 0), threadIdx.x, blockDim.x)) || len < 0) return;
   const int* table = a.table + (size_t)s * a.W;
   const size_t head = (size_t)a.page * a.row16, pg = head * a.KV;
   uint4* plane = static_cast<uint4*>(a.pool) + (size_t)blockIdx.y * a.P * pg;
