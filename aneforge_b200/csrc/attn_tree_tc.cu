@@ -459,6 +459,7 @@ __global__ void __launch_bounds__(tt::THREADS, 1)
             *(volatile int*)&sh->holes = 1;
             af_set_err(a.err, AF_DEV_BAD_POS);
           }
+          __syncwarp();                                      // `holes` is written before the leader's next arrival
         }
         const unsigned live = (__ballot_sync(0xffffffffu, pages >= 0) >> (g * nbox)) & ((1u << nbox) - 1);
         if ((sc.t0 + j + 1) * BK > sc.len) dependency();     // the nodes' rows

@@ -336,3 +336,34 @@ def test_nan_stays_where_nothing_finite_is_seen(dh, page):
   for r in range(32):                                      # the first 32 keys are NaN, the others are not
     e["kc"][int(e["table"][0, r // page]), :, r % page] = float("nan")
   assert torch.isnan(call(e, 4, 2, dh, 0.1)).all()
+
+
+@pytest.mark.parametrize("dh,page", [(32, 16), (64, 16), (128, 16), (128, 64), (64, 5)])
+@pytest.mark.parametrize("T,H,KV", [(1, 4, 2), (9, 8, 2), (70, 4, 1), (40, 8, 1)])
+def test_pages_missing_from_a_prefix(dh, page, T, H, KV):
+  """Rows (and nodes) of pages that the table does not name, or names outside the pool, are left out and recorded."""
+  d = setup(2, T, H, KV, dh, [700, 300], page, seed=19 + T)
+  P, lost = d["kc"].shape[0], [2, 640 // page, 333 // page]
+  full = d["table"].clone()
+  d["table"][0, lost[0]], d["table"][0, lost[1]], d["table"][1, lost[2] - 40 // page] = -1, P, -5
+  gone = [[j for j in range(700 + T) if j // page in lost[:2]], [j for j in range(300 + T) if j // page == lost[2] - 40 // page]]
+  err = torch.zeros(1, dtype=torch.int32).cuda()
+  scale = dh ** -0.5
+  out = call(d, H, KV, dh, scale, err=err).double().cpu().view(2, T, H, dh)
+  assert int(err) == 2
+  kc, vc = d["kc"].double().cpu(), d["vc"].double().cpu()
+  qkv, words = d["qkv"].cpu().view(2, T, H + 2 * KV, dh), d["mask"].cpu().numpy().view(np.uint32)
+  for b, n in enumerate((700, 300)):
+    rows = [j for j in range(n) if j not in set(gone[b])]
+    at = [(int(full[b, j // page]), j % page) for j in rows]
+    x = qkv[b].half().double()
+    for h in range(KV):
+      k = torch.cat([torch.stack([kc[p, h, r] for p, r in at]), x[:, H + h]])
+      v = torch.cat([torch.stack([vc[p, h, r] for p, r in at]), x[:, H + KV + h]])
+      sees = torch.ones(T, len(rows) + T, dtype=torch.bool)
+      sees[:, len(rows):] = torch.tensor([[n + u not in gone[b] and bool(words[b, t, u // 32] >> (u % 32) & 1) for u in range(T)]
+                                          for t in range(T)])
+      for g in range(H // KV):
+        w = torch.softmax((x[:, h * (H // KV) + g] @ k.T * scale).masked_fill(~sees, float("-inf")), 1)
+        bound = (2.0 ** -10 + 2.0 ** -12) * (w @ v.abs()) + 2.0 ** -24
+        assert ((out[b, :, h * (H // KV) + g] - w @ v).abs() <= bound).all()
