@@ -13,10 +13,12 @@
 //   attn_tree    softmax(scale q k^T) v over the prefix and the visible nodes; scores, maximum, sum and
 //                output in fp32
 //
-// attn_tree_tc.cu has the second kernel for head dims 64 and 128 whose pages are of 8 rows or more (or one page a
-// sequence); the one here takes the rest: head dims 16 and 32, odd page sizes, and scales that are not positive
-// (the other's running maximum is of unscaled scores). It is the simple one, bound by its dot products: with 24
-// nodes x 4 heads at 4001 rows of 8 key heads of 128 it took 1270 us where the other takes 21 us.
+// attn_tree_tc.cu has the second kernel for head dims 64 and 128 whose pages are of a multiple of 8 rows (or one page a
+// sequence); the one here takes the rest: head dims 16 and 32, pages of 100, 37 or 4 rows and the like, and scales that
+// are not positive (the other's running maximum is of unscaled scores). It is the simple one: a warp has a query row's
+// keys to itself, 32 at a time, and is bound by their dot products one after the other. B200, 8 key heads of 128: 24
+// nodes x 4 heads at 4001 rows in pages of 100 took 1170 us (pages of 64, the other kernel: 21.6 us), 12 x 16 nodes x 8
+// heads over 2000..8000 rows 8.3 ms (63 us), one node x 4 heads at 576 rows 163 us (13.4 us).
 //
 // A table entry outside the pool ends the sequence there for reading (its rows count as masked) and is
 // recorded as an error; nothing is read or written through it.
@@ -36,7 +38,7 @@ AF_DEV int tree_page(const AttnTreeArgs& a, int b, int j) {
 }
 
 // grid (B * T, ceil((H + KV) / 8)), a warp per head; latency of one dependent chain of loads for few rows (2.8 us for
-// one node of 32 + 8 heads of 128), fp32 in and fp16 out for many (13 MB read in 8 us for 192 nodes of 64 + 8 heads)
+// one node of 32 + 8 heads of 128), fp32 in and fp16 out for many (8 MB read in 8 us for 192 nodes of 64 + 8 heads)
 template <int DH>
 __global__ void __launch_bounds__(256) tree_append_kernel(AttnTreeArgs a) {
   using HL = HeadLayout<DH>;

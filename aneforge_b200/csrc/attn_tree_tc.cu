@@ -13,7 +13,9 @@
 //                P takes S's place in tensor memory
 //   O += P V     P from tensor memory, V from shared memory as an MN-major operand
 // O is rescaled only when the maximum has risen by more than 2^8: P stays under 2^14 (weights carry a
-// factor 2^6, so that the small ones keep their bits), and the sum uses the same factor.
+// factor 2^6, so that the small ones keep their bits), and the sum uses the same factor. P in 16 bits is the price of
+// the matrix instruction: each weight is off by 2^-11 at most, the sum is of the unrounded ones, and the output's error
+// against 64 bits is 3.3e-4 to 3.6e-4 of its size where fp32 weights give 3.0e-4 (q, k, v and the output are 16 bits).
 //
 // Work split: the key tiles of all (sequence, key head) pairs in a row are cut into equal runs, one for
 // each block, whatever the sequences' lengths; a pair that was cut leaves partial (m, l, O) behind, which
@@ -31,14 +33,15 @@
 // gives up records AF_DEV_WAIT_TIMEOUT, waits for its copies and products in flight, frees its tensor memory and
 // returns.
 //
-// Bounds, and times of the three kernels together on B200 (8 key heads of 128):
-//   few rows a key     memory. 32 sequences of 8192 rows, one node, groups of 4: 172 us, 6.2 TB/s
+// Bounds, and times of the three kernels together on B200 (8 key heads of 128), 20 calls replayed from a graph:
+//   few rows a key     memory. 32 sequences of 8192 rows, one node, groups of 4: 174 us, 6.2 TB/s
 //   short or few       latency of the three launches, the copies' first tile and the join: one node at 576 rows
-//                      12.8 us, 24 nodes at 4001 rows 21 us (tree_append 2.8 and 3 of them)
-//   many rows a key    the rows' warps. 8 sequences of 32768 rows, 64 nodes x 4 heads: 315 us, 874 TFLOP/s: 1.3 us
-//                      for a tile of 64 keys and 2 x 128 rows, of which the warps of a group work 0.95 us; the
+//                      13.4 us, 24 nodes at 4001 rows 21.6 us (tree_append 2.8 and 3 of them)
+//   many rows a key    the rows' warps. 8 sequences of 32768 rows, 64 nodes x 4 heads: 313 us, 880 TFLOP/s at 1965 MHz;
+//                      called for seconds 375 to 387 us, 720 TFLOP/s: the power limit holds the clock near 1510 MHz.
+//                      1.3 us for a tile of 64 keys and 2 x 128 rows, of which the warps of a group work 0.95 us; the
 //                      products take 0.76 us at the rate of a large library product, the memory 0.74, the
-//                      exponentials alone 0.53
+//                      exponentials alone 0.53 (counters: tensor pipe 48 % of its cycles, memory 45 %, issue 42 %)
 //   pages of 16 rows   the copies: four boxes a tile. 12 sequences of 2000..8000 rows, 16 nodes x 8 heads: 77 us,
 //                      with pages of 64 rows 63 us
 // Tiles of 128 keys with one score buffer took 421 us in the third case; the second buffer keeps the products ahead

@@ -22,8 +22,8 @@
 //
 // B200, 32 layers of 8 key heads of 128, pages of 64 rows (4 KB a row and layer, K and V together): fork of one
 // sequence into three 3.7 us, the pages for their next rows 5.1 us and three copies of 33 rows 8.2 us; 56 copies of 53
-// rows (389 MB written, 56 MB of sources read) 81 us, 5.5 TB/s. Compacting 5 rows of one sequence 3.3 us, 7 rows
-// of 48 sequences in 80 layers (110 MB each way) 37.5 us, 5.9 TB/s. The small calls are bound by launches: the copies
+// rows (389 MB written, 56 MB of sources read) 81 us, 5.5 TB/s. Compacting 5 rows of one sequence 4.4 us (replayed
+// from a graph), 7 rows of 48 sequences in 80 layers (110 MB each way) 36.7 us, 6.0 TB/s. The small calls are bound by launches: the copies
 // start behind the reservation without a gap (dependent launch), and compact sets the new lengths itself.
 #include "af_common.cuh"
 #include "af_kernels.h"

@@ -74,9 +74,9 @@ struct RowScale {
 // of e (exactly: a bin's tokens share an octave, so a count and the sum of the lower bits give their
 // weight), only the bin that the limit falls into is sorted, and the kept sums come from the registers.
 // Bound by latency: a row of 0.5 MB takes 0.1 us to read, the cluster's barriers, scans and the sort take the rest.
-// B200, one row of 128256 fp32: greedy 4.2 us, plain 7.0, min-p 8.9, top-k 50 with top-p 11.9, top-k 1000 26,
-// nucleus 18.0; 16 rows of 152064 with mixed settings 35 (two blocks share an SM; top-k 1000 and the nuclei are the
-// slowest). Up to 16 blocks a row, each down to a vector a thread: a single block (below) takes 33 us for the row of top-k, 101 us for the nucleus.
+// B200, replayed from a graph, one row of 128256 fp32: greedy 4.6 us, plain 7.4, min-p 9.4, top-k 50 with top-p 12.1,
+// top-k 1000 26, nucleus 18.1; 16 rows of 152064 with mixed settings 35.5 (two blocks share an SM; top-k 1000 and the
+// nuclei are the slowest). Up to 16 blocks a row, each down to a vector a thread: a single block (below) takes 33 us for the row of top-k, 101 us for the nucleus.
 namespace smr {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 256;                      // 32 nats: what lies further below weighs nothing
@@ -959,9 +959,12 @@ __global__ void __launch_bounds__(smr::THREADS, NV * 16 / (int)sizeof(T) <= 32 ?
 // run ("cell") of the row, and the one cell that the target falls into. What does not fit its list or bin goes
 // the general way: a radix search, a pass over the row for each 8 bits.
 // B200, 256 rows of 128256 fp32 (131 MB, 20 us at the rate of a copy): greedy 25 us, min-p 65, top-k 50 with top-p
-// 71, top-k 1000 128, plain 75, nucleus 160. The first pass comes from memory at 5.3 TB/s; the passes that need every token's exact
-// e are bound by their instructions (16 warps a row, about 40 a token) and not by L2: a nucleus has one such pass
-// and one over the tokens that reach the limit's bin, which are queued so that a warp works on 32 of them.
+// 70, top-k 1000 133, plain 74, nucleus 159. The first pass comes from memory at 5.3 TB/s; the passes that need every token's exact
+// e are bound by their instructions (16 warps a row, about 40 a token) and not by L2. A nucleus walks the whole row three
+// times: maximum and an estimate of the total, with every token's approximate e; every token's exact weight, and the
+// bins; and, to sum the kept weights, every logit against the limit's bin, of which only those that reach it are queued
+// for an exact e, 32 to a warp (this walk takes about as long as the second). Counters: an instruction in 69 % of the
+// issue slots, memory at 26 %.
 namespace smw {
 constexpr int CELLS = 1024;                    // runs of 32 * K vectors
 }

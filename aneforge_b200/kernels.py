@@ -359,7 +359,8 @@ def attn_tree(qkv, kc, vc, table, lens, cos_t, sin_t, H, KV, dh, scale, mask=Non
   nodes set in mask [B, T, ceil(T / 32)] (int32 bits, see `tree_layout`; default: a chain). T = 1 is the ordinary
   decode step. nodes [B]: live nodes of each sequence. lens is left as it is (`kv_compact` advances it). Returns
   fp16 [B * T, H * dh], zeros for nodes that see nothing or are not live. err: int32 [1], zero: gets the device
-  error code of a node without a page or rotary position."""
+  error code of a node without a page or rotary position. Head dims 64 and 128 with pages of a multiple of 8 rows (or
+  W = 1) run on the tensor cores, the rest takes ten times as long and more."""
   f16 = torch.float16
   dev = qkv.get_device()
   if not (dev >= 0 and qkv.dtype == torch.float32 and qkv.dim() == 2 and table.dim() == 2):

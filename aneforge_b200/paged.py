@@ -30,7 +30,9 @@ class PagedKV:
   """`slots` sequences of at most `max_len` cache rows in `pages` pages of `page` rows each (default: enough for
   every slot to be full), for a model of cfg.n_layers layers. pool [L, 2, pages, KV, page, dh] fp16, table
   [slots, width] int32 (-1: no page), lens [slots], refs [pages]: all on the device, changed by kernels in the
-  order of the current stream. Slots and counts are lists or int32 tensors on the device."""
+  order of the current stream. Slots and counts are lists or int32 tensors on the device. Take a `page` of a multiple
+  of 8 rows, best 64 or 128: with others (and with head dims 16 and 32) attention runs without the tensor cores and
+  takes ten times as long and more."""
 
   def __init__(self, cfg, slots: int, max_len: int, pages: int | None = None, page: int = 64, device: int = 0):
     self.slots, self.page = int(slots), int(page)

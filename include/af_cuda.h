@@ -259,8 +259,9 @@ int af_sample(const void* logits, int dtype, long long ld, int rows, int vocab, 
  * node number, mask = the nodes up to itself, cos_t / sin_t = no RoPE, qn / kn = no per-head norm. A
  * node that sees nothing and nodes from nodes[b] on give zeros. dh 16, 32, 64 or 128; t <= 256. lens is
  * not changed. A row without a page, or a position past rope_rows, records AF_DEV_BAD_POS in err (may be
- * NULL) and is left out. Scratch: af_attn_tree_scratch_bytes, zero before the first call, left so that
- * the next call can use it. */
+ * NULL) and is left out. dh 64 or 128 with pages of a multiple of 8 rows (or one page a sequence) runs on
+ * the tensor cores; other pages and dh 16 / 32 take ten times as long and more. Scratch:
+ * af_attn_tree_scratch_bytes, 16-byte aligned, whatever it holds; one call at a time. */
 size_t af_attn_tree_scratch_bytes(int b, int t, int h, int kv, int dh);
 int af_attn_tree(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t* vc, long long page_stride, int n_pages, int page,
                  const int* table, int table_width, const int* lens, const int* nodes, const int* depth, const int* mask,
@@ -271,7 +272,8 @@ int af_attn_tree(const float* qkv, int ld_qkv, uint16_t* kc, uint16_t* vc, long 
 /* Pages of a cache pool [layers][2][n_pages][kv][page][row_bytes] (no counterpart in the reference, whose
  * caches are one block per sequence). Slot s holds pages table[s][0..width) (-1: none), lens[s] rows of
  * them filled; refs[p] slots hold page p. At most 1024 slots a call, all distinct; a slot out of range or
- * listed twice is left out and recorded in err (may be NULL).
+ * listed twice (its later mentions) is left out and recorded in err (may be NULL), as is a length or a
+ * reservation that the table cannot hold.
  *   af_kv_fork     dst[i] gives back its pages and shares the ones that src[i] fills; no dst is a src
  *   af_kv_reserve  rows [lens, lens + rows[i]) of each slot become its own to write: missing pages are
  *                  taken from the free ones, lowest first, and a shared page with rows in it is copied
