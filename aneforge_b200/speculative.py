@@ -127,7 +127,8 @@ def tree_generate(target: LlamaPrefill, draft: LlamaPrefill, token_ids, max_new_
   """Speculative decoding with a drafted tree: every round the draft proposes its branches[d] best tokens after
   each node of level d, the target runs the last token and the whole tree in one step and draws its own token
   after every node, the matching path is kept in both caches and its tokens and one more are emitted. The head's
-  logits are the device's. `stats` gets the number of target steps and of accepted draft tokens."""
+  logits are the device's. A model with a learned position table needs len(branches) positions past the last token.
+  `stats` gets the number of target steps and of accepted draft tokens."""
   from .paged import PagedKV, TreeStep, _stops
   prompt = [int(t) for t in token_ids]
   target._check_ids(prompt)
